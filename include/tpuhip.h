@@ -516,6 +516,68 @@ int tpuhip_quant_f32_to_i8(tpuhip_ctx *ctx, const void *x_nchw_f32, void *y, int
 int tpuhip_dequant_i8_to_f32(tpuhip_ctx *ctx, const void *x, void *y_nchw_f32, int n, int c, int h,
                              int w, int cs, float scale);
 
+/* ---- Key/value cache in 4 or 8 bits -----------------------------------------
+ * What a language model keeps of the tokens it has seen: per token and head a row of keys and one of values, quantised as
+ * they are written, read back or attended to from there.  The reference has no counterpart (it compiles networks of
+ * convolutions); the operators take the place of the fp32 products a graph would hold instead.
+ *
+ * A row x of D numbers is held as integers c of 0..L, L = 2^bits - 1, with an offset m and a step s in bfloat16:
+ *   m = the largest bfloat16 <= min(x),  s = the smallest bfloat16 >= (max(x) - m) / L (0 below 2^-126),
+ *   c = rint((x - m) / s), a tie to the even one, at most L,
+ * in 32-bit arithmetic, and stands for m + s c: every element comes back within s / 2.  A row that holds an infinity or a NaN, or
+ * whose range 32 bits do not hold, comes back as NaN as a whole, and is harmless where a mask hides it.
+ *
+ * The cache is an array of pages of page_tokens tokens each, for all kv_heads heads.  Token positions are the caller's to
+ * give out: slot = page * page_tokens + place names one of them, and a page table lists the pages of a sequence in order.
+ * Fresh pages read as zeros.  A token takes 2 * (D * bits / 8 + 4) bytes a head, with D rounded up to 64, 96, 128, 192
+ * or 256.  Everything is issued to the stream of the context that a call is given; a cache may be used from any context of its
+ * device, calls that touch the same tokens are the caller's to order.  No call allocates, and all can be captured into a
+ * graph (indexes and lengths are read on the device when the graph runs). */
+typedef struct tpuhip_kv_cache tpuhip_kv_cache;
+typedef struct {
+  int pages, page_tokens;   /* page_tokens: a multiple of 32; pages * page_tokens < 2^31 */
+  int kv_heads, head_dim;   /* head_dim: 1..256 */
+  int bits;                 /* 4 or 8 */
+} tpuhip_kv_desc;
+enum { TPUHIP_BF16 = 0, TPUHIP_F16 = 1, TPUHIP_F32 = 2 };
+/* device memory a cache takes, 0 if its sizes are refused */
+size_t tpuhip_kv_cache_bytes(const tpuhip_kv_desc *desc);
+int tpuhip_kv_cache_create(tpuhip_ctx *ctx, const tpuhip_kv_desc *desc, tpuhip_kv_cache **out);
+int tpuhip_kv_cache_destroy(tpuhip_ctx *ctx, tpuhip_kv_cache *cache);
+
+/* keys and values [tokens, kv_heads, head_dim] of one type, strides in elements, a head's numbers next to each other */
+typedef struct {
+  int tokens, dtype;
+  void *k, *v;
+  int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+} tpuhip_kv_rows;
+/* Quantises rows into the cache, row i at slots[i] (device memory).  A slot outside the cache is passed over (-1 for rows that are
+ * padding); of two rows for one slot in a call either may stay. */
+int tpuhip_kv_write(tpuhip_ctx *ctx, tpuhip_kv_cache *cache, const tpuhip_kv_rows *rows, const int32_t *slots);
+/* Reads rows back: m + s c, rounded once to the type.  Row i from slots[i]; zeros from a slot outside the cache. */
+int tpuhip_kv_read(tpuhip_ctx *ctx, const tpuhip_kv_cache *cache, const tpuhip_kv_rows *rows, const int32_t *slots);
+
+/* Attention of queries to the cache.  The queries of sequence b are rows q_starts[b] .. q_starts[b + 1] - 1 of q and stand
+ * at the end of its kv_lens[b] tokens, which the cache holds already, theirs among them: query i of n at position
+ * p = kv_lens[b] - n + i.  It sees the tokens t <= p, and with a window those of t > p - window and of t < sinks:
+ *   out = sum_t softmax_t(scale * q . K_t) V_t,
+ * zeros where nothing is seen.  Head h reads the cache's head h * kv_heads / heads.  Token t lies in page
+ * page_table[b * table_stride + t / page_tokens]; a page outside the cache holds nothing to be seen (entries before the
+ * window need not be kept).  q_starts (n_seq + 1), kv_lens (n_seq), page_table are device memory; what they say is cut to
+ * total_q, max_q queries a sequence, max_kv tokens.
+ * Softmax and sums are 32-bit.  Queries are multiplied as float16 numbers scaled by a power of two for all queries of a tile (at most 64
+ * rows of a sequence), which is exact for rows within 2^16 of each other; weights as float16 likewise. */
+typedef struct {
+  int n_seq, heads, dtype;            /* dtype of q and out: TPUHIP_BF16 or TPUHIP_F16 */
+  int total_q, max_q, max_kv;
+  int window, sinks;                  /* window 0: none */
+  int table_stride;
+  float scale;
+  int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;
+} tpuhip_kv_attention_desc;
+int tpuhip_kv_attention(tpuhip_ctx *ctx, const tpuhip_kv_cache *cache, const tpuhip_kv_attention_desc *desc, const void *q,
+                        void *out, const int32_t *q_starts, const int32_t *kv_lens, const int32_t *page_table);
+
 /* ---- module interpreter ------------------------------------------------------ */
 
 /* Flat view of the C++ ModuleInterpreter (include/tpuhip/interpreter.hpp), which

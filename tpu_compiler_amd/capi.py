@@ -62,6 +62,20 @@ class PoolDesc(C.Structure):
         "x_cs", "y_cs")]
 
 
+class KVDesc(C.Structure):
+    _fields_ = [(k, C.c_int) for k in ("pages", "page_tokens", "kv_heads", "head_dim", "bits")]
+
+
+class KVRows(C.Structure):
+    _fields_ = [("tokens", C.c_int), ("dtype", C.c_int), ("k", C.c_void_p), ("v", C.c_void_p)] + \
+        [(k, C.c_int64) for k in ("k_token_stride", "k_head_stride", "v_token_stride", "v_head_stride")]
+
+
+class KVAttentionDesc(C.Structure):
+    _fields_ = [(k, C.c_int) for k in ("n_seq", "heads", "dtype", "total_q", "max_q", "max_kv", "window", "sinks", "table_stride")] + \
+        [("scale", C.c_float)] + [(k, C.c_int64) for k in ("q_token_stride", "q_head_stride", "out_token_stride", "out_head_stride")]
+
+
 ALGO_AUTO, ALGO_DIRECT, ALGO_MFMA, ALGO_DEPTHWISE, ALGO_DEPTHWISE_DOT, ALGO_STEM = 0, 1, 2, 3, 4, 5
 
 # name -> (restype, argtypes); every symbol include/tpuhip.h declares
@@ -241,6 +255,12 @@ PROTOTYPES.update({
                                              C.c_size_t, C.POINTER(C.c_size_t)]),
     "tpuhip_quantize_lut_table": (C.c_int, [C.c_int, C.c_float, C.c_float, C.c_float, C.c_float, C.c_float,
                                             C.c_void_p]),
+    "tpuhip_kv_cache_bytes": (C.c_size_t, [C.POINTER(KVDesc)]),
+    "tpuhip_kv_cache_create": (C.c_int, [C.c_void_p, C.POINTER(KVDesc), c_void_pp]),
+    "tpuhip_kv_cache_destroy": (C.c_int, [C.c_void_p] * 2),
+    "tpuhip_kv_write": (C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(KVRows), C.c_void_p]),
+    "tpuhip_kv_read": (C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(KVRows), C.c_void_p]),
+    "tpuhip_kv_attention": (C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(KVAttentionDesc)] + [C.c_void_p] * 5),
 })
 
 
@@ -398,12 +418,15 @@ class _Ops:
 
 
 class Context:
-    """One tpuhip context (one HIP stream) with numpy conveniences."""
+    """One tpuhip context (one HIP stream) with numpy conveniences.  stream: a hipStream_t of the caller's to work on (0: the default
+    one), made by the HIP runtime that the library runs on: in a process with torch, torch's if that was imported first."""
 
-    def __init__(self, device=0):
+    def __init__(self, device=0, stream=None):
         self.lib = bind()
+        self.device = device
         h = C.c_void_p()
-        check(self.lib, self.lib.tpuhip_ctx_create(device, C.byref(h)))
+        check(self.lib, self.lib.tpuhip_ctx_create(device, C.byref(h)) if stream is None else
+              self.lib.tpuhip_ctx_create_on_stream(device, stream, C.byref(h)))
         self.h = h
         self._ops = _Ops(self.lib)
 
