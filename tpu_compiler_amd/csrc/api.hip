@@ -171,6 +171,7 @@ int tpuhip_ctx_destroy(tpuhip_ctx *ctx) {
     (void)hipStreamSynchronize(ctx->stream);
   }
   if (ctx->workspace) (void)hipFree(ctx->workspace);
+  if (ctx->join) (void)hipFree(ctx->join);
   for (auto &s : ctx->slabs) (void)hipFree(s.base);
   host_io_release(ctx);
   tpuhip_static_scratch_forget(ctx);

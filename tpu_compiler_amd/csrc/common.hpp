@@ -54,6 +54,9 @@ struct tpuhip_ctx {
   // need, replaced when a larger one comes, freed with the context; never used by a launch that is being recorded
   void *workspace = nullptr;
   size_t workspace_bytes = 0;
+  // partial sums of attention to a key/value cache whose units are split over workgroups (kv_attention.hip): of one size, made with the
+  // context's first cache or on first need, kept until the context ends, so that recorded launches may use it
+  void *join = nullptr;
   // host tensors on their way to and from the device (host/host_io.cpp): a pinned buffer of at most 32 MiB, device memory
   // for the dense form of a tensor that takes more than one piece, events behind the pieces; made on first use
   void *stage = nullptr, *landing = nullptr;

@@ -358,6 +358,8 @@ int tpuhip_kv_cache_create(tpuhip_ctx *ctx, const tpuhip_kv_desc *desc, tpuhip_k
   if (!bytes) return TPUHIP_ERR_INVALID;
   if (int rc = not_captured(ctx, "tpuhip_kv_cache_create")) return rc;
   void *data = nullptr;
+  TPUHIP_CHECK_HIP(hipSetDevice(ctx->device));
+  if (int rc = attention_workspace(ctx)) return rc;
   if (int rc = tpuhip_malloc(ctx, (size_t)bytes, &data)) return rc;
   launch(ctx, kv_clear_kernel, dim3((unsigned)std::min<int64_t>(ceil_div64(bytes / 16, 256), 8192)), dim3(256), (uint4 *)data, bytes / 16);
   const hipError_t e = hipGetLastError();

@@ -74,6 +74,9 @@ int kv_dispatch(const tpuhip_kv_cache *c, F f) {
   return set_error(TPUHIP_ERR_INVALID, "kv cache: no kernels for a head size of %d", c->desc.head_dim);
 }
 
+// kv_attention.hip: makes ctx->join if it can
+int attention_workspace(tpuhip_ctx *ctx);
+
 __device__ __forceinline__ float bf16_to_f32(uint32_t b) { return __uint_as_float(b << 16); }
 
 }  // namespace tpuhip
