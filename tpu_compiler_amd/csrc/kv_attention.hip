@@ -14,10 +14,14 @@ struct AttentionArgs {
   const uint16_t *q;
   uint16_t *out;
   float *part, *part_ml;        // of each split and row: DP sums; the maximum and the sum of the weights
+  int *counters;                // of each tile: splits that have ended; NULL: another kernel joins them
   int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;
   FastDiv group, units_per_page, kv_heads;
-  int heads, dim, pages, table_stride, rows;   // rows: of a sequence and cache head at most
+  int heads, dim, pages, table_stride;
   int total_q, max_q, max_kv, window, sinks, bf16;
+  FastDiv split_count;
+  FastDiv class_heads;          // cache heads of a class of XCDs
+  int classes, works, n_seq, one_tile;   // works: workgroups of a class
   int splits, chunk;            // a split takes `chunk` units of those that a wave's rows see
   int q_wide, out_wide;         // rows begin at dwords / at every fourth element
   float scale;
@@ -39,12 +43,62 @@ __device__ __forceinline__ uint32_t store16(float v, int bf16) {
 __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((float2v){a, b}, half2v));
 }
+// two floats past the caches that a device's XCDs have of their own
+__device__ __forceinline__ void store2(float *p, float x, float y) {
+  __hip_atomic_store((uint64_t *)p, __builtin_bit_cast(uint64_t, (float2v){x, y}), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2v load2(const float *p) {
+  return __builtin_bit_cast(float2v, __hip_atomic_load((const uint64_t *)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
 __device__ __forceinline__ float exp2_fast(float v) { return __builtin_amdgcn_exp2f(v); }
 
-// What a sequence's row of the call sees.
-struct Sequence {
-  int begin, n, first;          // its first query, how many, the position of the first
-  __device__ __forceinline__ Sequence(const AttentionArgs &a, int seq) {
+// inclusive sums over the lanes of a wave
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_add(int v) {
+  return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ int sums_upto(int v) {
+  v = dpp_add<0x111, 0xf>(v);                                  // from 1, 2, 4 and 8 lanes below in each 16,
+  v = dpp_add<0x112, 0xf>(v);
+  v = dpp_add<0x114, 0xf>(v);
+  v = dpp_add<0x118, 0xf>(v);
+  v = dpp_add<0x142, 0xa>(v);                                  // from lane 15 to 16..31 and 47 to 48..63,
+  return dpp_add<0x143, 0xc>(v);                               // from lane 31 to 32..63
+}
+
+// A tile of R rows of a sequence, the `slot`th of those of all sequences: which sequence, its first query, how many it has, the position
+// of the first.  A lane counts the tiles of a sequence; the host knows a bound of their number only, and tile is -1 where there are
+// fewer.  With one tile a sequence at most, the slot is the sequence.
+struct Tile {
+  int seq, tile, begin, n, first;
+  template <int R>
+  __device__ __forceinline__ static Tile find(const AttentionArgs &a, int slot) {
+    Tile t;
+    if (a.one_tile) {
+      t.seq = slot;
+      t.look_up(a);
+      t.tile = t.n > 0 ? 0 : -1;
+      return t;
+    }
+    for (int first = 0; first < a.n_seq; first += 64) {
+      t.seq = min(first + ((int)threadIdx.x & 63), a.n_seq - 1);
+      t.look_up(a);
+      const int tiles = first + ((int)threadIdx.x & 63) < a.n_seq ? (t.n * (int)a.group.d + R - 1) / R : 0, upto = sums_upto(tiles);
+      if (const uint64_t there = __ballot(upto > slot)) {
+        const int at = __builtin_ctzll(there);
+        return {first + at, __builtin_amdgcn_readlane(upto, at) - 1 - slot,   // the last tiles, which see the most, begin first
+                __builtin_amdgcn_readlane(t.begin, at), __builtin_amdgcn_readlane(t.n, at), __builtin_amdgcn_readlane(t.first, at)};
+      }
+      slot -= __builtin_amdgcn_readlane(upto, 63);
+    }
+    return {0, -1, 0, 0, 0};
+  }
+  // the same in all lanes, for the compiler
+  __device__ __forceinline__ Tile uniform() const {
+    return {__builtin_amdgcn_readfirstlane(seq), __builtin_amdgcn_readfirstlane(tile), __builtin_amdgcn_readfirstlane(begin),
+            __builtin_amdgcn_readfirstlane(n), __builtin_amdgcn_readfirstlane(first)};
+  }
+  __device__ __forceinline__ void look_up(const AttentionArgs &a) {
     begin = min(max(a.q_starts[seq], 0), a.total_q);
     n = min(min(max(a.q_starts[seq + 1], begin), a.total_q) - begin, a.max_q);
     first = min(max(a.kv_lens[seq], 0), a.max_kv) - n;
@@ -62,8 +116,10 @@ struct UnitList {
   __device__ __forceinline__ int block(int i) const { return i < sinks ? i : low + i - sinks; }
 };
 
-constexpr int kAttentionWaves = 4;
+constexpr int kAttentionWaves = 4, kXcds = 8;
+constexpr int kMostTokens = 1 << 30;  // of a sequence: sums and differences of two positions are ints
 constexpr float kNothing = -1e30f;   // the maximum of no scores
+constexpr int kJoinAtOnce = 8;       // splits whose sums are loaded together
 
 // A wave takes 16 NC rows (a row: a query and one of the heads that share a cache head) and units of 32 tokens:
 //   S^T = K Q^T   tokens x rows:    a lane has one row (of each 16) and the tokens 4g..4g+3, 16+4g..16+4g+3 of a unit, g = lane / 16
@@ -71,32 +127,41 @@ constexpr float kNothing = -1e30f;   // the maximum of no scores
 // The left operands are the codes themselves: masked out of a dword, two of them are a pair of subnormal float16 numbers
 // c 2^-24 (of a byte's upper half c 2^-20), which the matrix unit takes as they are and multiplies exactly.  Steps and offsets are applied to
 // what is small: x = s_t (q.c_t) + m_t sum(q) to the scores, and P'_t = p_t s_t to the weights, with sum(p_t m_t) added to all channels.
-// Four waves share a workgroup's rows (WR = 1: they take every fourth unit and join their sums in LDS) or have rows of their own (WR = 4).
+// Of a workgroup's four waves, WR have rows of their own; the 4 / WR with the same rows take every so manieth unit and join their sums in LDS.
 template <typename U, int NC, int WR>
 __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(AttentionArgs a) {
   constexpr int DP = U::kDim, KD = U::kRow / 16, STEPS = DP / 32, OB = DP / 16, WK = kAttentionWaves / WR;
-  constexpr bool IN_LDS = NC > 1;                              // the queries: read once a unit, they need no registers
+  constexpr bool IN_LDS = NC > 2;                              // the queries: read once a unit, they need no registers
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
-  const int kvh = blockIdx.y, group = (int)a.group.d;
-  const Sequence seq(a, blockIdx.z);
-  const int rows = seq.n * group, tiles = (rows + 16 * NC * WR - 1) / (16 * NC * WR);
-  // the last tiles, which see the most, begin first
-  const int tile = tiles - 1 - (int)blockIdx.x / a.splits, split = blockIdx.x % a.splits;
+  const int group = (int)a.group.d;
+  // Workgroups go to the XCDs in turn.  An XCD, or the 2, 4 or 8 of a class where there are fewer heads, takes every so manieth cache head
+  // of all sequences: an L2 holds the keys and values that the workgroups on it read at a time, and sequences of any lengths
+  // are shared out evenly.
+  const uint32_t xcd = blockIdx.x % kXcds, of_head = xcd & (a.classes - 1);
+  uint32_t work = blockIdx.x / kXcds * (kXcds / a.classes) + xcd / a.classes;
+  if (work >= (uint32_t)a.works) return;
+  uint32_t slot = a.class_heads.split(work);                   // the first tile of all heads, then the second one, ...
+  const int kvh = (int)(work * a.classes + of_head);
+  const int split = (int)(slot - a.split_count.div(slot) * a.split_count.d);
+  slot = a.split_count.div(slot);
+  const Tile seq = Tile::find<16 * NC * WR>(a, (int)slot).uniform();
+  const int tile = seq.tile, rows = seq.n * group;
   if (tile < 0) return;
-  const int row0 = (tile * WR + (WR > 1 ? wave : 0)) * 16 * NC;
-  if (row0 >= rows) return;                                    // WR > 1 only: the workgroup shares nothing
-  const int p_lo = seq.first + (int)a.group.div(row0), p_hi = seq.first + (int)a.group.div(min(row0 + 16 * NC, rows) - 1);
-  const UnitList list(a, p_lo, p_hi);
+  const int row0 = (tile * WR + wave / WK) * 16 * NC;
+  if (WK == 1 && row0 >= rows) return;                         // the waves share nothing
+  const int p_lo = seq.first + (int)a.group.div(row0), p_hi = seq.first + (int)a.group.div(max(min(row0 + 16 * NC, rows), 1) - 1);
+  const UnitList list(a, p_lo, row0 < rows ? p_hi : -1);
   int i = split * a.chunk;
   const int end = min(list.count, i + a.chunk);
-  if (split > 0 && i >= end) return;                           // no such split: the joining kernel counts them the same way
-  i += WR > 1 ? 0 : wave;
+  if (WR != 2 && split > 0 && i >= end) return;                // no such split: what joins them counts them the same way
+  const int splits = max(1, (list.count + a.chunk - 1) / a.chunk);   // that there are
+  i += wave % WK;
 
   // ---- queries
   int pos[NC];
   float q_sum[NC];
   uint4v q[NC][STEPS];
-  __shared__ uint4v q_shared[IN_LDS ? WR : 1][IN_LDS ? NC * STEPS * 64 : 1];   // WR = 1: the same from each wave
+  __shared__ uint4v q_shared[IN_LDS ? WR : 1][IN_LDS ? NC * STEPS * 64 : 1];   // the same from waves that share rows
   uint32_t most = 0;
   int e2 = 0;
 #pragma unroll
@@ -125,6 +190,66 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
       q[nc][st] = raw;
     }
   }
+  // ---- units: each lane looks up one of the wave's next 64
+  int held = 0, held_at = -64 * WK;
+  const auto unit_at = [&](int at) -> int {                    // -1: none
+    if (at >= end) return -1;
+    if (at >= held_at + 64 * WK) {
+      held_at = at;
+      const int mine = at + lane * WK;
+      held = -1;
+      if (mine < end) {
+        uint32_t in_page = list.block(mine);
+        const int page = a.table[(int64_t)seq.seq * a.table_stride + a.units_per_page.split(in_page)];
+        if ((unsigned)page < (unsigned)a.pages) held = page * (int)a.units_per_page.d + (int)in_page;
+      }
+    }
+    return __builtin_amdgcn_readlane(held, (at - held_at) / WK);
+  };
+  const auto address = [&](int unit) { return a.data + ((int64_t)max(unit, 0) * a.kv_heads.d + kvh) * U::kBytes; };
+  uint32_t k_raw[2][KD], v_raw[U::kBlocks][2], param;         // of the unit that comes next
+  const auto load_k = [&](const uint8_t *u) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t *at = (const uint32_t *)(u + (h * 16 + col) * U::kRow + g * (U::kRow / 4));
+#pragma unroll
+      for (int d = 0; d < KD; ++d) k_raw[h][d] = at[d];
+    }
+  };
+  const auto load_params = [&](const uint8_t *u) { param = ((const uint32_t *)(u + U::kParams))[lane]; };
+  const auto load_v = [&](const uint8_t *u) {
+    u += U::kCodes;
+    if constexpr (U::kPaired) {
+#pragma unroll
+      for (int b = 0; b < U::kBlocks; b += 2) {
+        const uint4v w = *(const uint4v *)(u + b / 2 * 1024 + lane * 16);
+        v_raw[b][0] = w[0], v_raw[b][1] = w[1], v_raw[b + 1][0] = w[2], v_raw[b + 1][1] = w[3];
+      }
+    } else {
+#pragma unroll
+      for (int b = 0; b < U::kBlocks; ++b) {
+        const uint2 w = *(const uint2 *)(u + b * 512 + lane * 8);
+        v_raw[b][0] = w.x, v_raw[b][1] = w.y;
+      }
+    }
+  };
+
+  // Loads are waited for in the order of their issue: params for the next unit go out when this one's have been handed on, keys when they have
+  // been multiplied, then values, each a good part of a unit's work before they are used.  The compiler has to keep the order (it would
+  // issue the params last, and wait for the values with the keys), and to read the queries from LDS where they are used.
+  const auto in_order = [] { asm volatile("" ::: "memory"); };
+  int unit = unit_at(i);
+  {
+    const uint8_t *u = address(unit);
+    load_params(u);
+    in_order();
+    load_k(u);
+    in_order();
+    load_v(u);
+    in_order();
+  }
+
+  // ---- queries as the matrix unit takes them, while the first unit is on its way
   const auto queries = [&](auto is_bf16) {
     constexpr int bf16 = decltype(is_bf16)::value;
 #pragma unroll
@@ -169,55 +294,11 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
 #pragma unroll
     for (int nc = 0; nc < NC; ++nc)
 #pragma unroll
-      for (int st = 0; st < STEPS; ++st) q_shared[WR > 1 ? wave : 0][(nc * STEPS + st) * 64 + lane] = q[nc][st];
+      for (int st = 0; st < STEPS; ++st) q_shared[wave / WK][(nc * STEPS + st) * 64 + lane] = q[nc][st];
   }
   const float log2e = 1.44269504088896341f;
   const float offset_scale = a.scale * log2e, step_scale = ldexpf(offset_scale, e2 + 24);
 
-  // ---- units: each lane looks up one of the wave's next 64
-  int held = 0, held_at = -64 * WK;
-  const auto unit_at = [&](int at) -> int {                    // -1: none
-    if (at >= end) return -1;
-    if (at >= held_at + 64 * WK) {
-      held_at = at;
-      const int mine = at + lane * WK;
-      held = -1;
-      if (mine < end) {
-        uint32_t in_page = list.block(mine);
-        const int page = a.table[(int64_t)blockIdx.z * a.table_stride + a.units_per_page.split(in_page)];
-        if ((unsigned)page < (unsigned)a.pages) held = page * (int)a.units_per_page.d + (int)in_page;
-      }
-    }
-    return __builtin_amdgcn_readlane(held, (at - held_at) / WK);
-  };
-  const auto address = [&](int unit) { return a.data + ((int64_t)max(unit, 0) * a.kv_heads.d + kvh) * U::kBytes; };
-  uint32_t k_raw[2][KD], v_raw[U::kBlocks][2];
-  uint32_t param;
-  const auto load_k = [&](const uint8_t *u) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint32_t *at = (const uint32_t *)(u + (h * 16 + col) * U::kRow + g * (U::kRow / 4));
-#pragma unroll
-      for (int d = 0; d < KD; ++d) k_raw[h][d] = at[d];
-    }
-  };
-  const auto load_params = [&](const uint8_t *u) { param = ((const uint32_t *)(u + U::kParams))[lane]; };
-  const auto load_v = [&](const uint8_t *u) {
-    u += U::kCodes;
-    if constexpr (U::kPaired) {
-#pragma unroll
-      for (int b = 0; b < U::kBlocks; b += 2) {
-        const uint4v w = *(const uint4v *)(u + b / 2 * 1024 + lane * 16);
-        v_raw[b][0] = w[0], v_raw[b][1] = w[1], v_raw[b + 1][0] = w[2], v_raw[b + 1][1] = w[3];
-      }
-    } else {
-#pragma unroll
-      for (int b = 0; b < U::kBlocks; ++b) {
-        const uint2 w = *(const uint2 *)(u + b * 512 + lane * 8);
-        v_raw[b][0] = w.x, v_raw[b][1] = w.y;
-      }
-    }
-  };
 
   // ---- the sums
   float top[NC], limit[NC], total[NC], offsets[NC];   // limit: a score above it, relative to the maximum, raises that
@@ -235,7 +316,7 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
   constexpr float kStepLimit = 1024, kLag = 5;   // weights up to 2^5 (of a maximum that lags), times steps up to 2^10: below float16's 65504
 
   __shared__ __attribute__((aligned(16))) float params[kAttentionWaves][128];
-  const int window = a.window ? a.window : INT_MAX / 2;
+  const int window = a.window ? a.window : kMostTokens;
   // A maximum or a step has gone up, which it seldom does after the first units: what has been summed, and this unit's scores, relative to
   // the new ones.
   const auto rescale = [&](float v_step, float (&high)[NC], float4v (&s)[2][NC], float (&vs)[8]) {
@@ -266,27 +347,8 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
       for (int b = 0; b < OB; ++b) o[b][nc] *= change * v_change;
     }
   };
-  const auto softmax = [&](int t0, float4v (&s)[2][NC], uint4v (&p)[NC]) {
+  const auto softmax = [&](int t0, float v_step, float (&ks)[8], float (&km)[8], float (&vs)[8], float (&vm)[8], float4v (&s)[2][NC], uint4v (&p)[NC]) {
     const bool all = t0 + kUnitTokens - 1 <= p_lo && (t0 > p_hi - window || t0 + kUnitTokens - 1 < a.sinks);
-    // a lane has the keys' (lanes 0..31) or the values' step and offset of one token; through LDS each gets those of its eight
-    float step = bf16_to_f32(param), offset = __uint_as_float(param & 0xFFFF0000);
-    if (lane < 32) {
-      step *= step_scale;
-      offset *= offset_scale;
-    } else if (t0 + lane - 32 > p_hi) {
-      step = 0;                                                 // of no token yet
-    }
-    const float v_step = lane < 32 ? 0.0f : step;
-    params[wave][lane] = lane < 32 ? step : step * v_scale;
-    params[wave][64 + lane] = offset;
-    float ks[8], km[8], vs[8], vm[8];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      *(float4v *)(ks + h * 4) = *(const float4v *)&params[wave][h * 16 + g * 4];
-      *(float4v *)(vs + h * 4) = *(const float4v *)&params[wave][32 + h * 16 + g * 4];
-      *(float4v *)(km + h * 4) = *(const float4v *)&params[wave][64 + h * 16 + g * 4];
-      *(float4v *)(vm + h * 4) = *(const float4v *)&params[wave][96 + h * 16 + g * 4];
-    }
     bool rise = v_step * v_scale > kStepLimit;
     const auto scores = [&](const float (&top)[NC]) {           // s: x - top
 #pragma unroll
@@ -298,13 +360,15 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
     scores(top);
     if (!all) {
 #pragma unroll
-      for (int nc = 0; nc < NC; ++nc)
+      for (int nc = 0; nc < NC; ++nc) {
+        const int back = pos[nc] - t0 - g * 4, first = a.sinks - t0 - g * 4;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const int t = t0 + j / 4 * 16 + g * 4 + (j & 3);
-          const bool seen = (t <= pos[nc]) & ((t > pos[nc] - window) | (t < a.sinks));
+          const int t = j / 4 * 16 + (j & 3);
+          const bool seen = ((uint32_t)(back - t) < (uint32_t)window) | ((t < first) & (t <= back));
           s[j / 4][nc][j & 3] = seen ? s[j / 4][nc][j & 3] : -INFINITY;
         }
+      }
     }
     float high[NC];
 #pragma unroll
@@ -336,16 +400,31 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
     }
   };
 
-  int unit = unit_at(i);
-  {
-    const uint8_t *u = address(unit);
-    load_k(u);
-    load_params(u);
-    load_v(u);
-  }
   for (; i < end; i += WK) {
     const int next = unit_at(i + WK);
     const uint8_t *u = address(next);
+    const int t0 = unit < 0 ? kMostTokens : list.block(i) * kUnitTokens;   // a page outside the cache: nothing is seen
+    // a lane has the keys' (lanes 0..31) or the values' step and offset of one token; through LDS each gets those of its eight
+    float step = bf16_to_f32(param), offset = __uint_as_float(param & 0xFFFF0000);
+    if (lane < 32) {
+      step *= step_scale;
+      offset *= offset_scale;
+    } else if (t0 + lane - 32 > p_hi) {
+      step = 0;                                                 // of no token yet
+    }
+    const float v_step = lane < 32 ? 0.0f : step;
+    params[wave][lane] = lane < 32 ? step : step * v_scale;
+    params[wave][64 + lane] = offset;
+    float ks[8], km[8], vs[8], vm[8];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      *(float4v *)(ks + h * 4) = *(const float4v *)&params[wave][h * 16 + g * 4];
+      *(float4v *)(vs + h * 4) = *(const float4v *)&params[wave][32 + h * 16 + g * 4];
+      *(float4v *)(km + h * 4) = *(const float4v *)&params[wave][64 + h * 16 + g * 4];
+      *(float4v *)(vm + h * 4) = *(const float4v *)&params[wave][96 + h * 16 + g * 4];
+    }
+    load_params(u);
+    in_order();
     float4v s[2][NC];
 #pragma unroll
     for (int nc = 0; nc < NC; ++nc) s[0][nc] = s[1][nc] = (float4v){0, 0, 0, 0};
@@ -364,17 +443,16 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
       }
 #pragma unroll
       for (int nc = 0; nc < NC; ++nc) {
-        const uint4v rows = IN_LDS ? q_shared[WR > 1 ? wave : 0][(nc * STEPS + st) * 64 + lane] : q[nc][st];
+        const uint4v rows = IN_LDS ? q_shared[wave / WK][(nc * STEPS + st) * 64 + lane] : q[nc][st];
 #pragma unroll
         for (int h = 0; h < 2; ++h)
           s[h][nc] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, w[h]), __builtin_bit_cast(half8, rows), s[h][nc], 0, 0, 0);
       }
     }
     load_k(u);
+    in_order();
     uint4v p[NC];
-    const int t0 = unit < 0 ? INT_MAX - kUnitTokens : list.block(i) * kUnitTokens;   // a page outside the cache: nothing is seen
-    softmax(t0, s, p);
-    load_params(u);
+    softmax(t0, v_step, ks, km, vs, vm, s, p);
 #pragma unroll
     for (int b = 0; b < U::kBlocks; ++b) {
       const uint32_t d = v_raw[b][0], f = v_raw[b][1];
@@ -392,6 +470,7 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
       }
     }
     load_v(u);
+    in_order();
     unit = next;
   }
 
@@ -411,37 +490,52 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
       for (int r = 0; r < 4; ++r) o[b][nc][r] = __builtin_fmaf(o[b][nc][r], f, offsets[nc]);
     }
   }
-  // v[0..3]: four channels of a row's result or, of several splits, of its sums
-  const auto write = [&](int row, int c0, float4v v, float high, float sum) {
-    if (row >= rows) return;
-    if (a.splits > 1) {
-      const int64_t at = ((int64_t)split * gridDim.z + blockIdx.z) * gridDim.y + kvh;
-      *(float4v *)(a.part + (at * a.rows + row) * DP + c0) = v;
-      if (c0 == 0) *(float2v *)(a.part_ml + (at * a.rows + row) * 2) = (float2v){high, sum};
-      return;
-    }
-    if (c0 >= a.dim) return;
+  const int64_t between = (int64_t)a.total_q * a.heads, first_row = ((int64_t)kvh * a.total_q + seq.begin) * group, part_row = split * between + first_row;
+  // v[0..3]: four channels of a row's sums, or its result
+  const auto keep = [&](int row, int c0, float4v v, float high, float sum) {
+    float *to = a.part + (part_row + row) * DP + c0;
+    store2(to, v[0], v[1]);
+    store2(to + 2, v[2], v[3]);
+    if (c0 == 0) store2(a.part_ml + (part_row + row) * 2, high, sum);
+  };
+  const auto result = [&](int row) {
     uint32_t h = row;
     const int token = (int)a.group.split(h);
-    uint16_t *dst = a.out + (int64_t)(seq.begin + token) * a.out_token_stride + (int64_t)(kvh * group + (int)h) * a.out_head_stride + c0;
-    const float inv = sum != 0 ? 1.0f / sum : 0.0f;
+    return a.out + (int64_t)(seq.begin + token) * a.out_token_stride + (int64_t)(kvh * group + (int)h) * a.out_head_stride;
+  };
+  const auto write = [&](uint16_t *dst, int c0, float4v v, float inv) {
     v *= inv;
+    uint32_t b[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) b[r] = store16(v[r], a.bf16);
     if (a.out_wide && c0 + 4 <= a.dim) {
-      *(uint2 *)dst = make_uint2(store16(v[0], a.bf16) | store16(v[1], a.bf16) << 16, store16(v[2], a.bf16) | store16(v[3], a.bf16) << 16);
+      *(uint2 *)(dst + c0) = make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
     } else {
 #pragma unroll
       for (int r = 0; r < 4; ++r)
-        if (c0 + r < a.dim) dst[r] = (uint16_t)store16(v[r], a.bf16);
+        if (c0 + r < a.dim) dst[c0 + r] = (uint16_t)b[r];
     }
   };
-  if constexpr (WR > 1) {
+  if constexpr (WK == 1) {
 #pragma unroll
-    for (int nc = 0; nc < NC; ++nc)
+    for (int nc = 0; nc < NC; ++nc) {
+      const int row = row0 + nc * 16 + col;
+      if (row >= rows) continue;
+      if (splits > 1) {
 #pragma unroll
-      for (int b = 0; b < OB; ++b) write(row0 + nc * 16 + col, b * 16 + g * 4, o[b][nc], top[nc], total[nc]);
+        for (int b = 0; b < OB; ++b) keep(row, b * 16 + g * 4, o[b][nc], top[nc], total[nc]);
+      } else {
+        uint16_t *dst = result(row);
+        const float inv = total[nc] != 0 ? 1.0f / total[nc] : 0.0f;
+#pragma unroll
+        for (int b = 0; b < OB; ++b) write(dst, b * 16 + g * 4, o[b][nc], inv);
+      }
+    }
   } else {
-    __shared__ float sums[WK][16][DP + 4];
-    __shared__ float tops[WK][16], totals[WK][16];
+    __shared__ float sums[kAttentionWaves][16][DP + 4];
+    __shared__ float tops[kAttentionWaves][16], totals[kAttentionWaves][16];
+    constexpr int PARTS = 16 / WR;                               // threads a row
+    const int r = threadIdx.x / PARTS % 16, first_wave = threadIdx.x / (PARTS * 16) * WK, part = threadIdx.x % PARTS;
 #pragma unroll
     for (int nc = 0; nc < NC; ++nc) {
       if (nc) __syncthreads();
@@ -452,46 +546,104 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
         totals[wave][col] = total[nc];
       }
       __syncthreads();
-      const int r = threadIdx.x >> 4, part = threadIdx.x & 15;
-      float high = tops[0][r], w[WK], sum = 0;
+      const int row = (tile * WR + first_wave / WK) * 16 * NC + nc * 16 + r;
+      if (row >= rows || split >= splits) continue;
+      float high = tops[first_wave][r], w[WK], sum = 0;
 #pragma unroll
-      for (int k = 1; k < WK; ++k) high = fmaxf(high, tops[k][r]);
+      for (int k = 1; k < WK; ++k) high = fmaxf(high, tops[first_wave + k][r]);
 #pragma unroll
       for (int k = 0; k < WK; ++k) {
-        w[k] = exp2_fast(tops[k][r] - high);
-        sum = __builtin_fmaf(totals[k][r], w[k], sum);
+        w[k] = exp2_fast(tops[first_wave + k][r] - high);
+        sum = __builtin_fmaf(totals[first_wave + k][r], w[k], sum);
       }
+      uint16_t *dst = result(row);
+      const float inv = sum != 0 ? 1.0f / sum : 0.0f;
 #pragma unroll
-      for (int c = 0; c < DP; c += 64) {
-        if (c + part * 4 >= DP) break;
+      for (int c = part * 4; c < DP; c += PARTS * 4) {
         float4v v = {0, 0, 0, 0};
 #pragma unroll
-        for (int k = 0; k < WK; ++k) v += *(const float4v *)&sums[k][r][c + part * 4] * w[k];
-        write(row0 + nc * 16 + r, c + part * 4, v, high, sum);
+        for (int k = 0; k < WK; ++k) v += *(const float4v *)&sums[first_wave + k][r][c] * w[k];
+        if (splits > 1)
+          keep(row, c, v, high, sum);
+        else
+          write(dst, c, v, inv);
       }
+    }
+    if (WR > 1 || splits == 1 || !a.counters) return;
+    // The last of a tile's splits to end joins them.  Their sums went past the caches of their XCDs (store2), so that they are where every
+    // XCD sees them when their wave's vmcnt is 0, and the counter goes up after that; they are read past the caches too.  A release and
+    // an acquire of the whole device would write back and drop an L2 for each workgroup: 28 us more for 1024 of them.
+    __shared__ int last;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    int *counter = a.counters + slot * a.kv_heads.d + kvh;
+    if (threadIdx.x == 0) {
+      const int before = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      last = before == splits - 1;
+      if (last) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // for the next call
+    }
+    __syncthreads();
+    if (!last) return;
+    constexpr int PAIRS = DP / 2;
+    for (int at = threadIdx.x; at < min(16 * NC, rows - row0) * PAIRS; at += 64 * kAttentionWaves) {
+      const int row = row0 + at / PAIRS, c = at % PAIRS * 2;
+      float high = kNothing, sum = 0;
+      float2v v = {0, 0};
+      for (int k0 = 0; k0 < splits; k0 += kJoinAtOnce) {
+        float2v ml[kJoinAtOnce], x[kJoinAtOnce];
+#pragma unroll
+        for (int k = 0; k < kJoinAtOnce; ++k) {
+          const int64_t at = first_row + min(k0 + k, splits - 1) * between + row;
+          ml[k] = load2(a.part_ml + at * 2);
+          x[k] = load2(a.part + at * DP + c);
+        }
+        float now = high;
+#pragma unroll
+        for (int k = 0; k < kJoinAtOnce; ++k) now = fmaxf(now, ml[k][0]);
+        const float change = exp2_fast(high - now);
+        high = now;
+        sum *= change;
+        v *= change;
+#pragma unroll
+        for (int k = 0; k < kJoinAtOnce; ++k) {
+          const float w = k0 + k < splits ? exp2_fast(ml[k][0] - high) : 0.0f;
+          sum = __builtin_fmaf(ml[k][1], w, sum);
+          v[0] = __builtin_fmaf(x[k][0], w, v[0]);
+          v[1] = __builtin_fmaf(x[k][1], w, v[1]);
+        }
+      }
+      uint16_t *dst = result(row) + c;
+      const float inv = sum != 0 ? 1.0f / sum : 0.0f;
+      if (c < a.dim) dst[0] = (uint16_t)store16(v[0] * inv, a.bf16);
+      if (c + 1 < a.dim) dst[1] = (uint16_t)store16(v[1] * inv, a.bf16);
     }
   }
 }
 
-// The splits of a row, joined: a wave a row, a lane a channel of each 64.
-template <typename U, int ROWS>
+// The splits of a row, joined: a workgroup a row, whose waves take every fourth split, a lane a channel of each 64.
+template <typename U, int NC, int WR>
 __global__ __launch_bounds__(256) void kv_join_kernel(AttentionArgs a) {
-  constexpr int DP = U::kDim, C = (DP + 63) / 64;
-  const int lane = threadIdx.x & 63, kvh = blockIdx.y, group = (int)a.group.d;
-  const int row = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Sequence seq(a, blockIdx.z);
-  const int rows = seq.n * group;
+  constexpr int DP = U::kDim, C = (DP + 63) / 64, WAVES = 4;
+  __shared__ float sums[WAVES][C * 64], totals[WAVES];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kvh = blockIdx.y, group = (int)a.group.d;
+  constexpr int ROWS = 16 * NC, R = ROWS * WR;
+  const Tile seq = Tile::find<R>(a, blockIdx.x / R).uniform();
+  const int tile = seq.tile;
+  if (tile < 0) return;
+  const int rows = seq.n * group, row = tile * R + (int)blockIdx.x % R;
   if (row >= rows) return;
   const int row0 = row / ROWS * ROWS;
   const UnitList list(a, seq.first + (int)a.group.div(row0), seq.first + (int)a.group.div(min(row0 + ROWS, rows) - 1));
   const int splits = max(1, (list.count + a.chunk - 1) / a.chunk);
-  const int64_t at = ((int64_t)blockIdx.z * gridDim.y + kvh) * a.rows + row, between = (int64_t)gridDim.z * gridDim.y * a.rows;
+  if (splits == 1) return;                                     // written already
+  const int64_t between = (int64_t)a.total_q * a.heads, at = ((int64_t)kvh * a.total_q + seq.begin) * group + row;
   float high = kNothing;
   for (int s = lane; s < splits; s += 64) high = fmaxf(high, a.part_ml[(at + s * between) * 2]);
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) high = fmaxf(high, __shfl_xor(high, d));
   float sum = 0, v[C] = {};
-  for (int s = 0; s < splits; ++s) {
+#pragma unroll 4
+  for (int s = wave; s < splits; s += WAVES) {
     const float2v ml = *(const float2v *)(a.part_ml + (at + s * between) * 2);
     const float w = exp2_fast(ml[0] - high);
     sum = __builtin_fmaf(ml[1], w, sum);
@@ -499,25 +651,38 @@ __global__ __launch_bounds__(256) void kv_join_kernel(AttentionArgs a) {
     for (int c = 0; c < C; ++c)
       if (DP % 64 == 0 || c * 64 + lane < DP) v[c] = __builtin_fmaf(a.part[(at + s * between) * DP + c * 64 + lane], w, v[c]);
   }
+#pragma unroll
+  for (int c = 0; c < C; ++c) sums[wave][c * 64 + lane] = v[c];
+  if (lane == 0) totals[wave] = sum;
+  __syncthreads();
+  const int c = threadIdx.x;
+  if (c >= a.dim) return;
+  sum = totals[0] + totals[1] + totals[2] + totals[3];
+  const float x = sums[0][c] + sums[1][c] + sums[2][c] + sums[3][c];
   uint32_t h = row;
   const int token = (int)a.group.split(h);
   uint16_t *dst = a.out + (int64_t)(seq.begin + token) * a.out_token_stride + (int64_t)(kvh * group + (int)h) * a.out_head_stride;
-  const float inv = sum != 0 ? 1.0f / sum : 0.0f;
-#pragma unroll
-  for (int c = 0; c < C; ++c)
-    if (c * 64 + lane < a.dim) dst[c * 64 + lane] = (uint16_t)store16(v[c] * inv, a.bf16);
+  dst[c] = (uint16_t)store16(sum != 0 ? x / sum : 0.0f, a.bf16);
 }
 
 // Splits' sums: a split of 16 rows of 128 channels takes 8 KiB, four of them on each of 256 CUs 8 MiB.
 constexpr size_t kJoinBytes = 32 << 20;
+constexpr int kCounters = 16384, kJoinInKernel = 16;   // tiles with a counter; splits up to which the last workgroup joins them
 
 int attention_workspace(tpuhip_ctx *ctx) {
   if (ctx->join) return TPUHIP_OK;
   hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
   TPUHIP_CHECK_HIP(hipStreamIsCapturing(ctx->stream, &capture));
-  if (capture != hipStreamCaptureStatusNone || hipMalloc(&ctx->join, kJoinBytes) != hipSuccess) {   // does without: one split
+  if (capture != hipStreamCaptureStatusNone || hipMalloc(&ctx->join, kCounters * 4 + kJoinBytes) != hipSuccess) {   // does without: one split
     (void)hipGetLastError();
     ctx->join = nullptr;
+    return TPUHIP_OK;
+  }
+  const hipError_t e = hipMemsetAsync(ctx->join, 0, kCounters * 4, ctx->stream);
+  if (e != hipSuccess) {
+    (void)hipFree(ctx->join);
+    ctx->join = nullptr;
+    TPUHIP_CHECK_HIP(e);
   }
   return TPUHIP_OK;
 }
@@ -541,7 +706,7 @@ int tpuhip_kv_attention(tpuhip_ctx *ctx, const tpuhip_kv_cache *cache, const tpu
   TPUHIP_REQUIRE(d->n_seq >= 0 && d->n_seq <= 65535, "%s: %d sequences", what, d->n_seq);
   TPUHIP_REQUIRE(d->total_q >= 0 && d->max_q >= 0 && d->max_kv >= 0, "%s: %d queries, at most %d a sequence, of %d tokens", what,
                  d->total_q, d->max_q, d->max_kv);
-  TPUHIP_REQUIRE((int64_t)d->max_q * d->heads <= INT_MAX / 2 && d->max_kv <= INT_MAX - 4096, "%s: %d queries of %d heads, %d tokens",
+  TPUHIP_REQUIRE((int64_t)d->max_q * d->heads <= kMostTokens / 2 && d->max_kv <= kMostTokens, "%s: %d queries of %d heads, %d tokens",
                  what, d->max_q, d->heads, d->max_kv);
   TPUHIP_REQUIRE(d->window >= 0 && d->sinks >= 0, "%s: a window of %d, %d first tokens", what, d->window, d->sinks);
   TPUHIP_REQUIRE(std::isfinite(d->scale), "%s: the scale is not finite", what);
@@ -578,24 +743,35 @@ int tpuhip_kv_attention(tpuhip_ctx *ctx, const tpuhip_kv_cache *cache, const tpu
   a.total_q = d->total_q;
   a.max_q = d->max_q < d->total_q ? d->max_q : d->total_q;
   a.max_kv = d->max_kv;
-  a.window = d->window;
-  a.sinks = d->sinks;
+  a.window = std::min(d->window, kMostTokens);
+  a.sinks = std::min(d->sinks, d->max_kv);
   a.bf16 = d->dtype == TPUHIP_BF16;
   a.scale = d->scale;
   a.q_wide = (uintptr_t)q % 4 == 0 && d->q_token_stride % 2 == 0 && d->q_head_stride % 2 == 0;
   a.out_wide = (uintptr_t)out % 8 == 0 && ts % 4 == 0 && hs % 4 == 0;
-  a.rows = a.max_q * (int)a.group.d;
+  a.n_seq = d->n_seq;
+  // The form of the kernel, R rows a workgroup: the more rows a wave has, the fewer times codes are unpacked and the fewer of the
+  // matrix unit's rows stay empty; but the workgroups have to fill the CUs.
+  const int group = (int)a.group.d, num_cu = ctx->num_cu;
+  const int64_t rows_max = (int64_t)a.max_q * group;             // of a sequence and cache head
+  const int64_t rows_all = std::min<int64_t>(rows_max * d->n_seq, (int64_t)a.total_q * group) * kv_heads;
   return kv_dispatch(cache, [&](auto u) -> int {
     using U = decltype(u);
-    constexpr int WIDE = U::kDim <= 64 ? 4 : U::kDim <= 128 ? 3 : 2;   // 16s of rows a wave: their sums take DP / 4 registers each
     const auto run = [&](auto nc, auto wr) -> int {
       constexpr int NC = decltype(nc)::value, WR = decltype(wr)::value, R = 16 * NC * WR;
-      const int tiles = (int)ceil_div64(a.rows, R);
-      // units that a tile sees at most, and how many workgroups there would be
+      a.one_tile = rows_max <= R;
+      const int64_t slots = a.one_tile ? d->n_seq : std::min(ceil_div64(rows_max, R) * d->n_seq, (int64_t)a.total_q * group / R + d->n_seq);
+      // units that a tile sees at most
       int64_t units = ceil_div64(a.max_kv, kUnitTokens);
-      if (a.window) units = std::min<int64_t>(units, ceil_div64(a.sinks, kUnitTokens) + (a.window + R / (int)a.group.d + 2) / kUnitTokens + 2);
-      const int64_t base = (int64_t)tiles * kv_heads * d->n_seq, row_bytes = (int64_t)a.rows * kv_heads * d->n_seq * (U::kDim + 2) * 4;
-      int64_t splits = std::max<int64_t>(1, std::min(ceil_div64(4 * ctx->num_cu, base), units / 16));
+      if (a.window) units = std::min<int64_t>(units, ceil_div64(a.sinks, kUnitTokens) + (a.window + R / group + 2) / kUnitTokens + 2);
+      const int64_t base = slots * kv_heads, row_bytes = (int64_t)a.total_q * a.heads * (U::kDim + 2) * 4;
+      int64_t splits = 1;
+      if (WR == 1) {
+        // two workgroups a CU, and none of more than 128 units, as lengths may differ; but a unit for each wave, and sixteen splits, which the
+        // last one joins, rather than more where these have six units a wave
+        splits = std::min(std::max(ceil_div64(2 * num_cu, base), ceil_div64(units, 128)), std::max<int64_t>(units / 2, 1));
+        if (units <= kJoinInKernel * 24) splits = std::min<int64_t>(splits, kJoinInKernel);
+      }
       splits = std::min(splits, std::max<int64_t>(1, (int64_t)kJoinBytes / row_bytes));
       if (splits > 1) {
         if (int rc = attention_workspace(ctx)) return rc;
@@ -603,21 +779,30 @@ int tpuhip_kv_attention(tpuhip_ctx *ctx, const tpuhip_kv_cache *cache, const tpu
       }
       a.chunk = (int)std::max<int64_t>(round_up((int)ceil_div64(units, splits), 4 / WR), 1);
       a.splits = (int)std::max<int64_t>(1, ceil_div64(units, a.chunk));
-      a.part_ml = (float *)ctx->join;
-      a.part = a.part_ml + (int64_t)a.splits * a.rows * kv_heads * d->n_seq * 2;
-      TPUHIP_REQUIRE((int64_t)tiles * a.splits <= INT_MAX, "%s: %d queries", what, a.max_q);
-      launch(ctx, kv_attention_kernel<U, NC, WR>, dim3((unsigned)(tiles * a.splits), (unsigned)kv_heads, (unsigned)d->n_seq),
-             dim3(64 * kAttentionWaves), a);
+      const bool in_kernel = WR == 1 && a.splits <= kJoinInKernel && base <= kCounters;
+      a.counters = in_kernel ? (int *)ctx->join : nullptr;
+      a.part_ml = (float *)((char *)ctx->join + kCounters * 4);
+      a.part = a.part_ml + (int64_t)a.splits * a.total_q * a.heads * 2;
+      a.classes = kv_heads % 8 == 0 ? 8 : kv_heads % 4 == 0 ? 4 : kv_heads % 2 == 0 ? 2 : 1;
+      a.class_heads = FastDiv(kv_heads / a.classes);
+      a.split_count = FastDiv(a.splits);
+      const int64_t works = slots * a.splits * (kv_heads / a.classes);
+      TPUHIP_REQUIRE(works * a.classes < INT_MAX - kXcds && slots * R <= INT_MAX, "%s: %d queries of %d sequences", what, a.total_q, d->n_seq);
+      a.works = (int)works;
+      launch(ctx, kv_attention_kernel<U, NC, WR>, dim3((unsigned)(ceil_div64(works, kXcds / a.classes) * kXcds)), dim3(64 * kAttentionWaves), a);
       TPUHIP_CHECK_HIP(hipGetLastError());
-      if (a.splits > 1) {
-        launch(ctx, kv_join_kernel<U, 16 * NC>, dim3((unsigned)ceil_div64(a.rows, 4), (unsigned)kv_heads, (unsigned)d->n_seq), dim3(256), a);
+      if (a.splits > 1 && !in_kernel) {
+        launch(ctx, kv_join_kernel<U, NC, WR>, dim3((unsigned)(slots * R), (unsigned)kv_heads), dim3(256), a);
         TPUHIP_CHECK_HIP(hipGetLastError());
       }
       return TPUHIP_OK;
     };
     using std::integral_constant;
-    if (a.rows <= 16) return run(integral_constant<int, 1>{}, integral_constant<int, 1>{});
-    if (a.rows <= 16 * WIDE) return run(integral_constant<int, WIDE>{}, integral_constant<int, 1>{});
+    constexpr int WIDE = U::kDim <= 128 ? 2 : 1;   // 16s of rows a wave: their sums take DP / 4 registers each
+    const auto enough = [&](int r, int a_cu) { return ceil_div64(rows_all, r) >= (int64_t)a_cu * num_cu; };
+    if (WIDE > 1 && rows_max <= 16) return run(integral_constant<int, 1>{}, integral_constant<int, 1>{});
+    if (rows_max <= 16 * WIDE || !enough(32 * WIDE, 1)) return run(integral_constant<int, WIDE>{}, integral_constant<int, 1>{});
+    if (!enough(64 * WIDE, 4)) return run(integral_constant<int, WIDE>{}, integral_constant<int, 2>{});
     return run(integral_constant<int, WIDE>{}, integral_constant<int, 4>{});
   });
 }
