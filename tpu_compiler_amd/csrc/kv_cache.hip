@@ -44,6 +44,7 @@ struct RowsArgs {
   int64_t token_stride[2], head_stride[2];
   FastDiv head_count;
   int tokens, heads, dim, most; // slots below `most` exist
+  int half;                     // few workgroups: so many take whole units and as many what is left; 0: each takes both
   int dwords, wide;             // rows begin at dwords; and all DP elements are there
 };
 
@@ -236,7 +237,8 @@ __global__ __launch_bounds__(kRowsThreads) void kv_write_kernel(RowsArgs a) {
   __shared__ __attribute__((aligned(16))) uint8_t keys[U::kCodes], values[kUnitTokens * STRIDE];
   __shared__ __attribute__((aligned(16))) uint32_t params[2 * kUnitTokens];
   __shared__ int slots[kUnitTokens];
-  uint32_t at_head = blockIdx.x;                               // the heads of a token next to each other, as in memory
+  const bool second = a.half && blockIdx.x >= (unsigned)a.half;
+  uint32_t at_head = second ? blockIdx.x - a.half : blockIdx.x;   // the heads of a token next to each other, as in memory
   const int first = (int)a.head_count.split(at_head) * kUnitTokens, head = (int)at_head;
   const int t = threadIdx.x & (kRowThreads - 1), row = threadIdx.x / kRowThreads;
   T raw[2][2 * E];
@@ -259,8 +261,8 @@ __global__ __launch_bounds__(kRowsThreads) void kv_write_kernel(RowsArgs a) {
     }
   };
   const Runs runs(a, first);
-  for (int whole = runs.start >= 0; whole >= 0; --whole) {
-    if (!whole && !runs.left) return;
+  for (int whole = runs.start >= 0 && !second; whole >= 0; --whole) {
+    if (!whole && (!runs.left || (a.half && !second))) return;
     load(whole ? runs.start : first);
     int slot = runs.slot_of(whole, row);
     if (!whole && !(runs.left >> row & 1)) slot = -1;
@@ -365,12 +367,13 @@ template <typename U, typename T, bool WIDE>
 __global__ __launch_bounds__(kRowsThreads) void kv_read_kernel(RowsArgs a) {
   constexpr int E = U::kDim / 16, HALF = U::kDim / 2, B = E * U::kBits / 8, STRIDE = ValueColumns<U>::kStride;
   __shared__ __attribute__((aligned(16))) uint8_t values[kUnitTokens * STRIDE];
-  uint32_t at_head = blockIdx.x;                               // the heads of a token next to each other, as in memory
+  const bool second = a.half && blockIdx.x >= (unsigned)a.half;
+  uint32_t at_head = second ? blockIdx.x - a.half : blockIdx.x;   // the heads of a token next to each other, as in memory
   const int first = (int)a.head_count.split(at_head) * kUnitTokens, head = (int)at_head;
   const int t = threadIdx.x & (kRowThreads - 1), row = threadIdx.x / kRowThreads;
   const Runs runs(a, first);
-  for (int whole = runs.start >= 0; whole >= 0; --whole) {
-    if (!whole && !runs.left) return;
+  for (int whole = runs.start >= 0 && !second; whole >= 0; --whole) {
+    if (!whole && (!runs.left || (a.half && !second))) return;
     const int at = (whole ? runs.start : first) + row;
     const bool there = whole || (runs.left >> row & 1);
     const int slot = runs.slot_of(whole, row);
@@ -491,6 +494,13 @@ static int rows_args(tpuhip_ctx *ctx, const tpuhip_kv_cache *c, const tpuhip_kv_
   return TPUHIP_OK;
 }
 
+// workgroups of a launch
+static int64_t rows_blocks(const tpuhip_ctx *ctx, RowsArgs *a) {
+  const int64_t blocks = ceil_div64(a->tokens, kUnitTokens) * a->heads;
+  a->half = a->tokens >= kUnitTokens && blocks <= 2 * ctx->num_cu ? (int)blocks : 0;
+  return a->half ? 2 * blocks : blocks;
+}
+
 }  // namespace tpuhip
 
 using namespace tpuhip;
@@ -541,13 +551,14 @@ int tpuhip_kv_write(tpuhip_ctx *ctx, tpuhip_kv_cache *cache, const tpuhip_kv_row
   if (a.tokens == 0) return TPUHIP_OK;
   return kv_dispatch(cache, [&](auto u) -> int {
     using U = decltype(u);
+    const int64_t blocks = rows_blocks(ctx, &a);
     const auto pick = [&](auto wide) {
       constexpr bool W = decltype(wide)::value;
       return rows->dtype == TPUHIP_BF16 ? kv_write_kernel<U, Bf16, W>
              : rows->dtype == TPUHIP_F16 ? kv_write_kernel<U, _Float16, W> : kv_write_kernel<U, float, W>;
     };
     const auto kernel = a.wide ? pick(std::true_type{}) : pick(std::false_type{});
-    launch(ctx, kernel, dim3((unsigned)(ceil_div64(a.tokens, kUnitTokens) * a.heads)), dim3(kRowsThreads), a);
+    launch(ctx, kernel, dim3((unsigned)blocks), dim3(kRowsThreads), a);
     TPUHIP_CHECK_HIP(hipGetLastError());
     return TPUHIP_OK;
   });
@@ -559,13 +570,14 @@ int tpuhip_kv_read(tpuhip_ctx *ctx, const tpuhip_kv_cache *cache, const tpuhip_k
   if (a.tokens == 0) return TPUHIP_OK;
   return kv_dispatch(cache, [&](auto u) -> int {
     using U = decltype(u);
+    const int64_t blocks = rows_blocks(ctx, &a);
     const auto pick = [&](auto wide) {
       constexpr bool W = decltype(wide)::value;
       return rows->dtype == TPUHIP_BF16 ? kv_read_kernel<U, Bf16, W>
              : rows->dtype == TPUHIP_F16 ? kv_read_kernel<U, _Float16, W> : kv_read_kernel<U, float, W>;
     };
     const auto kernel = a.wide ? pick(std::true_type{}) : pick(std::false_type{});
-    launch(ctx, kernel, dim3((unsigned)(ceil_div64(a.tokens, kUnitTokens) * a.heads)), dim3(kRowsThreads), a);
+    launch(ctx, kernel, dim3((unsigned)blocks), dim3(kRowsThreads), a);
     TPUHIP_CHECK_HIP(hipGetLastError());
     return TPUHIP_OK;
   });
