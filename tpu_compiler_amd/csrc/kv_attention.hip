@@ -131,7 +131,6 @@ constexpr int kJoinAtOnce = 8;       // splits whose sums are loaded together
 template <typename U, int NC, int WR>
 __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(AttentionArgs a) {
   constexpr int DP = U::kDim, KD = U::kRow / 16, STEPS = DP / 32, OB = DP / 16, WK = kAttentionWaves / WR;
-  constexpr bool IN_LDS = NC > 2;                              // the queries: read once a unit, they need no registers
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
   const int group = (int)a.group.d;
   // Workgroups go to the XCDs in turn.  An XCD, or the 2, 4 or 8 of a class where there are fewer heads, takes every so manieth cache head
@@ -161,7 +160,6 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
   int pos[NC];
   float q_sum[NC];
   uint4v q[NC][STEPS];
-  __shared__ uint4v q_shared[IN_LDS ? WR : 1][IN_LDS ? NC * STEPS * 64 : 1];   // the same from waves that share rows
   uint32_t most = 0;
   int e2 = 0;
 #pragma unroll
@@ -236,7 +234,7 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
 
   // Loads are waited for in the order of their issue: params for the next unit go out when this one's have been handed on, keys when they have
   // been multiplied, then values, each a good part of a unit's work before they are used.  The compiler has to keep the order (it would
-  // issue the params last, and wait for the values with the keys), and to read the queries from LDS where they are used.
+  // issue the params last, and wait for the values with the keys).
   const auto in_order = [] { asm volatile("" ::: "memory"); };
   int unit = unit_at(i);
   {
@@ -289,12 +287,6 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
   for (int nc = 0; nc < NC; ++nc) {
     q_sum[nc] += __shfl_xor(q_sum[nc], 16);
     q_sum[nc] += __shfl_xor(q_sum[nc], 32);
-  }
-  if constexpr (IN_LDS) {
-#pragma unroll
-    for (int nc = 0; nc < NC; ++nc)
-#pragma unroll
-      for (int st = 0; st < STEPS; ++st) q_shared[wave / WK][(nc * STEPS + st) * 64 + lane] = q[nc][st];
   }
   const float log2e = 1.44269504088896341f;
   const float offset_scale = a.scale * log2e, step_scale = ldexpf(offset_scale, e2 + 24);
@@ -443,16 +435,19 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
       }
 #pragma unroll
       for (int nc = 0; nc < NC; ++nc) {
-        const uint4v rows = IN_LDS ? q_shared[wave / WK][(nc * STEPS + st) * 64 + lane] : q[nc][st];
 #pragma unroll
         for (int h = 0; h < 2; ++h)
-          s[h][nc] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, w[h]), __builtin_bit_cast(half8, rows), s[h][nc], 0, 0, 0);
+          s[h][nc] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, w[h]), __builtin_bit_cast(half8, q[nc][st]), s[h][nc], 0, 0, 0);
       }
     }
     load_k(u);
     in_order();
+    // bound by the vector ALU: a wave with scores to work on goes before one that feeds the matrix unit, and products of values, which
+    // end its unit, before those of keys (a prompt of 8192 tokens: 595 us without, 582 with)
+    __builtin_amdgcn_s_setprio(2);
     uint4v p[NC];
     softmax(t0, v_step, ks, km, vs, vm, s, p);
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int b = 0; b < U::kBlocks; ++b) {
       const uint32_t d = v_raw[b][0], f = v_raw[b][1];
@@ -469,6 +464,7 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
               __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, x), __builtin_bit_cast(half8, p[nc]), o[OB / 2 + b][nc], 0, 0, 0);
       }
     }
+    __builtin_amdgcn_s_setprio(0);
     load_v(u);
     in_order();
     unit = next;
