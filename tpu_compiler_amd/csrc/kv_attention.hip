@@ -23,7 +23,6 @@ struct AttentionArgs {
   FastDiv class_heads;          // cache heads of a class of XCDs
   int classes, works, n_seq, one_tile;   // works: workgroups of a class
   int splits, chunk;            // a split takes `chunk` units of those that a wave's rows see
-  int q_wide, out_wide;         // rows begin at dwords / at every fourth element
   float scale;
 };
 
@@ -32,7 +31,8 @@ typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef float float2v __attribute__((ext_vector_type(2)));
 typedef float float4v __attribute__((ext_vector_type(4)));
 typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
-typedef uint32_t uint4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t uint2u __attribute__((ext_vector_type(2), aligned(2)));
+typedef uint32_t uint4u __attribute__((ext_vector_type(4), aligned(2)));   // memory takes any address
 
 __device__ __forceinline__ float load16(uint32_t b, int bf16) {
   return bf16 ? bf16_to_f32(b & 0xFFFF) : (float)__builtin_bit_cast(_Float16, (uint16_t)b);
@@ -120,6 +120,7 @@ constexpr int kAttentionWaves = 4, kXcds = 8;
 constexpr int kMostTokens = 1 << 30;  // of a sequence: sums and differences of two positions are ints
 constexpr float kNothing = -1e30f;   // the maximum of no scores
 constexpr int kJoinAtOnce = 8;       // splits whose sums are loaded together
+constexpr int kJoinWaves = 16;
 
 // A wave takes 16 NC rows (a row: a query and one of the heads that share a cache head) and units of 32 tokens:
 //   S^T = K Q^T   tokens x rows:    a lane has one row (of each 16) and the tokens 4g..4g+3, 16+4g..16+4g+3 of a unit, g = lane / 16
@@ -160,7 +161,7 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
   int pos[NC];
   float q_sum[NC];
   uint4v q[NC][STEPS];
-  uint32_t most = 0;
+  float most = 0;
   int e2 = 0;
 #pragma unroll
   for (int nc = 0; nc < NC; ++nc) {
@@ -175,7 +176,7 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
       const int c0 = g * (DP / 4) + st * 8;
       uint4v raw = {0, 0, 0, 0};
       if (valid && c0 < a.dim) {
-        if (a.q_wide && c0 + 8 <= a.dim) {
+        if (c0 + 8 <= a.dim) {
           raw = *(const uint4u *)(src + c0);
         } else {
 #pragma unroll
@@ -258,14 +259,26 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
         for (int e = 0; e < 8; ++e) {
           const float v = load16(q[nc][st][e / 2] >> 16 * (e & 1), bf16);
           q_sum[nc] += v;
-          const uint32_t size = __float_as_uint(v) & 0x7FFFFFFF;
-          most = size < 0x7F800000 ? max(most, size) : most;
+          most = fmaxf(most, fabsf(v));
         }
+    if (__any(!(most <= __FLT_MAX__))) {                        // infinities, which are not to count; NaN does not
+      most = 0;
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) most = max(most, (uint32_t)__shfl_xor((int)most, d));
+      for (int nc = 0; nc < NC; ++nc)
+#pragma unroll
+        for (int st = 0; st < STEPS; ++st)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float v = fabsf(load16(q[nc][st][e / 2] >> 16 * (e & 1), bf16));
+            most = v <= __FLT_MAX__ ? fmaxf(most, v) : most;
+          }
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) most = fmaxf(most, __shfl_xor(most, d));
     // the wave's queries times one power of two, the largest number just below 2^15: float16 holds bfloat16's 8 bits of all that are
     // within 2^29 of it.  A number past the bounds of the exponent becomes an infinity, in its own row.
-    e2 = min(max((int)(most >> 23) - 127 - 14, -100), 88);
+    e2 = min(max((int)(__float_as_uint(most) >> 23) - 127 - 14, -100), 88);
+    const float down = __uint_as_float((uint32_t)(127 - e2) << 23);
 #pragma unroll
     for (int nc = 0; nc < NC; ++nc)
 #pragma unroll
@@ -273,7 +286,7 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
         float v[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e)   // odd channels lie in the upper halves of 4-bit bytes, 16 times their size
-          v[e] = ldexpf(load16(q[nc][st][e / 2] >> 16 * (e & 1), bf16), U::kBits == 4 && e & 1 ? -e2 - 4 : -e2);
+          v[e] = load16(q[nc][st][e / 2] >> 16 * (e & 1), bf16) * (U::kBits == 4 && e & 1 ? down / 16 : down);
         // in the order of the codes' pairs
         q[nc][st] = U::kBits == 4 ? (uint4v){pack_f16(v[0], v[4]), pack_f16(v[1], v[5]), pack_f16(v[2], v[6]), pack_f16(v[3], v[7])}
                                   : (uint4v){pack_f16(v[0], v[2]), pack_f16(v[1], v[3]), pack_f16(v[4], v[6]), pack_f16(v[5], v[7])};
@@ -504,8 +517,8 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
     uint32_t b[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) b[r] = store16(v[r], a.bf16);
-    if (a.out_wide && c0 + 4 <= a.dim) {
-      *(uint2 *)(dst + c0) = make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
+    if (c0 + 4 <= a.dim) {
+      *(uint2u *)(dst + c0) = (uint2u){b[0] | b[1] << 16, b[2] | b[3] << 16};
     } else {
 #pragma unroll
       for (int r = 0; r < 4; ++r)
@@ -580,18 +593,19 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
     }
     __syncthreads();
     if (!last) return;
-    constexpr int PAIRS = DP / 2;
-    for (int at = threadIdx.x; at < min(16 * NC, rows - row0) * PAIRS; at += 64 * kAttentionWaves) {
-      const int row = row0 + at / PAIRS, c = at % PAIRS * 2;
+    constexpr int FOURS = DP / 4;
+    for (int at = threadIdx.x; at < min(16 * NC, rows - row0) * FOURS; at += 64 * kAttentionWaves) {
+      const int row = row0 + at / FOURS, c = at % FOURS * 4;
       float high = kNothing, sum = 0;
-      float2v v = {0, 0};
+      float4v v = {0, 0, 0, 0};
       for (int k0 = 0; k0 < splits; k0 += kJoinAtOnce) {
-        float2v ml[kJoinAtOnce], x[kJoinAtOnce];
+        float2v ml[kJoinAtOnce], x[kJoinAtOnce], y[kJoinAtOnce];
 #pragma unroll
         for (int k = 0; k < kJoinAtOnce; ++k) {
-          const int64_t at = first_row + min(k0 + k, splits - 1) * between + row;
-          ml[k] = load2(a.part_ml + at * 2);
-          x[k] = load2(a.part + at * DP + c);
+          const int64_t from = first_row + min(k0 + k, splits - 1) * between + row;
+          ml[k] = load2(a.part_ml + from * 2);
+          x[k] = load2(a.part + from * DP + c);
+          y[k] = load2(a.part + from * DP + c + 2);
         }
         float now = high;
 #pragma unroll
@@ -606,20 +620,19 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
           sum = __builtin_fmaf(ml[k][1], w, sum);
           v[0] = __builtin_fmaf(x[k][0], w, v[0]);
           v[1] = __builtin_fmaf(x[k][1], w, v[1]);
+          v[2] = __builtin_fmaf(y[k][0], w, v[2]);
+          v[3] = __builtin_fmaf(y[k][1], w, v[3]);
         }
       }
-      uint16_t *dst = result(row) + c;
-      const float inv = sum != 0 ? 1.0f / sum : 0.0f;
-      if (c < a.dim) dst[0] = (uint16_t)store16(v[0] * inv, a.bf16);
-      if (c + 1 < a.dim) dst[1] = (uint16_t)store16(v[1] * inv, a.bf16);
+      write(result(row), c, v, sum != 0 ? 1.0f / sum : 0.0f);
     }
   }
 }
 
-// The splits of a row, joined: a workgroup a row, whose waves take every fourth split, a lane a channel of each 64.
+// The splits of a row, joined: a workgroup a row, whose waves take every sixteenth split, a lane a channel of each 64.
 template <typename U, int NC, int WR>
-__global__ __launch_bounds__(256) void kv_join_kernel(AttentionArgs a) {
-  constexpr int DP = U::kDim, C = (DP + 63) / 64, WAVES = 4;
+__global__ __launch_bounds__(64 * kJoinWaves) void kv_join_kernel(AttentionArgs a) {
+  constexpr int DP = U::kDim, C = (DP + 63) / 64, WAVES = kJoinWaves;
   __shared__ float sums[WAVES][C * 64], totals[WAVES];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kvh = blockIdx.y, group = (int)a.group.d;
   constexpr int ROWS = 16 * NC, R = ROWS * WR;
@@ -653,8 +666,13 @@ __global__ __launch_bounds__(256) void kv_join_kernel(AttentionArgs a) {
   __syncthreads();
   const int c = threadIdx.x;
   if (c >= a.dim) return;
-  sum = totals[0] + totals[1] + totals[2] + totals[3];
-  const float x = sums[0][c] + sums[1][c] + sums[2][c] + sums[3][c];
+  sum = 0;
+  float x = 0;
+#pragma unroll
+  for (int k = 0; k < WAVES; ++k) {
+    sum += totals[k];
+    x += sums[k][c];
+  }
   uint32_t h = row;
   const int token = (int)a.group.split(h);
   uint16_t *dst = a.out + (int64_t)(seq.begin + token) * a.out_token_stride + (int64_t)(kvh * group + (int)h) * a.out_head_stride;
@@ -743,8 +761,6 @@ int tpuhip_kv_attention(tpuhip_ctx *ctx, const tpuhip_kv_cache *cache, const tpu
   a.sinks = std::min(d->sinks, d->max_kv);
   a.bf16 = d->dtype == TPUHIP_BF16;
   a.scale = d->scale;
-  a.q_wide = (uintptr_t)q % 4 == 0 && d->q_token_stride % 2 == 0 && d->q_head_stride % 2 == 0;
-  a.out_wide = (uintptr_t)out % 8 == 0 && ts % 4 == 0 && hs % 4 == 0;
   a.n_seq = d->n_seq;
   // The form of the kernel, R rows a workgroup: the more rows a wave has, the fewer times codes are unpacked and the fewer of the
   // matrix unit's rows stay empty; but the workgroups have to fill the CUs.
@@ -763,10 +779,11 @@ int tpuhip_kv_attention(tpuhip_ctx *ctx, const tpuhip_kv_cache *cache, const tpu
       const int64_t base = slots * kv_heads, row_bytes = (int64_t)a.total_q * a.heads * (U::kDim + 2) * 4;
       int64_t splits = 1;
       if (WR == 1) {
-        // two workgroups a CU, and none of more than 128 units, as lengths may differ; but a unit for each wave, and sixteen splits, which the
-        // last one joins, rather than more where these have six units a wave
-        splits = std::min(std::max(ceil_div64(2 * num_cu, base), ceil_div64(units, 128)), std::max<int64_t>(units / 2, 1));
-        if (units <= kJoinInKernel * 24) splits = std::min<int64_t>(splits, kJoinInKernel);
+        // Two workgroups a CU, and none of more than 128 units, as lengths may differ; but two units a wave at least, four with twice the
+        // rows, for a join takes as long (a wave takes 1 us a unit, the join of two splits 1.6), and so few splits that the last one can
+        // join them rather than another kernel, where these have six units a wave at most.
+        splits = std::min(std::max(ceil_div64(2 * num_cu, base), ceil_div64(units, 128)), ceil_div64(units, 8 * NC));
+        if (units <= kJoinInKernel * 24) splits = std::min<int64_t>(splits, kJoinInKernel / NC);
       }
       splits = std::min(splits, std::max<int64_t>(1, (int64_t)kJoinBytes / row_bytes));
       if (splits > 1) {
@@ -788,7 +805,7 @@ int tpuhip_kv_attention(tpuhip_ctx *ctx, const tpuhip_kv_cache *cache, const tpu
       launch(ctx, kv_attention_kernel<U, NC, WR>, dim3((unsigned)(ceil_div64(works, kXcds / a.classes) * kXcds)), dim3(64 * kAttentionWaves), a);
       TPUHIP_CHECK_HIP(hipGetLastError());
       if (a.splits > 1 && !in_kernel) {
-        launch(ctx, kv_join_kernel<U, NC, WR>, dim3((unsigned)(slots * R), (unsigned)kv_heads), dim3(256), a);
+        launch(ctx, kv_join_kernel<U, NC, WR>, dim3((unsigned)(slots * R), (unsigned)kv_heads), dim3(64 * kJoinWaves), a);
         TPUHIP_CHECK_HIP(hipGetLastError());
       }
       return TPUHIP_OK;

@@ -25,16 +25,22 @@ __device__ __forceinline__ Bf16 from_f32<Bf16>(float v) {
   return {__builtin_bit_cast(uint16_t, (__bf16)v)};
 }
 
-// E elements from or to memory that is aligned to a dword
+// Bytes between registers and LDS or memory, by sixteen as far as that goes: at dwords, or (rows of any stride) at any element
 typedef uint32_t dwords4 __attribute__((ext_vector_type(4), aligned(4)));
-template <int BYTES>
+typedef uint32_t row_dwords4 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t row_dword __attribute__((aligned(2)));
+template <int BYTES, typename V = dwords4, typename D = uint32_t>
 __device__ __forceinline__ void copy_dwords(void *dst, const void *src) {
   static_assert(BYTES % 4 == 0);
   constexpr int full = BYTES / 16;
 #pragma unroll
-  for (int i = 0; i < full; ++i) ((dwords4 *)dst)[i] = ((const dwords4 *)src)[i];
+  for (int i = 0; i < full; ++i) ((V *)dst)[i] = ((const V *)src)[i];
 #pragma unroll
-  for (int i = full * 4; i < BYTES / 4; ++i) ((uint32_t *)dst)[i] = ((const uint32_t *)src)[i];
+  for (int i = full * 4; i < BYTES / 4; ++i) ((D *)dst)[i] = ((const D *)src)[i];
+}
+template <int BYTES>
+__device__ __forceinline__ void copy_row(void *dst, const void *src) {
+  copy_dwords<BYTES, row_dwords4, row_dword>(dst, src);
 }
 
 struct RowsArgs {
@@ -45,7 +51,7 @@ struct RowsArgs {
   FastDiv head_count;
   int tokens, heads, dim, most; // slots below `most` exist
   int half;                     // few workgroups: so many take whole units and as many what is left; 0: each takes both
-  int dwords, wide;             // rows begin at dwords; and all DP elements are there
+  int wide;                     // all DP elements are there
 };
 
 // A workgroup takes 32 rows of one head, keys and values: eight threads a row, each with DP/16 channels of its lower half and as many
@@ -250,8 +256,8 @@ __global__ __launch_bounds__(kRowsThreads) void kv_write_kernel(RowsArgs a) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int c0 = h * HALF + t * E;
-        if (WIDE || (a.dwords && c0 + E <= a.dim)) {
-          copy_dwords<E * sizeof(T)>(raw[kv] + h * E, src + c0);
+        if (WIDE || c0 + E <= a.dim) {
+          copy_row<E * sizeof(T)>(raw[kv] + h * E, src + c0);
         } else {
           const int c = here(c0);
 #pragma unroll
@@ -415,8 +421,8 @@ __global__ __launch_bounds__(kRowsThreads) void kv_read_kernel(RowsArgs a) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int c0 = h * HALF + t * E;
-        if (WIDE || (a.dwords && c0 + E <= a.dim)) {
-          copy_dwords<E * sizeof(T)>(dst + c0, raw + h * E);
+        if (WIDE || c0 + E <= a.dim) {
+          copy_row<E * sizeof(T)>(dst + c0, raw + h * E);
         } else {
           const int c = here(c0);
 #pragma unroll
@@ -467,7 +473,6 @@ static int rows_args(tpuhip_ctx *ctx, const tpuhip_kv_cache *c, const tpuhip_kv_
   const int size = r->dtype == TPUHIP_F32 ? 4 : 2, dim = c->desc.head_dim, heads = c->desc.kv_heads;
   const int64_t ts[2] = {r->k_token_stride, r->v_token_stride}, hs[2] = {r->k_head_stride, r->v_head_stride};
   void *x[2] = {r->k, r->v};
-  a->dwords = 1;
   for (int i = 0; i < 2; ++i) {
     const char *name = i ? "values" : "keys";
     TPUHIP_REQUIRE(ts[i] >= 0 && hs[i] >= 0 && ts[i] <= INT64_MAX / 8 / r->tokens && hs[i] <= INT64_MAX / 8 / heads,
@@ -478,12 +483,11 @@ static int rows_args(tpuhip_ctx *ctx, const tpuhip_kv_cache *c, const tpuhip_kv_
       const bool by_head = (r->tokens == 1 || ts[i] >= dim) && (heads == 1 || hs[i] >= (r->tokens - 1) * ts[i] + dim);
       TPUHIP_REQUIRE(by_token || by_head, "%s: rows of the %s overlap", what, name);
     }
-    if ((uintptr_t)x[i] % 4 || ts[i] * size % 4 || hs[i] * size % 4) a->dwords = 0;
     a->x[i] = x[i];
     a->token_stride[i] = ts[i];
     a->head_stride[i] = hs[i];
   }
-  a->wide = a->dwords && dim == c->dp;
+  a->wide = dim == c->dp;
   a->data = c->data;
   a->slots = slots;
   a->tokens = r->tokens;
