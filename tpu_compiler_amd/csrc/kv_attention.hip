@@ -779,10 +779,13 @@ int tpuhip_kv_attention(tpuhip_ctx *ctx, const tpuhip_kv_cache *cache, const tpu
       const int64_t base = slots * kv_heads, row_bytes = (int64_t)a.total_q * a.heads * (U::kDim + 2) * 4;
       int64_t splits = 1;
       if (WR == 1) {
-        // Two workgroups a CU, and none of more than 128 units, as lengths may differ; but two units a wave at least, four with twice the
-        // rows, for a join takes as long (a wave takes 1 us a unit, the join of two splits 1.6), and so few splits that the last one can
-        // join them rather than another kernel, where these have six units a wave at most.
-        splits = std::min(std::max(ceil_div64(2 * num_cu, base), ceil_div64(units, 128)), ceil_div64(units, 8 * NC));
+        // Two workgroups a CU, without more than are there at a time (three, two with twice the rows or wider ones), and none of more than
+        // 128 units, as lengths may differ; but two units a wave at least, four with twice the rows, for a join takes as long (a wave takes
+        // 1 us a unit, the join of two splits 1.6), and so few splits that the last one can join them rather than another kernel, where
+        // these have six units a wave at most.
+        const int64_t there = (NC == 1 && U::kDim <= 128 ? 3 : 2) * num_cu;
+        splits = std::max<int64_t>(1, std::min(ceil_div64(2 * num_cu, base), there / base));
+        splits = std::min(std::max(splits, ceil_div64(units, 128)), ceil_div64(units, 8 * NC));
         if (units <= kJoinInKernel * 24) splits = std::min<int64_t>(splits, kJoinInKernel / NC);
       }
       splits = std::min(splits, std::max<int64_t>(1, (int64_t)kJoinBytes / row_bytes));
