@@ -454,6 +454,34 @@ def test_another_context_and_repeated_calls(ctx):
     s.cache.close()
 
 
+def test_a_context_on_the_stream_of_another(ctx):
+    rng = np.random.default_rng(14)
+    s = Sequences(ctx, rng, [100], 2, 64, 4)
+    q = rows(rng, 1, 4, 64, "bf16", False)
+    want = s.attend(q, [1], "bf16")
+    other = capi.Context(stream=ctx.lib.tpuhip_ctx_stream(ctx.h))
+    s.cache.ctx, s.ctx = other, other                # what the first one has issued is before this
+    assert np.array_equal(s.attend(q, [1], "bf16"), want)
+    s.cache.close()
+    other.close()
+
+
+def test_page_tables_whose_rows_end_early(ctx):
+    """the last sequence's row of a table ends where its pages do, whatever the distance of rows"""
+    rng = np.random.default_rng(15)
+    s = Sequences(ctx, rng, [70, 130], 1, 64, 4, page=32)
+    q = rows(rng, 2, 2, 64, "bf16", False)
+    want = s.attend(q, [1, 1], "bf16")
+    wide = np.full((2, 40), -1)
+    wide[:, 40 - s.table.shape[1]:] = s.table
+    base = array(ctx, wide, "i32")
+    out = DeviceArray(ctx, q.shape, "bf16")
+    s.cache.attention(array(ctx, q, "bf16"), out, array(ctx, [0, 1, 2], "i32"), array(ctx, [70, 130], "i32"),
+                      Strided(base, s.table.shape, (40, 1), 40 - s.table.shape[1]))
+    assert np.array_equal(out.numpy().astype(np.float64), want)
+    s.cache.close()
+
+
 def test_refusals(ctx):
     for sizes in ((0, 1, 64, 4, 64), (4, 0, 64, 4, 64), (4, 1, 0, 4, 64), (4, 1, 257, 4, 64), (4, 1, 64, 5, 64), (4, 1, 64, 4, 48),
                   (4, 1, 64, 4, 0), (1 << 26, 1, 64, 4, 32), (4, 70000, 64, 4, 32)):
@@ -491,3 +519,30 @@ def test_refusals(ctx):
     assert lib.tpuhip_kv_read(ctx.h, cache.h, rows, None) == 0      # nothing to do
     cache.close()
     cache.close()
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (40, 4)])
+def test_the_example_answers_as_with_exact_rows(ctx, window, sinks):
+    """prompts of different lengths, then single tokens: the logits are those of attention in 64 bits to the rows that the cache holds
+    of the same tokens.  Rows, queries and results are bfloat16 there and here, so that a step's logits differ by roundings of 2^-9 alone:
+    of a layer's result (twice, of what it adds), and of numbers that these move to the next one (four times as many, in three
+    layers); relative to logits of size one, 64 * 2^-9 is far above that and far below what a wrong token does."""
+    from tpu_compiler_amd import kv_example
+    model = kv_example.Model()
+    rng = np.random.default_rng(3)
+    prompts = [rng.integers(0, 512, n) for n in (3, 130, 64, 1)]
+    answers, steps, _ = kv_example.generate(ctx, model, prompts, 5, 8, window, sinks, page_tokens=32)
+    for i, prompt in enumerate(prompts):
+        held = [([], []) for _ in model.qkv]
+
+        def attend(layer, q, k, v):
+            for x, y in zip(held[layer], (k, v)):
+                x.append(O.values(O.rounded(y, "bf16"), 8))
+            kk, vv = (np.concatenate(x) for x in held[layer])
+            return O.rounded(O.attention(O.rounded(q, "bf16"), [kk], [vv], [len(q)], [len(kk)], 0.125, window, sinks)[0], "bf16")
+
+        new = prompt
+        for step, answer in zip(steps, answers[i]):
+            want = model(np.asarray(new), attend)[-1]
+            assert np.abs(step[i] - want).max() <= 64 * 2.0 ** -9
+            new = [answer]                           # the example's own, should two be alike
