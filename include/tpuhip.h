@@ -531,8 +531,9 @@ int tpuhip_dequant_i8_to_f32(tpuhip_ctx *ctx, const void *x, void *y_nchw_f32, i
  * give out: slot = page * page_tokens + place names one of them, and a page table lists the pages of a sequence in order.
  * Fresh pages read as zeros.  A token takes 2 * (D * bits / 8 + 4) bytes a head, with D rounded up to 64, 96, 128, 192
  * or 256.  Everything is issued to the stream of the context that a call is given; a cache may be used from any context of its
- * device, calls that touch the same tokens are the caller's to order.  No call allocates, and all can be captured into a
- * graph (indexes and lengths are read on the device when the graph runs). */
+ * device, calls that touch the same tokens are the caller's to order.  Calls can be captured into a graph (indexes and
+ * lengths are read on the device when it runs; a replay uses the context's memory, as its other calls do) and allocate
+ * nothing, but for 32 MiB of a context's partial sums, made with its first cache or the first attention that wants them. */
 typedef struct tpuhip_kv_cache tpuhip_kv_cache;
 typedef struct {
   int pages, page_tokens;   /* page_tokens: a multiple of 32; pages * page_tokens < 2^31 */
@@ -547,7 +548,7 @@ int tpuhip_kv_cache_destroy(tpuhip_ctx *ctx, tpuhip_kv_cache *cache);
 
 /* keys and values [tokens, kv_heads, head_dim] of one type, strides in elements, a head's numbers next to each other */
 typedef struct {
-  int tokens, dtype;
+  int tokens, dtype;        /* TPUHIP_BF16, TPUHIP_F16, TPUHIP_F32 */
   void *k, *v;
   int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
 } tpuhip_kv_rows;
@@ -565,8 +566,9 @@ int tpuhip_kv_read(tpuhip_ctx *ctx, const tpuhip_kv_cache *cache, const tpuhip_k
  * page_table[b * table_stride + t / page_tokens]; a page outside the cache holds nothing to be seen (entries before the
  * window need not be kept).  q_starts (n_seq + 1), kv_lens (n_seq), page_table are device memory; what they say is cut to
  * total_q, max_q queries a sequence, max_kv tokens.
- * Softmax and sums are 32-bit.  Queries are multiplied as float16 numbers scaled by a power of two for all queries of a tile (at most 64
- * rows of a sequence), which is exact for rows within 2^16 of each other; weights as float16 likewise. */
+ * Scores, maxima and sums are 32-bit.  Queries are multiplied as float16 numbers times a power of two for each tile of at most 32
+ * (query, head) pairs of a sequence, exactly as far as they are within 2^24 of the tile's largest; weights, times the values'
+ * steps, are rounded to float16. */
 typedef struct {
   int n_seq, heads, dtype;            /* dtype of q and out: TPUHIP_BF16 or TPUHIP_F16 */
   int total_q, max_q, max_kv;

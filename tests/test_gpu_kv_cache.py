@@ -515,6 +515,8 @@ def test_refusals(ctx):
     assert lib.tpuhip_kv_read(ctx.h, cache.h, rows, slots.ptr) == 1 and b"type" in lib.tpuhip_last_error()
     rows = capi.KVRows(3, 0, None, q.ptr, 128, 64, 128, 64)
     assert lib.tpuhip_kv_read(ctx.h, cache.h, rows, slots.ptr) == 1
+    rows = capi.KVRows(2 ** 30, 0, q.ptr, q.ptr, 128, 64, 128, 64)
+    assert lib.tpuhip_kv_write(ctx.h, cache.h, rows, slots.ptr) == 1 and b"one call" in lib.tpuhip_last_error()
     rows = capi.KVRows(0, 0, None, None, 0, 0, 0, 0)
     assert lib.tpuhip_kv_read(ctx.h, cache.h, rows, None) == 0      # nothing to do
     cache.close()

@@ -1,4 +1,4 @@
-// Attention to a key/value cache of 4 or 8 bits.
+// Attention to a key/value cache of 4 or 8 bits: single tokens, a few tokens and prompts, over all tokens or a window and the first ones.
 #include "kv_cache.hpp"
 
 #include <algorithm>
@@ -128,7 +128,16 @@ constexpr int kJoinWaves = 16;
 // The left operands are the codes themselves: masked out of a dword, two of them are a pair of subnormal float16 numbers
 // c 2^-24 (of a byte's upper half c 2^-20), which the matrix unit takes as they are and multiplies exactly.  Steps and offsets are applied to
 // what is small: x = s_t (q.c_t) + m_t sum(q) to the scores, and P'_t = p_t s_t to the weights, with sum(p_t m_t) added to all channels.
+// Scores, maxima and sums are 32 bits; weights are rounded once, to float16, as the result is (at most 1.4 times its own rounding in all).
 // Of a workgroup's four waves, WR have rows of their own; the 4 / WR with the same rows take every so manieth unit and join their sums in LDS.
+//
+// Bounds.  Few rows: memory.  A unit of 128 channels in 4 bits is 4352 bytes, read once, straight into the lanes that multiply it (no
+// barrier in the loop): one token for each of 64 sequences of 61 to 8192, 288 MB, takes 67 us, 4.3 TB/s (a copy moves 4.8, reading alone reaches
+// 6.0); for one of 131072, 143 MB, 28 us and 4.5 for the join.  Many rows: the vector ALU.  A unit costs a wave 80 instructions to unpack and
+// 7 a score (two fused products, half a maximum, an exponential, a sum, a step, an offset, half a conversion), 250 for 32 rows against 32
+// matrix instructions of 16 cycles; 8192 tokens of 32 heads, causal, 0.55 TFLOP, take 582 us, 940 TFLOP/s, 77 % of a large float16 product,
+// with the vector ALU busy for 75 % of the time.  More rows a wave would amortise unpacking, but 48 of 128 channels need the queries in LDS,
+// all registers, and gain 2 %; fewer, 16, have three waves a SIMD and take 709 us.
 template <typename U, int NC, int WR>
 __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(AttentionArgs a) {
   constexpr int DP = U::kDim, KD = U::kRow / 16, STEPS = DP / 32, OB = DP / 16, WK = kAttentionWaves / WR;
@@ -275,8 +284,8 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
     }
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) most = fmaxf(most, __shfl_xor(most, d));
-    // the wave's queries times one power of two, the largest number just below 2^15: float16 holds bfloat16's 8 bits of all that are
-    // within 2^29 of it.  A number past the bounds of the exponent becomes an infinity, in its own row.
+    // the wave's queries times one power of two, the largest number just below 2^15: float16 holds all bits of those within 2^24 of it,
+    // and of smaller ones a multiple of 2^-38 of it.  A number past the bounds of the exponent becomes an infinity, in its own row.
     e2 = min(max((int)(__float_as_uint(most) >> 23) - 127 - 14, -100), 88);
     const float down = __uint_as_float((uint32_t)(127 - e2) << 23);
 #pragma unroll
@@ -629,7 +638,9 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
   }
 }
 
-// The splits of a row, joined: a workgroup a row, whose waves take every sixteenth split, a lane a channel of each 64.
+// The splits of a row, joined: a workgroup a row, whose waves take every sixteenth split, a lane a channel of each 64.  Bound by latency: 64
+// splits of 64 rows, 2 MB, take 4.5 us with the gap before it (34 us with the attention, and 40 where the last workgroups join so many).  Few splits of
+// many rows are better joined there: 2 of 2048 rows take 68 us with the attention, and 97 with this kernel.
 template <typename U, int NC, int WR>
 __global__ __launch_bounds__(64 * kJoinWaves) void kv_join_kernel(AttentionArgs a) {
   constexpr int DP = U::kDim, C = (DP + 63) / 64, WAVES = kJoinWaves;
@@ -679,7 +690,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void kv_join_kernel(AttentionArgs 
   dst[c] = (uint16_t)store16(sum != 0 ? x / sum : 0.0f, a.bf16);
 }
 
-// Splits' sums: a split of 16 rows of 128 channels takes 8 KiB, four of them on each of 256 CUs 8 MiB.
+// Splits' sums: a split of 16 rows of 128 channels takes 8 KiB, three of them on each of 256 CUs 6 MiB.
 constexpr size_t kJoinBytes = 32 << 20;
 constexpr int kCounters = 16384, kJoinInKernel = 16;   // tiles with a counter; splits up to which the last workgroup joins them
 
@@ -762,8 +773,10 @@ int tpuhip_kv_attention(tpuhip_ctx *ctx, const tpuhip_kv_cache *cache, const tpu
   a.bf16 = d->dtype == TPUHIP_BF16;
   a.scale = d->scale;
   a.n_seq = d->n_seq;
-  // The form of the kernel, R rows a workgroup: the more rows a wave has, the fewer times codes are unpacked and the fewer of the
-  // matrix unit's rows stay empty; but the workgroups have to fill the CUs.
+  // The form of the kernel, R rows a workgroup: the more rows a wave has, the fewer times codes are unpacked; but the workgroups have to
+  // fill the CUs.  For 262144 rows of 128 channels in 4 bits R = 128, 64, 32 and 16 take 583, 618, 666 and 786 us; for 31200, behind a window of
+  // 1024, 44, 33, 40 and 43; for 24 sequences of 12 to 28 rows of 80 channels in 8 bits 130, 75, 24 and 27; for 64 of 4 rows 219, 137, 85 and 68.
+  // Rows of more than 128 channels have one block of 16 a wave: two would not fit into registers.
   const int group = (int)a.group.d, num_cu = ctx->num_cu;
   const int64_t rows_max = (int64_t)a.max_q * group;             // of a sequence and cache head
   const int64_t rows_all = std::min<int64_t>(rows_max * d->n_seq, (int64_t)a.total_q * group) * kv_heads;
@@ -803,7 +816,9 @@ int tpuhip_kv_attention(tpuhip_ctx *ctx, const tpuhip_kv_cache *cache, const tpu
       a.class_heads = FastDiv(kv_heads / a.classes);
       a.split_count = FastDiv(a.splits);
       const int64_t works = slots * a.splits * (kv_heads / a.classes);
-      TPUHIP_REQUIRE(works * a.classes < INT_MAX - kXcds && slots * R <= INT_MAX, "%s: %d queries of %d sequences", what, a.total_q, d->n_seq);
+      // a launch has fewer than 2^32 threads
+      TPUHIP_REQUIRE((works * a.classes + kXcds) * 64 * kAttentionWaves <= UINT32_MAX && slots * R * 64 * kJoinWaves <= UINT32_MAX,
+                     "%s: %d queries of %d sequences in one call", what, a.total_q, d->n_seq);
       a.works = (int)works;
       launch(ctx, kv_attention_kernel<U, NC, WR>, dim3((unsigned)(ceil_div64(works, kXcds / a.classes) * kXcds)), dim3(64 * kAttentionWaves), a);
       TPUHIP_CHECK_HIP(hipGetLastError());
