@@ -504,6 +504,7 @@ def test_refusals(ctx):
     for a in ((DeviceArray(ctx, (3, 5, 64), "bf16"),) * 2, (DeviceArray(ctx, (3, 4, 64), "f32"),) * 2, (q, y), (q, DeviceArray(ctx, (2, 4, 64), "bf16")),
               (q, Strided(q, (3, 4, 64), (64, 64, 1), 0))):
         refused(cache.attention, *a, starts, lens, table)
+    refused(cache.attention, q, q, starts, lens, table)             # in place
     for how in (dict(max_kv=65), dict(window=-1), dict(sinks=-1), dict(scale=float("nan")), dict(max_q=-1), dict(max_kv=-1)):
         refused(cache.attention, q, q, starts, lens, table, **how)
     refused(cache.attention, q, q, starts, array(ctx, [3, 3], "i32"), table)

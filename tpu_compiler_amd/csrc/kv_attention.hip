@@ -134,9 +134,9 @@ constexpr int kJoinWaves = 16;
 // Bounds.  Few rows: memory.  A unit of 128 channels in 4 bits is 4352 bytes, read once, straight into the lanes that multiply it (no
 // barrier in the loop): one token for each of 64 sequences of 61 to 8192, 288 MB, takes 67 us, 4.3 TB/s (a copy moves 4.8, reading alone reaches
 // 6.0); for one of 131072, 143 MB, 28 us and 4.5 for the join.  Many rows: the vector ALU.  A unit costs a wave 80 instructions to unpack and
-// 7 a score (two fused products, half a maximum, an exponential, a sum, a step, an offset, half a conversion), 250 for 32 rows against 32
+// 7 a score (two fused products, half a maximum, an exponential, a sum, a step, an offset, half a conversion), 235 for 32 rows against 32
 // matrix instructions of 16 cycles; 8192 tokens of 32 heads, causal, 0.55 TFLOP, take 582 us, 940 TFLOP/s, 77 % of a large float16 product,
-// with the vector ALU busy for 75 % of the time.  More rows a wave would amortise unpacking, but 48 of 128 channels need the queries in LDS,
+// with the vector ALU busy for 83 % of the time and the matrix unit for 37 %.  More rows a wave would amortise unpacking, but 48 of 128 channels need the queries in LDS,
 // all registers, and gain 2 %; fewer, 16, have three waves a SIMD and take 709 us.
 template <typename U, int NC, int WR>
 __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(AttentionArgs a) {
@@ -746,6 +746,7 @@ int tpuhip_kv_attention(tpuhip_ctx *ctx, const tpuhip_kv_cache *cache, const tpu
   TPUHIP_REQUIRE(((d->heads == 1 || hs >= dim) && (d->total_q == 1 || ts >= (d->heads - 1) * hs + dim)) ||
                      ((d->total_q == 1 || ts >= dim) && (d->heads == 1 || hs >= (d->total_q - 1) * ts + dim)),
                  "%s: rows of the result overlap", what);
+  TPUHIP_REQUIRE(q != out, "%s: the result takes the queries' place", what);
   TPUHIP_REQUIRE((uintptr_t)q % 2 == 0 && (uintptr_t)out % 2 == 0, "%s: q or out does not begin at an element", what);
   AttentionArgs a{};
   a.data = cache->data;

@@ -152,8 +152,8 @@ class KVCache:
 
     def plan_attention(self, q, out, q_starts, kv_lens, page_table, max_q=None, max_kv=None, scale=None, window=0, sinks=0):
         """A call in which queries attend to the cache.  q, out: [queries, heads, head_dim], the sequences' one after the other; q_starts
-        [sequences + 1], kv_lens [sequences] (the queries' own tokens among them), page_table [sequences, pages]: int32.  A query sees
-        the tokens up to its own, with a window the last `window` of them and the first `sinks` of the sequence.  max_q, max_kv: no
+        [sequences + 1], kv_lens [sequences] (the queries' own tokens among them), page_table [sequences, pages]: int32.  out is no part of q.
+        A query sees the tokens up to its own, with a window the last `window` of them and the first `sinks` of the sequence.  max_q, max_kv: no
         sequence has more queries or tokens (the fewer, the better the work is split).  scale: 1 / sqrt(head_dim)."""
         heads, total = int(q.shape[1]) if len(q.shape) == 3 else 0, int(q.shape[0])
         qs, outs = _rows3(q, "q", self.ctx, heads, self.head_dim), _rows3(out, "out", self.ctx, heads, self.head_dim)
