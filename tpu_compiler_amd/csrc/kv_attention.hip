@@ -28,6 +28,8 @@ struct AttentionArgs {
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef unsigned short ushort2v __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float float2v __attribute__((ext_vector_type(2)));
 typedef float float4v __attribute__((ext_vector_type(4)));
 typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
@@ -42,6 +44,9 @@ __device__ __forceinline__ uint32_t store16(float v, int bf16) {
 }
 __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((float2v){a, b}, half2v));
+}
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((float2v){a, b}, bf16x2));
 }
 // two floats past the caches that a device's XCDs have of their own
 __device__ __forceinline__ void store2(float *p, float x, float y) {
@@ -64,6 +69,20 @@ __device__ __forceinline__ int sums_upto(int v) {
   v = dpp_add<0x118, 0xf>(v);
   v = dpp_add<0x142, 0xa>(v);                                  // from lane 15 to 16..31 and 47 to 48..63,
   return dpp_add<0x143, 0xc>(v);                               // from lane 31 to 32..63
+}
+
+// the largest of a wave's numbers, in a scalar register
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_max(uint32_t v) {
+  return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+  v = dpp_max<0xB1>(v);                                        // of lanes 1 and 2 apart, of halves of 16 and of 16 turned round,
+  v = dpp_max<0x4E>(v);
+  v = dpp_max<0x141>(v);
+  v = dpp_max<0x140>(v);
+  const auto of = [&](int l) { return (uint32_t)__builtin_amdgcn_readlane((int)v, l); };
+  return max(max(of(0), of(16)), max(of(32), of(48)));
 }
 
 // A tile of R rows of a sequence, the `slot`th of those of all sequences: which sequence, its first query, how many it has, the position
@@ -168,34 +187,31 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
 
   // ---- queries
   int pos[NC];
-  float q_sum[NC];
   uint4v q[NC][STEPS];
-  float most = 0;
-  int e2 = 0;
 #pragma unroll
   for (int nc = 0; nc < NC; ++nc) {
-    uint32_t h = row0 + nc * 16 + col;
-    const bool valid = (int)h < rows;
+    uint32_t h = min(row0 + nc * 16 + col, rows - 1);           // past the last row: that one again, to be thrown away
     const int token = (int)a.group.split(h);
     pos[nc] = seq.first + token;
     const uint16_t *src = a.q + (int64_t)(seq.begin + token) * a.q_token_stride + (int64_t)(kvh * group + (int)h) * a.q_head_stride;
-    q_sum[nc] = 0;
+    if (a.dim % 8 == 0) {
 #pragma unroll
-    for (int st = 0; st < STEPS; ++st) {
-      const int c0 = g * (DP / 4) + st * 8;
-      uint4v raw = {0, 0, 0, 0};
-      if (valid && c0 < a.dim) {
-        if (c0 + 8 <= a.dim) {
-          raw = *(const uint4u *)(src + c0);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const uint32_t b = src[min(c0 + e, a.dim - 1)];
-            raw[e / 2] |= (c0 + e < a.dim ? b : 0) << 16 * (e & 1);
-          }
-        }
+      for (int st = 0; st < STEPS; ++st) {
+        const int c0 = g * (DP / 4) + st * 8;
+        q[nc][st] = *(const uint4u *)(src + (c0 < a.dim ? c0 : 0));
       }
-      q[nc][st] = raw;
+    } else {
+#pragma unroll
+      for (int st = 0; st < STEPS; ++st) {
+        const int c0 = g * (DP / 4) + st * 8;
+        uint4v raw = {0, 0, 0, 0};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t b = src[min(c0 + e, a.dim - 1)];
+          raw[e / 2] |= (c0 + e < a.dim ? b : 0) << 16 * (e & 1);
+        }
+        q[nc][st] = raw;
+      }
     }
   }
   // ---- units: each lane looks up one of the wave's next 64
@@ -257,37 +273,37 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
     in_order();
   }
 
-  // ---- queries as the matrix unit takes them, while the first unit is on its way
-  const auto queries = [&](auto is_bf16) {
-    constexpr int bf16 = decltype(is_bf16)::value;
+  // ---- queries as the matrix unit takes them, while the first unit is on its way: the wave's times one power of two, the largest number
+  // just below 2^15.  float16 holds all bits of those within 2^24 of it, and of smaller ones a multiple of 2^-38 of it.  A number past the
+  // bounds of the exponent becomes an infinity, in its own row.
+  ushort2v most2 = {0, 0};                                      // magnitudes are in order as integers
+#pragma unroll
+  for (int nc = 0; nc < NC; ++nc)
+#pragma unroll
+    for (int st = 0; st < STEPS; ++st) {
+      if (g * (DP / 4) + st * 8 >= a.dim) q[nc][st] = (uint4v){0, 0, 0, 0};
+#pragma unroll
+      for (int d = 0; d < 4; ++d) most2 = __builtin_elementwise_max(most2, __builtin_bit_cast(ushort2v, q[nc][st][d] & 0x7FFF7FFF));
+    }
+  const uint32_t infinite = a.bf16 ? 0x7F80 : 0x7C00;
+  uint32_t most = max((uint32_t)most2[0], (uint32_t)most2[1]);
+  if (__any(most >= infinite)) {                                // those are not to count
+    most = 0;
 #pragma unroll
     for (int nc = 0; nc < NC; ++nc)
 #pragma unroll
       for (int st = 0; st < STEPS; ++st)
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float v = load16(q[nc][st][e / 2] >> 16 * (e & 1), bf16);
-          q_sum[nc] += v;
-          most = fmaxf(most, fabsf(v));
+          const uint32_t v = q[nc][st][e / 2] >> 16 * (e & 1) & 0x7FFF;
+          most = max(most, v < infinite ? v : 0u);
         }
-    if (__any(!(most <= __FLT_MAX__))) {                        // infinities, which are not to count; NaN does not
-      most = 0;
-#pragma unroll
-      for (int nc = 0; nc < NC; ++nc)
-#pragma unroll
-        for (int st = 0; st < STEPS; ++st)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float v = fabsf(load16(q[nc][st][e / 2] >> 16 * (e & 1), bf16));
-            most = v <= __FLT_MAX__ ? fmaxf(most, v) : most;
-          }
-    }
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) most = fmaxf(most, __shfl_xor(most, d));
-    // the wave's queries times one power of two, the largest number just below 2^15: float16 holds all bits of those within 2^24 of it,
-    // and of smaller ones a multiple of 2^-38 of it.  A number past the bounds of the exponent becomes an infinity, in its own row.
-    e2 = min(max((int)(__float_as_uint(most) >> 23) - 127 - 14, -100), 88);
-    const float down = __uint_as_float((uint32_t)(127 - e2) << 23);
+  }
+  most = wave_max(most);
+  const int e2 = min(max((int)(__float_as_uint(load16(most, a.bf16)) >> 23) - 127 - 14, -100), 88);
+  const float down = __uint_as_float((uint32_t)(127 - e2) << 23);
+  const auto queries = [&](auto is_bf16) {
+    constexpr int bf16 = decltype(is_bf16)::value;
 #pragma unroll
     for (int nc = 0; nc < NC; ++nc)
 #pragma unroll
@@ -305,10 +321,16 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
     queries(std::true_type{});
   else
     queries(std::false_type{});
+  // their sums, of the same rounded numbers: a token whose codes are all one
+  float q_sum[NC];
+  constexpr uint32_t one = 0x3C003C00, odd = U::kBits == 4 ? 0x4C004C00 : one;
 #pragma unroll
   for (int nc = 0; nc < NC; ++nc) {
-    q_sum[nc] += __shfl_xor(q_sum[nc], 16);
-    q_sum[nc] += __shfl_xor(q_sum[nc], 32);
+    float4v sum = {0, 0, 0, 0};
+#pragma unroll
+    for (int st = 0; st < STEPS; ++st)
+      sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, (uint4v){one, odd, one, odd}), __builtin_bit_cast(half8, q[nc][st]), sum, 0, 0, 0);
+    q_sum[nc] = ldexpf(sum[0], e2);
   }
   const float log2e = 1.44269504088896341f;
   const float offset_scale = a.scale * log2e, step_scale = ldexpf(offset_scale, e2 + 24);
@@ -521,17 +543,14 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
     const int token = (int)a.group.split(h);
     return a.out + (int64_t)(seq.begin + token) * a.out_token_stride + (int64_t)(kvh * group + (int)h) * a.out_head_stride;
   };
-  const auto write = [&](uint16_t *dst, int c0, float4v v, float inv) {
-    v *= inv;
-    uint32_t b[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) b[r] = store16(v[r], a.bf16);
+  const auto write = [&](uint16_t *dst, int c0, float4v v) {
+    const uint2u b = a.bf16 ? (uint2u){pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])} : (uint2u){pack_f16(v[0], v[1]), pack_f16(v[2], v[3])};
     if (c0 + 4 <= a.dim) {
-      *(uint2u *)(dst + c0) = (uint2u){b[0] | b[1] << 16, b[2] | b[3] << 16};
+      *(uint2u *)(dst + c0) = b;
     } else {
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (c0 + r < a.dim) dst[c0 + r] = (uint16_t)b[r];
+      for (int r = 0; r < 3; ++r)
+        if (c0 + r < a.dim) dst[c0 + r] = (uint16_t)(b[r / 2] >> 16 * (r & 1));
     }
   };
   if constexpr (WK == 1) {
@@ -546,7 +565,7 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
         uint16_t *dst = result(row);
         const float inv = total[nc] != 0 ? 1.0f / total[nc] : 0.0f;
 #pragma unroll
-        for (int b = 0; b < OB; ++b) write(dst, b * 16 + g * 4, o[b][nc], inv);
+        for (int b = 0; b < OB; ++b) write(dst, b * 16 + g * 4, o[b][nc] * inv);
       }
     }
   } else {
@@ -584,7 +603,7 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
         if (splits > 1)
           keep(row, c, v, high, sum);
         else
-          write(dst, c, v, inv);
+          write(dst, c, v * inv);
       }
     }
     if (WR > 1 || splits == 1 || !a.counters) return;
@@ -633,7 +652,7 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
           v[3] = __builtin_fmaf(y[k][1], w, v[3]);
         }
       }
-      write(result(row), c, v, sum != 0 ? 1.0f / sum : 0.0f);
+      write(result(row), c, v * (sum != 0 ? 1.0f / sum : 0.0f));
     }
   }
 }
