@@ -569,7 +569,7 @@ int tpuhip_kv_read(tpuhip_ctx *ctx, const tpuhip_kv_cache *cache, const tpuhip_k
  * with q (workgroups that split a sequence read the queries again).
  * Scores, maxima and sums are 32-bit.  Queries are multiplied as float16 numbers times a power of two for each tile of at most 32
  * (query, head) pairs of a sequence, exactly as far as they are within 2^24 of the tile's largest; weights, times the values'
- * steps, are rounded to float16. */
+ * steps, are rounded to float16.  Sums are divided by that of the weights at the end: values past 1e30 may overflow them. */
 typedef struct {
   int n_seq, heads, dtype;            /* dtype of q and out: TPUHIP_BF16 or TPUHIP_F16 */
   int total_q, max_q, max_kv;

@@ -65,3 +65,22 @@ def attention(q, k, v, q_lens, kv_lens, scale, window=0, sinks=0):
                         size[row, h] = w @ np.abs(vv[t, g])
             row += 1
     return out, size
+
+
+def attention_of_finite(q, k, v, q_lens, kv_lens, scale, window=0, sinks=0):
+    """the same where all numbers are finite, a cache head's rows at a time"""
+    heads, dim = q.shape[1:]
+    out, size = np.zeros(q.shape), np.zeros(q.shape)
+    row = 0
+    for kk, vv, n, length in zip(k, v, q_lens, kv_lens):
+        p, t = length - n + np.arange(n)[:, None], np.arange(length)
+        seen = (t <= p) & ((t > p - window) | (t < sinks)) if window else t <= p
+        group = heads // kk.shape[1]
+        for g in range(kk.shape[1]):
+            at = np.s_[row:row + n, g * group:(g + 1) * group]
+            x = np.where(seen[:, None], q[at].astype(np.float64) @ kk[:, g].T.astype(np.float64) * scale, -np.inf)
+            w = np.exp(x - np.maximum(x.max(-1, keepdims=True, initial=-np.inf), -1e300)) * seen[:, None]
+            w /= np.maximum(w.sum(-1, keepdims=True), 1e-300)
+            out[at], size[at] = w @ vv[:, g].astype(np.float64), w @ np.abs(vv[:, g]).astype(np.float64)
+        row += n
+    return out, size

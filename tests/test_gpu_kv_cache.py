@@ -196,12 +196,12 @@ def bound(q, seqs, want, size, scale, dtype, least=2.0 ** -24):
     return unit * np.abs(want) + (2.0 ** -10 + 2 * 300 * 2.0 ** -24 * t) * (size + 3 * offsets) + least
 
 
-def check(rng, ctx, kv_lens, q_lens, heads, kv_heads, dim, bits, dtype, page=64, scale=None, q=None, k=None, v=None, **how):
+def check(rng, ctx, kv_lens, q_lens, heads, kv_heads, dim, bits, dtype, page=64, scale=None, q=None, k=None, v=None, oracle=O.attention, **how):
     s = Sequences(ctx, rng, kv_lens, kv_heads, dim, bits, page, k=k, v=v)
     if q is None:
         q = rows(rng, sum(q_lens), heads, dim, dtype, spread=False)
     used = dim ** -0.5 if scale is None else scale
-    want, size = O.attention(q, s.k, s.v, q_lens, kv_lens, used, **how)
+    want, size = oracle(q, s.k, s.v, q_lens, kv_lens, used, **how)
     got = s.attend(q, q_lens, dtype, scale=scale, **how)
     limit = bound(q, s, want, size, used, dtype)
     s.cache.close()
@@ -237,6 +237,15 @@ def test_head_sizes(ctx, bits, dim):
 @pytest.mark.parametrize("q,kv", [(2, 2), (5, 64), (17, 40), (33, 33), (64, 500), (65, 65), (129, 400), (300, 300)])
 def test_prompts_and_parts_of_them(ctx, bits, dtype, q, kv):
     check(np.random.default_rng(q), ctx, [kv, kv + 9], [q, max(1, q - 1)], 4, 2, 128, bits, dtype)
+
+
+@pytest.mark.parametrize("bits,dim,dtype", [(4, 64, "bf16"), (8, 80, "f16"), (4, 128, "f16"), (8, 128, "bf16"), (4, 200, "bf16"), (8, 250, "f16")])
+@pytest.mark.parametrize("q,kv,heads,kv_heads", [(41, 250, 96, 3), (150, 230, 70, 7), (270, 290, 50, 2), (270, 290, 96, 8), (270, 290, 260, 4), (60, 1500, 12, 1)])
+def test_many_rows(ctx, bits, dim, dtype, q, kv, heads, kv_heads):
+    """so many that each form of the kernel has its turn: 16 to 128 rows a workgroup, of which one to four waves have their own"""
+    rng = np.random.default_rng(q + heads)
+    check(rng, ctx, [kv, 40], [q, 7], heads, kv_heads, dim, bits, dtype, page=32, oracle=O.attention_of_finite)
+    check(rng, ctx, [kv], [q], heads, kv_heads, dim, bits, dtype, window=kv // 3, sinks=33, oracle=O.attention_of_finite)
 
 
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (5, 2), (32, 0), (33, 4), (64, 40), (100, 64), (1000, 3), (7, 1000)])

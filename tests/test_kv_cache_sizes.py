@@ -1,8 +1,10 @@
 """The key/value cache's sizes and refusals: host code, no GPU."""
 import ctypes as C
 
+import numpy as np
 import pytest
 
+import kv_oracle as O
 from tpu_compiler_amd import capi
 
 
@@ -35,3 +37,12 @@ def test_no_context_or_descriptor_is_refused():
     assert lib.tpuhip_kv_cache_destroy(None, None) == 1
     assert lib.tpuhip_kv_write(None, None, None, None) == 1 and lib.tpuhip_kv_read(None, None, None, None) == 1
     assert lib.tpuhip_kv_attention(None, None, None, None, None, None, None, None) == 1
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (5, 2)])
+def test_the_oracle_by_heads_is_the_oracle(window, sinks):
+    rng = np.random.default_rng(1)
+    q = rng.standard_normal((12, 6, 8))
+    k, v = ([rng.standard_normal((n, 2, 8)) for n in (20, 0, 3)] for _ in "kv")
+    for a, b in zip(O.attention(q, k, v, [5, 2, 5], [20, 0, 3], 0.3, window, sinks), O.attention_of_finite(q, k, v, [5, 2, 5], [20, 0, 3], 0.3, window, sinks)):
+        assert np.abs(a - b).max() < 1e-14

@@ -157,6 +157,9 @@ constexpr int kJoinWaves = 16;
 // matrix instructions of 16 cycles; 8192 tokens of 32 heads, causal, 0.55 TFLOP, take 582 us, 940 TFLOP/s, 77 % of a large float16 product,
 // with the vector ALU busy for 83 % of the time and the matrix unit for 37 %.  More rows a wave would amortise unpacking, but 48 of 128 channels need the queries in LDS,
 // all registers, and gain 2 %; fewer, 16, have three waves a SIMD and take 709 us.
+// In between, latency: a SIMD with one wave issues a vector instruction every eight clocks instead of four to five, and a unit of 32 rows takes it
+// 0.95 us, where two waves take 1.13 for one each.  Multiplying the next unit's keys before this one's scores, and handing on its params, took nothing
+// off that and 5 % more where memory bounds.  A wave's way in and out is four units' worth of instructions.
 template <typename U, int NC, int WR>
 __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(AttentionArgs a) {
   constexpr int DP = U::kDim, KD = U::kRow / 16, STEPS = DP / 32, OB = DP / 16, WK = kAttentionWaves / WR;
@@ -793,22 +796,20 @@ int tpuhip_kv_attention(tpuhip_ctx *ctx, const tpuhip_kv_cache *cache, const tpu
   a.bf16 = d->dtype == TPUHIP_BF16;
   a.scale = d->scale;
   a.n_seq = d->n_seq;
-  // The form of the kernel, R rows a workgroup: the more rows a wave has, the fewer times codes are unpacked; but the workgroups have to
-  // fill the CUs.  For 262144 rows of 128 channels in 4 bits R = 128, 64, 32 and 16 take 583, 618, 666 and 786 us; for 31200, behind a window of
-  // 1024, 44, 33, 40 and 43; for 24 sequences of 12 to 28 rows of 80 channels in 8 bits 130, 75, 24 and 27; for 64 of 4 rows 219, 137, 85 and 68.
-  // Rows of more than 128 channels have one block of 16 a wave: two would not fit into registers.
   const int group = (int)a.group.d, num_cu = ctx->num_cu;
   const int64_t rows_max = (int64_t)a.max_q * group;             // of a sequence and cache head
   const int64_t rows_all = std::min<int64_t>(rows_max * d->n_seq, (int64_t)a.total_q * group) * kv_heads;
   return kv_dispatch(cache, [&](auto u) -> int {
     using U = decltype(u);
+    const auto units_of = [&](int r) -> int64_t {               // that a tile of r rows sees at most
+      const int64_t units = ceil_div64(a.max_kv, kUnitTokens);
+      return a.window ? std::min<int64_t>(units, ceil_div64(a.sinks, kUnitTokens) + (a.window + r / group + 2) / kUnitTokens + 2) : units;
+    };
     const auto run = [&](auto nc, auto wr) -> int {
       constexpr int NC = decltype(nc)::value, WR = decltype(wr)::value, R = 16 * NC * WR;
       a.one_tile = rows_max <= R;
       const int64_t slots = a.one_tile ? d->n_seq : std::min(ceil_div64(rows_max, R) * d->n_seq, (int64_t)a.total_q * group / R + d->n_seq);
-      // units that a tile sees at most
-      int64_t units = ceil_div64(a.max_kv, kUnitTokens);
-      if (a.window) units = std::min<int64_t>(units, ceil_div64(a.sinks, kUnitTokens) + (a.window + R / group + 2) / kUnitTokens + 2);
+      const int64_t units = units_of(R);
       const int64_t base = slots * kv_heads, row_bytes = (int64_t)a.total_q * a.heads * (U::kDim + 2) * 4;
       int64_t splits = 1;
       if (WR == 1) {
@@ -848,13 +849,38 @@ int tpuhip_kv_attention(tpuhip_ctx *ctx, const tpuhip_kv_cache *cache, const tpu
       }
       return TPUHIP_OK;
     };
+    // The form of the kernel: 16 NC rows a wave, WR of the four waves with rows of their own.  Wide waves unpack codes less often, waves
+    // with the same rows end a long list sooner, and there have to be workgroups for the CUs, more than two at a time where tiles differ.
+    // Microseconds of 4 sequences of n tokens, causal, heads of 128 in 4 bits by fours (NC, WR; the chosen one in brackets):
+    //    n  heads  rows a CU    2, 4     2, 2     2, 1     1, 4     1, 1
+    //    64    4        16       9.4      9.0      8.2      7.6     [6.5]
+    //   512    4        32      21.5     15.9     11.8     16.1     [9.8]
+    //  1088    4        68      37.4     24.8    [19.4]    27.6     20.6
+    //    64  128       128      11.6     12.8     19.9    [10.1]    19.8
+    //   512   16       128      24.3    [21.0]    24.8     21.4     24.6
+    //   256   64       256     [22.6]    27.1     38.0     23.6     37.0
+    //  1088   64      1088    [125.5]   158.5    209.9    139.6    212.8
+    // and of 64 queries of each behind 4096 tokens of 8 heads 115.8, 65.9, 24.0, 84.6 and [19.3]; of one prompt of 2176 of 32 heads (272 rows a
+    // CU) 76.8, [67.1], 77.2, 65.8 and 79.0; of a draft, 24 sequences of 12 to 28 rows of 80 channels in 8 bits, 130, 75, [23.9], 102 and 27.1.
+    // Rows of more than 128 channels have one block of 16 a wave, as two do not fit into registers.
     using std::integral_constant;
-    constexpr int WIDE = U::kDim <= 128 ? 2 : 1;   // 16s of rows a wave: their sums take DP / 4 registers each
-    const auto enough = [&](int r, int a_cu) { return ceil_div64(rows_all, r) >= (int64_t)a_cu * num_cu; };
-    if (WIDE > 1 && rows_max <= 16) return run(integral_constant<int, 1>{}, integral_constant<int, 1>{});
-    if (rows_max <= 16 * WIDE || !enough(32 * WIDE, 1)) return run(integral_constant<int, WIDE>{}, integral_constant<int, 1>{});
-    if (!enough(64 * WIDE, 4)) return run(integral_constant<int, WIDE>{}, integral_constant<int, 2>{});
-    return run(integral_constant<int, WIDE>{}, integral_constant<int, 4>{});
+    const integral_constant<int, 1> one;
+    const integral_constant<int, 2> two;
+    const integral_constant<int, 4> four;
+    const auto enough = [&](int rows_a_cu) { return rows_all > (int64_t)rows_a_cu * num_cu; };
+    if constexpr (U::kDim <= 128) {
+      const int64_t seen = units_of(32);
+      if (rows_max <= 16 || (rows_max > 32 && !enough(32))) return run(one, one);
+      if (rows_max <= 32) return run(two, one);
+      if (seen <= 8) return run(one, four);
+      if (!enough(80)) return run(two, one);
+      if (!enough(seen <= 40 ? 255 : 511)) return run(two, two);
+      return run(two, four);
+    } else {
+      if (rows_max <= 16 || !enough(31)) return run(one, one);
+      if (!enough(255)) return run(one, two);
+      return run(one, four);
+    }
   });
 }
 
