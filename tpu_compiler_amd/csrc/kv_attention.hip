@@ -197,24 +197,24 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
     const int token = (int)a.group.split(h);
     pos[nc] = seq.first + token;
     const uint16_t *src = a.q + (int64_t)(seq.begin + token) * a.q_token_stride + (int64_t)(kvh * group + (int)h) * a.q_head_stride;
-    if (a.dim % 8 == 0) {
 #pragma unroll
-      for (int st = 0; st < STEPS; ++st) {
-        const int c0 = g * (DP / 4) + st * 8;
-        q[nc][st] = *(const uint4u *)(src + (c0 < a.dim ? c0 : 0));
-      }
-    } else {
-#pragma unroll
-      for (int st = 0; st < STEPS; ++st) {
-        const int c0 = g * (DP / 4) + st * 8;
-        uint4v raw = {0, 0, 0, 0};
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint32_t b = src[min(c0 + e, a.dim - 1)];
-          raw[e / 2] |= (c0 + e < a.dim ? b : 0) << 16 * (e & 1);
+    for (int st = 0; st < STEPS; ++st) {
+      const int c0 = g * (DP / 4) + st * 8;
+      uint4v raw = {0, 0, 0, 0};
+      if (a.dim >= 8) {                                         // the last eight channels in place of eight that are not all there
+        const int at = min(c0, a.dim - 8);
+        raw = *(const uint4u *)(src + at);
+        if (a.dim % 8 && at < c0) {
+          const int by = min(c0 - at, 7) * 16;
+          const uint64_t low = raw[0] | (uint64_t)raw[1] << 32, high = raw[2] | (uint64_t)raw[3] << 32;
+          const uint64_t down = by < 64 ? low >> by | high << 1 << (63 - by) : high >> (by - 64), up = by < 64 ? high >> by : 0;
+          raw = (uint4v){(uint32_t)down, (uint32_t)(down >> 32), (uint32_t)up, (uint32_t)(up >> 32)};
         }
-        q[nc][st] = raw;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) raw[e / 2] |= (e < a.dim ? src[min(e, a.dim - 1)] : 0u) << 16 * (e & 1);
       }
+      q[nc][st] = raw;
     }
   }
   // ---- units: each lane looks up one of the wave's next 64
