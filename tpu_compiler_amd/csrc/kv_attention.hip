@@ -155,7 +155,7 @@ constexpr int kJoinWaves = 16;
 // 6.0); for one of 131072, 143 MB, 28 us and 4.5 for the join.  Many rows: the vector ALU.  A unit costs a wave 80 instructions to unpack and
 // 7 a score (two fused products, half a maximum, an exponential, a sum, a step, an offset, half a conversion), 235 for 32 rows against 32
 // matrix instructions of 16 cycles; 8192 tokens of 32 heads, causal, 0.55 TFLOP, take 590 us, 930 TFLOP/s, 76 % of a large float16 product,
-// with the vector ALU busy for 83 % of the time and the matrix unit for 37 %.  More rows a wave would amortise unpacking, but 48 of 128 channels need the queries in LDS,
+// with the vector ALU busy for 80 % of the time and the matrix unit for 36 %.  More rows a wave would amortise unpacking, but 48 of 128 channels need the queries in LDS,
 // all registers, and gained 2 %; fewer, 16, have three waves a SIMD and take 709 us.
 // In between, latency: a SIMD with one wave issues a vector instruction every eight clocks instead of four to five, and a unit of 32 rows takes it
 // 0.95 us, where two waves take 1.13 for one each.  Multiplying the next unit's keys before this one's scores, and handing on its params, took nothing
