@@ -350,26 +350,31 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
 #pragma unroll
     for (int b = 0; b < OB; ++b) o[b][nc] = (float4v){0, 0, 0, 0};
   }
-  float v_scale = 1;            // steps of the values are taken times this power of two: 2^8 to 2^10 for the largest so far
-  bool scaled = false;
-  constexpr float kStepLimit = 1024, kLag = 5;   // weights up to 2^5 (of a maximum that lags), times steps up to 2^10: below float16's 65504
+  // Steps of the values are taken times a power of two, the same for a wave and in scalar registers: 2^8 to 2^10 for the largest so far,
+  // chosen by the first that is not zero.  Weights up to 2^5 (of a maximum that lags) times these are below float16's 65504.
+  const auto power = [](int e) { return __uint_as_float((uint32_t)min(max(e + 127, 0), 254) << 23); };
+  int v_exp = 0;
+  float v_scale = 1, step_limit = 0;
+  constexpr int kStepLimit = 10;
+  constexpr float kLag = 5;
 
   __shared__ __attribute__((aligned(16))) float params[kAttentionWaves][128];
   const int window = a.window ? a.window : kMostTokens;
   // A maximum or a step has gone up, which it seldom does after the first units: what has been summed, and this unit's scores, relative to
   // the new ones.
   const auto rescale = [&](float v_step, float (&high)[NC], float4v (&s)[2][NC], float (&vs)[8]) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) v_step = fmaxf(v_step, __shfl_xor(v_step, d));
+    const uint32_t most = wave_max(__float_as_uint(v_step));    // numbers that are not negative are in order as integers
     float v_change = 1;
-    if (v_step * v_scale > kStepLimit || !scaled) {
-      scaled = true;
-      const float now = ldexpf(1.0f, min(8 - ((int)(__float_as_uint(v_step) >> 23) - 127), 99));
-      v_change = now / v_scale;
-      v_scale = now;
-    }
+    if (most > __float_as_uint(step_limit)) {
+      const int now = min(8 - ((int)(most >> 23) - 127), 99);
+      v_change = power(now - v_exp);
+      v_exp = now;
+      v_scale = power(now);
+      step_limit = power(kStepLimit - now);
+      if (lane >= 32) params[wave][lane] = v_step * v_scale;    // from the step itself: with the scale so far it may be infinite
 #pragma unroll
-    for (int j = 0; j < 8; ++j) vs[j] *= v_change;
+      for (int h = 0; h < 2; ++h) *(float4v *)(vs + h * 4) = *(const float4v *)&params[wave][32 + h * 16 + g * 4];
+    }
 #pragma unroll
     for (int nc = 0; nc < NC; ++nc) {
       high[nc] = fmaxf(high[nc], __shfl_xor(high[nc], 16));
@@ -388,7 +393,7 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
   };
   const auto softmax = [&](int t0, float v_step, float (&ks)[8], float (&km)[8], float (&vs)[8], float (&vm)[8], float4v (&s)[2][NC], uint4v (&p)[NC]) {
     const bool all = t0 + kUnitTokens - 1 <= p_lo && (t0 > p_hi - window || t0 + kUnitTokens - 1 < a.sinks);
-    bool rise = v_step * v_scale > kStepLimit;
+    bool rise = v_step > step_limit;
     const auto scores = [&](const float (&top)[NC]) {           // s: x - top
 #pragma unroll
       for (int nc = 0; nc < NC; ++nc)
@@ -518,7 +523,7 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
   }
 
   // ---- results: channels 16 b + 4 g + 0..3 of a row in each lane
-  const float back = 0x1p24f / v_scale;
+  const float back = ldexpf(1.0f, 24 - v_exp);
 #pragma unroll
   for (int nc = 0; nc < NC; ++nc) {
     total[nc] += __shfl_xor(total[nc], 16);
