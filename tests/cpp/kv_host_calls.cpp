@@ -1,0 +1,124 @@
+// The host side of the key/value cache's calls, with no device: this program stands in for the runtime's functions and notes what the
+// library asks of them and on which device.  `kv_host_calls <case>` exits with 0 when that is right.
+#define __HIP_PLATFORM_AMD__
+#include <hip/hip_runtime_api.h>
+
+#include <cstdint>
+#include <cstdio>
+#include <cstdlib>
+#include <cstring>
+#include <functional>
+#include <stdexcept>
+#include <string>
+#include <vector>
+
+#include "tpuhip.h"
+
+namespace {
+struct Note {
+  std::string what;
+  int device;
+  size_t size;                 // bytes, or workgroups
+};
+std::vector<Note> notes;
+int current = 0;
+bool capturing = false;
+dim3 grid, block;
+void note(const char *what, size_t size = 0) { notes.push_back({what, current, size}); }
+size_t count(const char *what) {
+  size_t n = 0;
+  for (auto &x : notes) n += x.what == what;
+  return n;
+}
+}  // namespace
+
+extern "C" {
+hipError_t hipGetDeviceCount(int *n) { return *n = 2, hipSuccess; }
+hipError_t hipSetDevice(int d) { return current = d, hipSuccess; }
+hipError_t hipGetDevicePropertiesR0600(hipDeviceProp_tR0600 *p, int) {
+  memset(p, 0, sizeof *p);
+  strcpy(p->gcnArchName, "gfx950");
+  p->multiProcessorCount = 256;
+  return hipSuccess;
+}
+hipError_t hipGetSymbolAddress(void **p, const void *s) { return *p = const_cast<void *>(s), hipSuccess; }
+hipError_t hipStreamCreateWithFlags(hipStream_t *s, unsigned) { return *s = (hipStream_t)malloc(1), hipSuccess; }
+hipError_t hipStreamDestroy(hipStream_t s) { return free((void *)s), hipSuccess; }
+hipError_t hipStreamSynchronize(hipStream_t) { return note("wait"), hipSuccess; }
+hipError_t hipStreamIsCapturing(hipStream_t, hipStreamCaptureStatus *s) {
+  return *s = capturing ? hipStreamCaptureStatusActive : hipStreamCaptureStatusNone, hipSuccess;
+}
+hipError_t hipMalloc(void **p, size_t bytes) { return note("malloc", bytes), *p = malloc(16), hipSuccess; }
+hipError_t hipFree(void *p) { return note("free"), free(p), hipSuccess; }
+hipError_t hipMemsetAsync(void *, int, size_t bytes, hipStream_t) { return note("memset", bytes), hipSuccess; }
+hipError_t hipGetLastError() { return hipSuccess; }
+hipError_t __hipPushCallConfiguration(dim3 g, dim3 b, size_t, hipStream_t) { return grid = g, block = b, hipSuccess; }
+hipError_t __hipPopCallConfiguration(dim3 *g, dim3 *b, size_t *shared, hipStream_t *s) {
+  return *g = grid, *b = block, *shared = 0, *s = nullptr, hipSuccess;
+}
+hipError_t hipLaunchKernel(const void *, dim3 g, dim3 b, void **, size_t, hipStream_t) {
+  if ((uint64_t)g.x * b.x > UINT32_MAX || g.y > 65535) return hipErrorInvalidValue;
+  return note("launch", (size_t)g.x * g.y), hipSuccess;
+}
+}
+
+namespace {
+void expect(bool held, const char *what) {
+  if (!held) throw std::runtime_error(what);
+}
+void check(int status) {
+  if (status != TPUHIP_OK) throw std::runtime_error(tpuhip_last_error());
+}
+
+struct Cache {
+  tpuhip_ctx *ctx = nullptr;
+  tpuhip_kv_cache *cache = nullptr;
+  explicit Cache(int device, int kv_heads = 2, int dim = 64, int pages = 64) {
+    check(tpuhip_ctx_create(device, &ctx));
+    const tpuhip_kv_desc d = {pages, 32, kv_heads, dim, 4};
+    check(tpuhip_kv_cache_create(ctx, &d, &cache));
+  }
+  ~Cache() {
+    tpuhip_kv_cache_destroy(ctx, cache);
+    tpuhip_ctx_destroy(ctx);
+  }
+};
+
+tpuhip_kv_attention_desc attention(int n_seq, int heads, int total, int max_q, int max_kv, int dim) {
+  return {n_seq, heads, TPUHIP_BF16, total, max_q, max_kv, 0, 0, 1 << 20, 1.0f, (int64_t)heads * dim, dim, (int64_t)heads * dim, dim};
+}
+int attend(tpuhip_ctx *ctx, const tpuhip_kv_cache *cache, const tpuhip_kv_attention_desc &d, bool table = true) {
+  static int32_t there[4];
+  static uint16_t q, out;
+  return tpuhip_kv_attention(ctx, cache, &d, &q, &out, there, there, table ? there : nullptr);
+}
+
+// no tokens at all: a launch that writes zeros, in every form of the kernel
+void no_tokens() {
+  for (int dim : {64, 128, 192, 256})
+    for (int q : {1, 5, 16, 40, 400, 20000}) {
+      Cache c(0, 2, dim);
+      notes.clear();
+      check(attend(c.ctx, c.cache, attention(3, 4, 3 * q, q, 0, dim), q % 2));
+      expect(count("launch") == 1, "not one launch");
+    }
+}
+}  // namespace
+
+int main(int argc, char **argv) {
+  const struct {
+    const char *name;
+    std::function<void()> run;
+  } cases[] = {{"no_tokens", no_tokens}};
+  try {
+    for (auto &c : cases)
+      if (argc == 2 && !strcmp(argv[1], c.name)) {
+        c.run();
+        return 0;
+      }
+    throw std::runtime_error("no such case");
+  } catch (const std::exception &e) {
+    fprintf(stderr, "%s\n", e.what());
+    return 1;
+  }
+}

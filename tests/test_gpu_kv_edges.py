@@ -4,7 +4,8 @@ import pytest
 
 import kv_bounds
 import kv_oracle as O
-from test_gpu_kv_cache import Sequences, ctx, rows  # noqa: F401 (a fixture)
+from test_gpu_kv_cache import Sequences, array, ctx, rows  # noqa: F401 (a fixture)
+from tpu_compiler_amd.kv_cache import DeviceArray, KVCache
 
 pytestmark = pytest.mark.gpu
 
@@ -32,3 +33,18 @@ def test_values_that_grow_from_nothing(ctx, bits, first, size, q_len, heads, kv_
     v[600:] = O.rounded(v[600:] * size, "bf16")
     q = rows(rng, q_len, heads, dim, "bf16", False)
     check(ctx, rng, q, [q_len], [k], [v], [n], bits, "bf16")
+
+
+@pytest.mark.parametrize("dim", [64, 128, 200])
+@pytest.mark.parametrize("q_len", [1, 20, 300])
+def test_sequences_that_are_all_empty(ctx, dim, q_len):
+    """no page and no token: zeros, by a table of no columns"""
+    cache = KVCache(ctx, 2, 2, dim, 4, 32)
+    q = array(ctx, np.ones((3 * q_len, 4, dim)), "bf16")
+    out = array(ctx, np.full((3 * q_len, 4, dim), 7.0), "bf16")
+    starts, lens = array(ctx, np.arange(4) * q_len, "i32"), array(ctx, np.zeros(3), "i32")
+    cache.attention(q, out, starts, lens, DeviceArray(ctx, (3, 0), "i32"))
+    assert not out.numpy().any()
+    cache.attention(q, out, starts, lens, DeviceArray(ctx, (3, 2), "i32"), max_q=q_len, max_kv=0)
+    assert not out.numpy().any()
+    cache.close()

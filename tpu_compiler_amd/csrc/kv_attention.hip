@@ -827,7 +827,7 @@ int tpuhip_kv_attention(tpuhip_ctx *ctx, const tpuhip_kv_cache *cache, const tpu
         splits = std::min(std::max(splits, ceil_div64(units, 128)), ceil_div64(units, 8 * NC));
         if (units <= kJoinInKernel * 24) splits = std::min<int64_t>(splits, kJoinInKernel / NC);
       }
-      splits = std::min(splits, std::max<int64_t>(1, (int64_t)kJoinBytes / row_bytes));
+      splits = std::max<int64_t>(1, std::min(splits, (int64_t)kJoinBytes / row_bytes));   // one also where there are no tokens at all
       if (splits > 1) {
         if (int rc = attention_workspace(ctx)) return rc;
         if (!ctx->join) splits = 1;
