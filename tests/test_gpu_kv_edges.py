@@ -48,3 +48,20 @@ def test_sequences_that_are_all_empty(ctx, dim, q_len):
     cache.attention(q, out, starts, lens, DeviceArray(ctx, (3, 2), "i32"), max_q=q_len, max_kv=0)
     assert not out.numpy().any()
     cache.close()
+
+
+@pytest.mark.parametrize("size", [1e6, 1e10, 1e25])
+@pytest.mark.parametrize("q_len,window,sinks", [(1, 40, 3), (1, 64, 0), (5, 40, 3), (70, 0, 0), (70, 33, 5)])
+@pytest.mark.parametrize("bits,dim", [(4, 64), (8, 128), (4, 160)])
+def test_large_values_where_a_query_does_not_look(ctx, bits, dim, size, q_len, window, sinks):
+    """finite numbers in hidden places, beside tokens that are seen in one unit: before the window, behind the first tokens, later than the query"""
+    rng = np.random.default_rng(2)
+    n = 300
+    k, v = (rows(rng, n, 2, dim, "bf16", False) for _ in "kv")
+    first = n - q_len
+    hidden = [t for t in (first - window - 1, first - window, sinks, sinks + 1) if window and sinks <= t <= first - window]
+    hidden += [n - 1, n - 17] if q_len > 20 else []
+    assert hidden
+    v[hidden] = O.rounded(v[hidden] * size, "bf16")
+    q = rows(rng, q_len, 4, dim, "bf16", False)
+    check(ctx, rng, q, [q_len], [k], [v], [n], bits, "bf16", window=window, sinks=sinks)

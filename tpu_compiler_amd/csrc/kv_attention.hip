@@ -85,6 +85,21 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
   return max(max(of(0), of(16)), max(of(32), of(48)));
 }
 
+// f over the four lanes of a column, 16 apart
+template <typename F>
+__device__ __forceinline__ float over_column(float v, F f) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return f(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float column_max(float v) {
+  return over_column(v, [](float x, float y) { return fmaxf(x, y); });
+}
+__device__ __forceinline__ float column_sum(float v) {
+  return over_column(v, [](float x, float y) { return x + y; });
+}
+
 // A tile of R rows of a sequence, the `slot`th of those of all sequences: which sequence, its first query, how many it has, the position
 // of the first.  A lane counts the tiles of a sequence; the host knows a bound of their number only, and tile is -1 where there are
 // fewer.  With one tile a sequence at most, the slot is the sequence.
@@ -350,38 +365,94 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
 #pragma unroll
     for (int b = 0; b < OB; ++b) o[b][nc] = (float4v){0, 0, 0, 0};
   }
-  // Steps of the values are taken times a power of two, the same for a wave and in scalar registers: 2^8 to 2^10 for the largest so far,
-  // chosen by the first that is not zero.  Weights up to 2^5 (of a maximum that lags) times these are below float16's 65504.
+  // Steps of the values are taken times a power of two, the same for a wave: 2^8 to 2^10 for the largest that any row has seen.  Weights up
+  // to 2^5 (of a maximum that lags) times these are below float16's 65504.  A row that has seen only far smaller ones, as the large ones
+  // are hidden from it, has a maximum that is lower by its `lift`, so that its weights are larger by a power of two (limit: kLag and that).
+  // An offset counts as a step of 2^-14 of it: what is rounded beside it is far below its own rounding, and its sum stays in bounds.
   const auto power = [](int e) { return __uint_as_float((uint32_t)min(max(e + 127, 0), 254) << 23); };
+  const auto exponent = [](uint32_t bits) { return (int)(bits >> 23) - 127; };
+  const auto size_of = [](float step, float offset) { return fmaxf(step, fabsf(offset) * 0x1p-14f); };   // of an offset that is a NaN, 0
   int v_exp = 0;
-  float v_scale = 1, step_limit = 0;
-  constexpr int kStepLimit = 10;
+  float v_scale = 1, size_limit = 0;                            // size_limit: a token above it may not fit; 0: none so far
+  uint32_t most_seen = 0;                                       // by any row; numbers that are not negative are in order as integers
+  bool uneven = false;                                          // whether rows have seen different ones: the largest of each is in row_size
+  constexpr int kMostSteps = 10, kLeastLift = 10, kMostLift = 100;
   constexpr float kLag = 5;
 
   __shared__ __attribute__((aligned(16))) float params[kAttentionWaves][128];
+  __shared__ float row_size[kAttentionWaves][NC * 16];
   const int window = a.window ? a.window : kMostTokens;
   // A maximum or a step has gone up, which it seldom does after the first units: what has been summed, and this unit's scores, relative to
-  // the new ones.
-  const auto rescale = [&](float v_step, float (&high)[NC], float4v (&s)[2][NC], float (&vs)[8]) {
-    const uint32_t most = wave_max(__float_as_uint(v_step));    // numbers that are not negative are in order as integers
+  // the new ones.  step, size: of the lane's token.
+  const auto rescale = [&](int t0, bool all, float step, float size, float (&high)[NC], float4v (&s)[2][NC], float (&vs)[8], const float (&vm)[8]) {
+    const auto steps = [&](float scale) {                       // from the steps themselves: with the scale so far they may be infinite
+      if (lane >= 32) params[wave][lane] = step * scale;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) *(float4v *)(vs + h * 4) = *(const float4v *)&params[wave][32 + h * 16 + g * 4];
+    };
+    const bool scaled = size_limit > 0;
+    float seen_size[NC];
+#pragma unroll
+    for (int nc = 0; nc < NC; ++nc) {
+      seen_size[nc] = uneven ? row_size[wave][nc * 16 + col] : __uint_as_float(most_seen);
+      high[nc] = column_max(high[nc]);
+    }
+    const int t = t0 + lane - 32;                               // the lane's token, and whether any row sees it
+    const bool there = lane >= 32 && t <= p_hi && (t > p_lo - window || t < a.sinks);
+    const uint32_t largest = wave_max(there ? __float_as_uint(size) : 0);
+    const auto least = [&] { return ~wave_max(there ? ~__float_as_uint(size) : 0); };
+    if (all || p_lo == p_hi) {                                  // all rows see the same of the unit
+      most_seen = max(most_seen, largest);
+#pragma unroll
+      for (int nc = 0; nc < NC; ++nc) seen_size[nc] = fmaxf(seen_size[nc], __uint_as_float(largest));
+    } else if (const uint32_t low = least(); exponent(largest) - exponent(low) < kLeastLift) {   // or about the same, if any: that there is more shows when it is above size_limit
+      uneven = true;
+      most_seen = max(most_seen, largest);
+#pragma unroll
+      for (int nc = 0; nc < NC; ++nc) seen_size[nc] = high[nc] > -INFINITY ? fmaxf(seen_size[nc], __uint_as_float(low)) : seen_size[nc];
+    } else {
+      uneven = true;
+      if (scaled) steps(1);
+      uint32_t most = 0;
+#pragma unroll
+      for (int nc = 0; nc < NC; ++nc) {
+        float sees = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sees = s[j / 4][nc][j & 3] > -INFINITY ? fmaxf(sees, size_of(vs[j], vm[j])) : sees;
+        seen_size[nc] = fmaxf(seen_size[nc], column_max(sees));
+        most = max(most, __float_as_uint(seen_size[nc]));
+      }
+      most_seen = max(most_seen, wave_max(most));
+    }
+    if (uneven)
+#pragma unroll
+      for (int nc = 0; nc < NC; ++nc) row_size[wave][nc * 16 + col] = seen_size[nc];
     float v_change = 1;
-    if (most > __float_as_uint(step_limit)) {
-      const int now = min(8 - ((int)(most >> 23) - 127), 99);
+    if (most_seen && (size_limit == 0 || exponent(most_seen) + v_exp >= kMostSteps)) {
+      const int now = min(8 - exponent(most_seen), 99);
       v_change = power(now - v_exp);
       v_exp = now;
       v_scale = power(now);
-      step_limit = power(kStepLimit - now);
-      if (lane >= 32) params[wave][lane] = v_step * v_scale;    // from the step itself: with the scale so far it may be infinite
-#pragma unroll
-      for (int h = 0; h < 2; ++h) *(float4v *)(vs + h * 4) = *(const float4v *)&params[wave][32 + h * 16 + g * 4];
     }
+    if (scaled) {
+      steps(v_scale);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) vs[j] *= v_scale;
+    }
+    if (!all) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) vs[j] = fminf(vs[j], 0x1p15f);   // of a hidden one, whose weight is 0
+    }
+    int most_lift = 0;
 #pragma unroll
     for (int nc = 0; nc < NC; ++nc) {
-      high[nc] = fmaxf(high[nc], __shfl_xor(high[nc], 16));
-      high[nc] = fmaxf(high[nc], __shfl_xor(high[nc], 32));
       const bool first = limit[nc] < 0, some = high[nc] > -INFINITY;
-      const float up = first ? some ? high[nc] : 0.0f : fmaxf(high[nc], 0.0f), change = first ? 1.0f : exp2_fast(-up);
-      limit[nc] = some ? kLag : limit[nc];
+      int lift = uneven && seen_size[nc] > 0 ? 8 - exponent(__float_as_uint(seen_size[nc])) - v_exp : 0;
+      lift = lift < kLeastLift ? 0 : min(lift, kMostLift);
+      most_lift = max(most_lift, lift);
+      const float up = (first ? some ? high[nc] : 0.0f : fmaxf(high[nc], limit[nc] - kLag)) - (float)lift, change = first ? 1.0f : exp2_fast(-up);
+      limit[nc] = some || !first ? kLag + (float)lift : limit[nc];
       top[nc] += up;
       total[nc] *= change;
       offsets[nc] *= change;
@@ -390,10 +461,11 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
 #pragma unroll
       for (int b = 0; b < OB; ++b) o[b][nc] *= change * v_change;
     }
+    if (most_seen) size_limit = power(kMostSteps - v_exp - (__any(most_lift) ? (int)wave_max(most_lift) : 0));
   };
-  const auto softmax = [&](int t0, float v_step, float (&ks)[8], float (&km)[8], float (&vs)[8], float (&vm)[8], float4v (&s)[2][NC], uint4v (&p)[NC]) {
+  const auto softmax = [&](int t0, float step, float size, float (&ks)[8], float (&km)[8], float (&vs)[8], float (&vm)[8], float4v (&s)[2][NC], uint4v (&p)[NC]) {
     const bool all = t0 + kUnitTokens - 1 <= p_lo && (t0 > p_hi - window || t0 + kUnitTokens - 1 < a.sinks);
-    bool rise = v_step > step_limit;
+    bool rise = (size > size_limit) & (lane >= 32);
     const auto scores = [&](const float (&top)[NC]) {           // s: x - top
 #pragma unroll
       for (int nc = 0; nc < NC; ++nc)
@@ -422,7 +494,7 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
       for (int j = 1; j < 8; ++j) high[nc] = fmaxf(high[nc], s[j / 4][nc][j & 3]);
       rise |= high[nc] > limit[nc];
     }
-    if (__builtin_expect(__any(rise), 0)) rescale(v_step, high, s, vs);
+    if (__builtin_expect(__any(rise), 0)) rescale(t0, all, step, size, high, s, vs, vm);
 #pragma unroll
     for (int nc = 0; nc < NC; ++nc) {
       float w[8];
@@ -449,14 +521,13 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
     const uint8_t *u = address(next);
     const int t0 = unit < 0 ? kMostTokens : list.block(i) * kUnitTokens;   // a page outside the cache: nothing is seen
     // a lane has the keys' (lanes 0..31) or the values' step and offset of one token; through LDS each gets those of its eight
+    if (lane >= 32 && t0 + lane - 32 > p_hi) param = 0;         // of no token yet
     float step = bf16_to_f32(param), offset = __uint_as_float(param & 0xFFFF0000);
+    const float size = size_of(step, offset);                   // of the values' lanes
     if (lane < 32) {
       step *= step_scale;
       offset *= offset_scale;
-    } else if (t0 + lane - 32 > p_hi) {
-      step = 0;                                                 // of no token yet
     }
-    const float v_step = lane < 32 ? 0.0f : step;
     params[wave][lane] = lane < 32 ? step : step * v_scale;
     params[wave][64 + lane] = offset;
     float ks[8], km[8], vs[8], vm[8];
@@ -498,7 +569,7 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
     // end its unit, before those of keys (a prompt of 8192 tokens: 595 us without, 582 with)
     __builtin_amdgcn_s_setprio(2);
     uint4v p[NC];
-    softmax(t0, v_step, ks, km, vs, vm, s, p);
+    softmax(t0, step, size, ks, km, vs, vm, s, p);
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int b = 0; b < U::kBlocks; ++b) {
@@ -523,14 +594,13 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
   }
 
   // ---- results: channels 16 b + 4 g + 0..3 of a row in each lane
-  const float back = ldexpf(1.0f, 24 - v_exp);
 #pragma unroll
   for (int nc = 0; nc < NC; ++nc) {
-    total[nc] += __shfl_xor(total[nc], 16);
-    total[nc] += __shfl_xor(total[nc], 32);
-    offsets[nc] += __shfl_xor(offsets[nc], 16);
-    offsets[nc] += __shfl_xor(offsets[nc], 32);
-    if (limit[nc] < 0) top[nc] = kNothing;
+    const int lift = limit[nc] > 0 ? (int)(limit[nc] - kLag) : 0;
+    const float down = power(-lift), back = ldexpf(1.0f, 24 - v_exp - lift);
+    total[nc] = column_sum(total[nc]) * down;
+    offsets[nc] = column_sum(offsets[nc]) * down;
+    top[nc] = limit[nc] < 0 ? kNothing : top[nc] + (float)lift;
 #pragma unroll
     for (int b = 0; b < OB; ++b) {
       const float f = U::kBits == 4 && b >= OB / 2 ? back / 16 : back;
