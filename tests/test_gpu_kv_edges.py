@@ -65,3 +65,18 @@ def test_large_values_where_a_query_does_not_look(ctx, bits, dim, size, q_len, w
     v[hidden] = O.rounded(v[hidden] * size, "bf16")
     q = rows(rng, q_len, 4, dim, "bf16", False)
     check(ctx, rng, q, [q_len], [k], [v], [n], bits, "bf16", window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("n,at", [(1, 0), (40, 39), (300, 3), (300, 150), (5000, 4999), (9000, 70)])
+def test_scores_far_below_zero(ctx, n, at):
+    """the largest of them is what the others are relative to, however low it is: one of -2.4e34 among others of -2.4e35, which is far more
+    apart than the roundings of such numbers, has all the weight, and its values come back as they are held"""
+    rng = np.random.default_rng(3)
+    k, v = np.full((n, 1, 64), 3e17, np.float32), rows(rng, n, 1, 64, "bf16", False)
+    k[at] = 3e16
+    q = np.full((1, 2, 64), -1e17, np.float32)
+    k, q = O.rounded(k, "bf16"), O.rounded(q, "bf16")
+    s = Sequences(ctx, rng, [n], 1, 64, 4, 32, k=[k], v=[v])
+    got = s.attend(q, [1], "bf16")
+    s.cache.close()
+    assert np.array_equal(got[0], np.repeat(O.rounded(O.values(v[at], 4), "bf16").astype(np.float64), 2, 0))

@@ -152,7 +152,7 @@ struct UnitList {
 
 constexpr int kAttentionWaves = 4, kXcds = 8;
 constexpr int kMostTokens = 1 << 30;  // of a sequence: sums and differences of two positions are ints
-constexpr float kNothing = -1e30f;   // the maximum of no scores
+constexpr float kNothing = -__FLT_MAX__;   // the maximum of no scores: below that of any
 constexpr int kJoinAtOnce = 8;       // splits whose sums are loaded together
 constexpr int kJoinWaves = 16;
 
