@@ -80,3 +80,19 @@ def test_scores_far_below_zero(ctx, n, at):
     got = s.attend(q, [1], "bf16")
     s.cache.close()
     assert np.array_equal(got[0], np.repeat(O.rounded(O.values(v[at], 4), "bf16").astype(np.float64), 2, 0))
+
+
+@pytest.mark.parametrize("n,at", [(70, 3), (70, 66), (64, 40), (300, 150)])
+@pytest.mark.parametrize("q_len", [1, 20])
+def test_a_row_that_cannot_be_held_shows_whatever_its_weight(ctx, n, at, q_len):
+    """a query sees values that are NaN with a weight that 32 bits do not hold: not a number, in a unit that is seen as a whole or in part"""
+    rng = np.random.default_rng(4)
+    k, v = (rows(rng, n, 1, 64, "bf16", False) for _ in "kv")
+    q = np.abs(rows(rng, q_len, 2, 64, "bf16", False))
+    k[:], k[at] = 0, -100
+    v[at] = np.nan
+    s = Sequences(ctx, rng, [n], 1, 64, 4, 32, k=[k], v=[v])
+    got = s.attend(q, [q_len], "bf16")
+    s.cache.close()
+    sees = n - q_len + np.arange(q_len) >= at
+    assert np.isnan(got[sees]).all() and not np.isnan(got[~sees]).any()

@@ -506,9 +506,10 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
       if (all) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) offsets[nc] = __builtin_fmaf(w[j], vm[j], offsets[nc]);
-      } else {                                                  // what is masked may be a NaN
+      } else {                                                  // what is masked may be a NaN, which is to show where it is not, however small its weight
 #pragma unroll
-        for (int j = 0; j < 8; ++j) offsets[nc] = w[j] != 0 ? __builtin_fmaf(w[j], vm[j], offsets[nc]) : offsets[nc];
+        for (int j = 0; j < 8; ++j)
+          offsets[nc] = s[j / 4][nc][j & 3] != -INFINITY ? __builtin_fmaf(w[j], vm[j], offsets[nc]) : offsets[nc];
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j) w[j] *= vs[j];
