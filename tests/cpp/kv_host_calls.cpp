@@ -103,13 +103,33 @@ void no_tokens() {
       expect(count("launch") == 1, "not one launch");
     }
 }
+
+// a context's first attention to another one's cache, on a thread where another device is current: its workspace is its device's
+void workspace_device() {
+  Cache c(1);
+  tpuhip_ctx *other = nullptr;
+  check(tpuhip_ctx_create(1, &other));
+  (void)hipSetDevice(0);
+  notes.clear();
+  check(attend(other, c.cache, attention(1, 4, 1, 1, 4096, 64)));
+  expect(count("malloc") == 1 && count("memset") == 1 && count("launch") >= 1, "no splits");
+  (void)hipSetDevice(0);
+  static uint16_t k, v;
+  static int32_t slot;
+  const tpuhip_kv_rows rows = {1, TPUHIP_BF16, &k, &v, 128, 64, 128, 64};
+  check(tpuhip_kv_write(other, c.cache, &rows, &slot));
+  (void)hipSetDevice(0);
+  check(tpuhip_kv_read(other, c.cache, &rows, &slot));
+  for (auto &n : notes) expect(n.device == 1, n.what.c_str());
+  check(tpuhip_ctx_destroy(other));
+}
 }  // namespace
 
 int main(int argc, char **argv) {
   const struct {
     const char *name;
     std::function<void()> run;
-  } cases[] = {{"no_tokens", no_tokens}};
+  } cases[] = {{"no_tokens", no_tokens}, {"workspace_device", workspace_device}};
   try {
     for (auto &c : cases)
       if (argc == 2 && !strcmp(argv[1], c.name)) {

@@ -846,6 +846,7 @@ int tpuhip_kv_attention(tpuhip_ctx *ctx, const tpuhip_kv_cache *cache, const tpu
                  "%s: rows of the result overlap", what);
   TPUHIP_REQUIRE(q != out, "%s: the result takes the queries' place", what);
   TPUHIP_REQUIRE((uintptr_t)q % 2 == 0 && (uintptr_t)out % 2 == 0, "%s: q or out does not begin at an element", what);
+  TPUHIP_CHECK_HIP(hipSetDevice(ctx->device));   // of the workspace, and of launches on its default stream
   AttentionArgs a{};
   a.data = cache->data;
   a.q_starts = q_starts;

@@ -557,6 +557,7 @@ int tpuhip_kv_write(tpuhip_ctx *ctx, tpuhip_kv_cache *cache, const tpuhip_kv_row
   RowsArgs a{};
   if (int rc = rows_args(ctx, cache, rows, slots, false, "tpuhip_kv_write", &a)) return rc;
   if (a.tokens == 0) return TPUHIP_OK;
+  TPUHIP_CHECK_HIP(hipSetDevice(ctx->device));
   return kv_dispatch(cache, [&](auto u) -> int {
     using U = decltype(u);
     const int64_t blocks = rows_blocks(ctx, &a);
@@ -576,6 +577,7 @@ int tpuhip_kv_read(tpuhip_ctx *ctx, const tpuhip_kv_cache *cache, const tpuhip_k
   RowsArgs a{};
   if (int rc = rows_args(ctx, cache, rows, slots, true, "tpuhip_kv_read", &a)) return rc;
   if (a.tokens == 0) return TPUHIP_OK;
+  TPUHIP_CHECK_HIP(hipSetDevice(ctx->device));
   return kv_dispatch(cache, [&](auto u) -> int {
     using U = decltype(u);
     const int64_t blocks = rows_blocks(ctx, &a);
