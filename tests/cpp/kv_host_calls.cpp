@@ -123,13 +123,31 @@ void workspace_device() {
   for (auto &n : notes) expect(n.device == 1, n.what.c_str());
   check(tpuhip_ctx_destroy(other));
 }
+
+// a cache that has been made can be used from any context: its pages are clear
+void pages_are_clear() {
+  tpuhip_ctx *ctx = nullptr;
+  check(tpuhip_ctx_create(0, &ctx));
+  notes.clear();
+  const tpuhip_kv_desc d = {4, 32, 2, 64, 4};
+  tpuhip_kv_cache *cache = nullptr;
+  check(tpuhip_kv_cache_create(ctx, &d, &cache));
+  size_t cleared = 0, waited = 0;
+  for (size_t i = 0; i < notes.size(); ++i) {
+    if (notes[i].what == "launch") cleared = i + 1;
+    if (notes[i].what == "wait") waited = i + 1;
+  }
+  expect(cleared && waited > cleared, "the call returned before its pages were clear");
+  check(tpuhip_kv_cache_destroy(ctx, cache));
+  check(tpuhip_ctx_destroy(ctx));
+}
 }  // namespace
 
 int main(int argc, char **argv) {
   const struct {
     const char *name;
     std::function<void()> run;
-  } cases[] = {{"no_tokens", no_tokens}, {"workspace_device", workspace_device}};
+  } cases[] = {{"no_tokens", no_tokens}, {"workspace_device", workspace_device}, {"pages_are_clear", pages_are_clear}};
   try {
     for (auto &c : cases)
       if (argc == 2 && !strcmp(argv[1], c.name)) {

@@ -527,7 +527,8 @@ int tpuhip_kv_cache_create(tpuhip_ctx *ctx, const tpuhip_kv_desc *desc, tpuhip_k
   if (int rc = attention_workspace(ctx)) return rc;
   if (int rc = tpuhip_malloc(ctx, (size_t)bytes, &data)) return rc;
   launch(ctx, kv_clear_kernel, dim3((unsigned)std::min<int64_t>(ceil_div64(bytes / 16, 256), 8192)), dim3(256), (uint4 *)data, bytes / 16);
-  const hipError_t e = hipGetLastError();
+  hipError_t e = hipGetLastError();
+  if (e == hipSuccess) e = hipStreamSynchronize(ctx->stream);   // the cache may be used from another context, whose stream does not wait for this one
   tpuhip_kv_cache *c = e == hipSuccess ? new (std::nothrow) tpuhip_kv_cache() : nullptr;
   if (!c) {
     (void)tpuhip_free(ctx, data);
