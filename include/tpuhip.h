@@ -565,7 +565,8 @@ int tpuhip_kv_read(tpuhip_ctx *ctx, const tpuhip_kv_cache *cache, const tpuhip_k
  * zeros where nothing is seen.  Head h reads the cache's head h * kv_heads / heads.  Token t lies in page
  * page_table[b * table_stride + t / page_tokens]; a page outside the cache holds nothing to be seen (entries before the
  * window need not be kept).  q_starts (n_seq + 1), kv_lens (n_seq), page_table are device memory; what they say is cut to
- * total_q, max_q queries a sequence, max_kv tokens.  Rows of out that belong to no sequence stay as they are; out shares no memory
+ * total_q, max_q queries a sequence, max_kv tokens.  A call has at most 65535 sequences and heads, max_q * heads of 2^29, max_kv of
+ * 2^30, and sequences * kv_heads (each sequence once for every 16 to 128 of its (query, shared head) pairs) below 2^24.  Rows of out that belong to no sequence stay as they are; out shares no memory
  * with q (workgroups that split a sequence read the queries again).
  * Scores, maxima and sums are 32-bit.  Queries are multiplied as float16 numbers times a power of two for each tile of at most 32
  * (query, head) pairs of a sequence, exactly as far as they are within 2^24 of the tile's largest; weights, times the values'

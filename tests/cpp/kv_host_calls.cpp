@@ -141,13 +141,42 @@ void pages_are_clear() {
   check(tpuhip_kv_cache_destroy(ctx, cache));
   check(tpuhip_ctx_destroy(ctx));
 }
+
+// many rows in one call: only those are refused that the launches cannot hold, and only for a launch that is made
+void many_rows() {
+  struct {
+    int n_seq, heads, max_q, max_kv, kv_heads, dim;
+  } const calls[] = {{1, 71, 60000, 60000, 1, 64},   {1, 64, 65536, 65536, 1, 64},   {1, 64, 1 << 20, 1 << 20, 1, 128},
+                     {50000, 64, 40, 40, 1, 128},    {40000, 32, 64, 4096, 8, 64},   {60000, 8, 300, 300, 1, 256},
+                     {65535, 8, 1, 131072, 8, 64},   {65535, 256, 1, 64, 256, 64}};
+  for (auto &x : calls) {
+    Cache c(0, x.kv_heads, x.dim);
+    notes.clear();
+    check(attend(c.ctx, c.cache, attention(x.n_seq, x.heads, x.n_seq * x.max_q, x.max_q, x.max_kv, x.dim)));
+    expect(count("launch") == 1, "not one launch");
+  }
+  Cache c(0, 2048, 64);
+  expect(attend(c.ctx, c.cache, attention(65535, 2048, 65535, 1, 64, 64)) == TPUHIP_ERR_INVALID, "2^27 tiles were not refused");
+  // few queries and long contexts: split, and joined by the last workgroups or by a launch
+  for (int max_kv : {4096, 1 << 20}) {
+    notes.clear();
+    check(attend(c.ctx, c.cache, attention(1, 2048, 1, 1, max_kv, 64)));
+    expect(count("launch") >= 1, "no launch");
+  }
+  Cache few(0, 2, 64);
+  notes.clear();
+  check(attend(few.ctx, few.cache, attention(1, 4, 1, 1, 1 << 20, 64)));
+  expect(count("launch") == 2, "many splits are joined by a launch");
+  notes.clear();
+  check(attend(few.ctx, few.cache, attention(65535, 4, 1, 1, 1 << 20, 64)));   // all but one of them without a query
+}
 }  // namespace
 
 int main(int argc, char **argv) {
   const struct {
     const char *name;
     std::function<void()> run;
-  } cases[] = {{"no_tokens", no_tokens}, {"workspace_device", workspace_device}, {"pages_are_clear", pages_are_clear}};
+  } cases[] = {{"no_tokens", no_tokens}, {"workspace_device", workspace_device}, {"pages_are_clear", pages_are_clear}, {"many_rows", many_rows}};
   try {
     for (auto &c : cases)
       if (argc == 2 && !strcmp(argv[1], c.name)) {

@@ -22,7 +22,7 @@ struct AttentionArgs {
   FastDiv split_count;
   FastDiv class_heads;          // cache heads of a class of XCDs
   int classes, works, n_seq, one_tile;   // works: workgroups of a class
-  int splits, chunk;            // a split takes `chunk` units of those that a wave's rows see
+  int splits, chunk;            // a split takes `chunk` units of those that a wave's rows see (where all waves of a workgroup have the same)
   float scale;
 };
 
@@ -188,8 +188,13 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
   if (work >= (uint32_t)a.works) return;
   uint32_t slot = a.class_heads.split(work);                   // the first tile of all heads, then the second one, ...
   const int kvh = (int)(work * a.classes + of_head);
-  const int split = (int)(slot - a.split_count.div(slot) * a.split_count.d);
-  slot = a.split_count.div(slot);
+  constexpr bool SPLIT = WR == 1;                              // the others are for rows enough: a tile's units are one workgroup's
+  int split = 0;
+  if constexpr (SPLIT) {
+    split = (int)slot;
+    slot = a.split_count.div(slot);
+    split -= (int)(slot * a.split_count.d);
+  }
   const Tile seq = Tile::find<16 * NC * WR>(a, (int)slot).uniform();
   const int tile = seq.tile, rows = seq.n * group;
   if (tile < 0) return;
@@ -197,10 +202,13 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
   if (WK == 1 && row0 >= rows) return;                         // the waves share nothing
   const int p_lo = seq.first + (int)a.group.div(row0), p_hi = seq.first + (int)a.group.div(max(min(row0 + 16 * NC, rows), 1) - 1);
   const UnitList list(a, p_lo, row0 < rows ? p_hi : -1);
-  int i = split * a.chunk;
-  const int end = min(list.count, i + a.chunk);
-  if (WR != 2 && split > 0 && i >= end) return;                // no such split: what joins them counts them the same way
-  const int splits = max(1, (list.count + a.chunk - 1) / a.chunk);   // that there are
+  int i = 0, end = list.count, splits = 1;
+  if constexpr (SPLIT) {
+    i = split * a.chunk;
+    end = min(end, i + a.chunk);
+    if (split > 0 && i >= end) return;                         // no such split: what joins them counts them the same way
+    splits = max(1, (list.count + a.chunk - 1) / a.chunk);     // that there are
+  }
   i += wave % WK;
 
   // ---- queries
@@ -609,20 +617,12 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
       for (int r = 0; r < 4; ++r) o[b][nc][r] = __builtin_fmaf(o[b][nc][r], f, offsets[nc]);
     }
   }
-  const int64_t between = (int64_t)a.total_q * a.heads, first_row = ((int64_t)kvh * a.total_q + seq.begin) * group, part_row = split * between + first_row;
-  // v[0..3]: four channels of a row's sums, or its result
-  const auto keep = [&](int row, int c0, float4v v, float high, float sum) {
-    float *to = a.part + (part_row + row) * DP + c0;
-    store2(to, v[0], v[1]);
-    store2(to + 2, v[2], v[3]);
-    if (c0 == 0) store2(a.part_ml + (part_row + row) * 2, high, sum);
-  };
   const auto result = [&](int row) {
     uint32_t h = row;
     const int token = (int)a.group.split(h);
     return a.out + (int64_t)(seq.begin + token) * a.out_token_stride + (int64_t)(kvh * group + (int)h) * a.out_head_stride;
   };
-  const auto write = [&](uint16_t *dst, int c0, float4v v) {
+  const auto write = [&](uint16_t *dst, int c0, float4v v) {   // four channels of a row's result
     const uint2u b = a.bf16 ? (uint2u){pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])} : (uint2u){pack_f16(v[0], v[1]), pack_f16(v[2], v[3])};
     if (c0 + 4 <= a.dim) {
       *(uint2u *)(dst + c0) = b;
@@ -637,19 +637,15 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
     for (int nc = 0; nc < NC; ++nc) {
       const int row = row0 + nc * 16 + col;
       if (row >= rows) continue;
-      if (splits > 1) {
+      uint16_t *dst = result(row);
+      const float inv = total[nc] != 0 ? 1.0f / total[nc] : 0.0f;
 #pragma unroll
-        for (int b = 0; b < OB; ++b) keep(row, b * 16 + g * 4, o[b][nc], top[nc], total[nc]);
-      } else {
-        uint16_t *dst = result(row);
-        const float inv = total[nc] != 0 ? 1.0f / total[nc] : 0.0f;
-#pragma unroll
-        for (int b = 0; b < OB; ++b) write(dst, b * 16 + g * 4, o[b][nc] * inv);
-      }
+      for (int b = 0; b < OB; ++b) write(dst, b * 16 + g * 4, o[b][nc] * inv);
     }
   } else {
     __shared__ float sums[kAttentionWaves][16][DP + 4];
     __shared__ float tops[kAttentionWaves][16], totals[kAttentionWaves][16];
+    const int64_t between = (int64_t)a.total_q * a.heads, first_row = ((int64_t)kvh * a.total_q + seq.begin) * group;
     constexpr int PARTS = 16 / WR;                               // threads a row
     const int r = threadIdx.x / PARTS % 16, first_wave = threadIdx.x / (PARTS * 16) * WK, part = threadIdx.x % PARTS;
 #pragma unroll
@@ -663,7 +659,7 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
       }
       __syncthreads();
       const int row = (tile * WR + first_wave / WK) * 16 * NC + nc * 16 + r;
-      if (row >= rows || split >= splits) continue;
+      if (row >= rows) continue;
       float high = tops[first_wave][r], w[WK], sum = 0;
 #pragma unroll
       for (int k = 1; k < WK; ++k) high = fmaxf(high, tops[first_wave + k][r]);
@@ -679,13 +675,17 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
         float4v v = {0, 0, 0, 0};
 #pragma unroll
         for (int k = 0; k < WK; ++k) v += *(const float4v *)&sums[first_wave + k][r][c] * w[k];
-        if (splits > 1)
-          keep(row, c, v, high, sum);
-        else
+        if (SPLIT && splits > 1) {
+          float *to = a.part + (split * between + first_row + row) * DP + c;
+          store2(to, v[0], v[1]);
+          store2(to + 2, v[2], v[3]);
+          if (c == 0) store2(a.part_ml + (split * between + first_row + row) * 2, high, sum);
+        } else {
           write(dst, c, v * inv);
+        }
       }
     }
-    if (WR > 1 || splits == 1 || !a.counters) return;
+    if (!SPLIT || splits == 1 || !a.counters) return;
     // The last of a tile's splits to end joins them.  Their sums went past the caches of their XCDs (store2), so that they are where every
     // XCD sees them when their wave's vmcnt is 0, and the counter goes up after that; they are read past the caches too.  A release and
     // an acquire of the whole device would write back and drop an L2 for each workgroup: 28 us more for 1024 of them.
@@ -739,19 +739,19 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
 // The splits of a row, joined: a workgroup a row, whose waves take every sixteenth split, a lane a channel of each 64.  Bound by latency: 64
 // splits of 64 rows, 2 MB, take 4.5 us with the gap before it (34 us with the attention, and 40 where the last workgroups join so many).  Few splits of
 // many rows are better joined there: 2 of 2048 rows take 68 us with the attention, and 97 with this kernel.
-template <typename U, int NC, int WR>
+template <typename U, int NC>
 __global__ __launch_bounds__(64 * kJoinWaves) void kv_join_kernel(AttentionArgs a) {
   constexpr int DP = U::kDim, C = (DP + 63) / 64, WAVES = kJoinWaves;
   __shared__ float sums[WAVES][C * 64], totals[WAVES];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kvh = blockIdx.y, group = (int)a.group.d;
-  constexpr int ROWS = 16 * NC, R = ROWS * WR;
+  constexpr int R = 16 * NC;
   const Tile seq = Tile::find<R>(a, blockIdx.x / R).uniform();
   const int tile = seq.tile;
   if (tile < 0) return;
   const int rows = seq.n * group, row = tile * R + (int)blockIdx.x % R;
   if (row >= rows) return;
-  const int row0 = row / ROWS * ROWS;
-  const UnitList list(a, seq.first + (int)a.group.div(row0), seq.first + (int)a.group.div(min(row0 + ROWS, rows) - 1));
+  const int row0 = tile * R;
+  const UnitList list(a, seq.first + (int)a.group.div(row0), seq.first + (int)a.group.div(min(row0 + R, rows) - 1));
   const int splits = max(1, (list.count + a.chunk - 1) / a.chunk);
   if (splits == 1) return;                                     // written already
   const int64_t between = (int64_t)a.total_q * a.heads, at = ((int64_t)kvh * a.total_q + seq.begin) * group + row;
@@ -886,44 +886,42 @@ int tpuhip_kv_attention(tpuhip_ctx *ctx, const tpuhip_kv_cache *cache, const tpu
       constexpr int NC = decltype(nc)::value, WR = decltype(wr)::value, R = 16 * NC * WR;
       a.one_tile = rows_max <= R;
       const int64_t slots = a.one_tile ? d->n_seq : std::min(ceil_div64(rows_max, R) * d->n_seq, (int64_t)a.total_q * group / R + d->n_seq);
-      const int64_t units = units_of(R);
-      const int64_t base = slots * kv_heads, row_bytes = (int64_t)a.total_q * a.heads * (U::kDim + 2) * 4;
-      int64_t splits = 1;
-      if (WR == 1) {
+      const int64_t base = slots * kv_heads, most = (UINT32_MAX / (64 * kAttentionWaves) - kXcds) / base;   // a launch has fewer than 2^32 threads
+      TPUHIP_REQUIRE(most >= 1, "%s: %d queries of %d sequences over %d heads in one call", what, a.total_q, d->n_seq, kv_heads);
+      a.splits = 1;
+      if constexpr (WR == 1) {
         // Two workgroups a CU, without more than are there at a time (three, two with twice the rows or wider ones), and none of more than
         // 128 units, as lengths may differ; but two units a wave at least, four with twice the rows, for a join takes as long (a wave takes
         // 1 us a unit, the join of two splits 1.6), and so few splits that the last one can join them rather than another kernel, where
         // these have six units a wave at most.
-        const int64_t there = (NC == 1 && U::kDim <= 128 ? 3 : 2) * num_cu;
-        splits = std::max<int64_t>(1, std::min(ceil_div64(2 * num_cu, base), there / base));
+        const int64_t units = units_of(R), there = (NC == 1 && U::kDim <= 128 ? 3 : 2) * num_cu;
+        int64_t splits = std::max<int64_t>(1, std::min(ceil_div64(2 * num_cu, base), there / base));
         splits = std::min(std::max(splits, ceil_div64(units, 128)), ceil_div64(units, 8 * NC));
         if (units <= kJoinInKernel * 24) splits = std::min<int64_t>(splits, kJoinInKernel / NC);
+        splits = std::min({splits, most, (int64_t)kJoinBytes / ((int64_t)a.total_q * a.heads * (U::kDim + 2) * 4)});
+        if (splits > 1) {
+          if (int rc = attention_workspace(ctx)) return rc;
+          if (!ctx->join) splits = 1;
+        }
+        splits = std::max<int64_t>(1, splits);                  // also where there are no tokens at all
+        a.chunk = std::max(round_up((int)ceil_div64(units, splits), kAttentionWaves), 1);
+        a.splits = (int)std::max<int64_t>(1, ceil_div64(units, a.chunk));
+        a.part_ml = (float *)((char *)ctx->join + kCounters * 4);
+        a.part = a.part_ml + (int64_t)a.splits * a.total_q * a.heads * 2;
       }
-      splits = std::max<int64_t>(1, std::min(splits, (int64_t)kJoinBytes / row_bytes));   // one also where there are no tokens at all
-      if (splits > 1) {
-        if (int rc = attention_workspace(ctx)) return rc;
-        if (!ctx->join) splits = 1;
-      }
-      a.chunk = (int)std::max<int64_t>(round_up((int)ceil_div64(units, splits), 4 / WR), 1);
-      a.splits = (int)std::max<int64_t>(1, ceil_div64(units, a.chunk));
-      const bool in_kernel = WR == 1 && a.splits <= kJoinInKernel && base <= kCounters;
+      const bool in_kernel = a.splits <= kJoinInKernel && base <= kCounters;
       a.counters = in_kernel ? (int *)ctx->join : nullptr;
-      a.part_ml = (float *)((char *)ctx->join + kCounters * 4);
-      a.part = a.part_ml + (int64_t)a.splits * a.total_q * a.heads * 2;
       a.classes = kv_heads % 8 == 0 ? 8 : kv_heads % 4 == 0 ? 4 : kv_heads % 2 == 0 ? 2 : 1;
       a.class_heads = FastDiv(kv_heads / a.classes);
       a.split_count = FastDiv(a.splits);
-      const int64_t works = slots * a.splits * (kv_heads / a.classes);
-      // a launch has fewer than 2^32 threads
-      TPUHIP_REQUIRE((works * a.classes + kXcds) * 64 * kAttentionWaves <= UINT32_MAX && slots * R * 64 * kJoinWaves <= UINT32_MAX,
-                     "%s: %d queries of %d sequences in one call", what, a.total_q, d->n_seq);
-      a.works = (int)works;
-      launch(ctx, kv_attention_kernel<U, NC, WR>, dim3((unsigned)(ceil_div64(works, kXcds / a.classes) * kXcds)), dim3(64 * kAttentionWaves), a);
+      a.works = (int)(slots * a.splits * (kv_heads / a.classes));
+      launch(ctx, kv_attention_kernel<U, NC, WR>, dim3((unsigned)(ceil_div64(a.works, kXcds / a.classes) * kXcds)), dim3(64 * kAttentionWaves), a);
       TPUHIP_CHECK_HIP(hipGetLastError());
-      if (a.splits > 1 && !in_kernel) {
-        launch(ctx, kv_join_kernel<U, NC, WR>, dim3((unsigned)(slots * R), (unsigned)kv_heads), dim3(64 * kJoinWaves), a);
-        TPUHIP_CHECK_HIP(hipGetLastError());
-      }
+      if constexpr (WR == 1)
+        if (a.splits > 1 && !in_kernel) {   // a workgroup a row: no more than kJoinBytes have room for, and R - 1 past the end of each sequence
+          launch(ctx, kv_join_kernel<U, NC>, dim3((unsigned)(slots * R), (unsigned)kv_heads), dim3(64 * kJoinWaves), a);
+          TPUHIP_CHECK_HIP(hipGetLastError());
+        }
       return TPUHIP_OK;
     };
     // The form of the kernel: 16 NC rows a wave, WR of the four waves with rows of their own.  Wide waves unpack codes less often, waves
