@@ -1,0 +1,109 @@
+"""The Python side of the key/value cache: what calls are made with, and which are refused.  A stand-in for the library notes its calls, so
+no device is needed."""
+import ctypes as C
+
+import pytest
+
+from tpu_compiler_amd import capi
+from tpu_compiler_amd.kv_cache import KVCache
+
+
+class Library:
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        def call(*args):
+            self.calls.append((name,) + args)
+            if name == "tpuhip_kv_cache_create":
+                args[2]._obj.value = 0x1000
+            if name == "tpuhip_malloc":
+                args[2]._obj.value = 0x2000
+            return 0
+        return call
+
+    def names(self):
+        return [c[0] for c in self.calls]
+
+
+def context():
+    ctx = capi.Context.__new__(capi.Context)
+    ctx._begin(Library(), 0, C.c_void_p(0x10))
+    return ctx
+
+
+class Array:
+    """device memory of some shape"""
+    ptr = 0x5000
+
+    def __init__(self, shape, dtype, stride=None):
+        self.shape, self.dtype, self._stride = shape, dtype, stride
+
+    def data_ptr(self):
+        return self.ptr
+
+    def stride(self):
+        if self._stride:
+            return self._stride
+        s = [1]
+        for n in self.shape[:0:-1]:
+            s.append(s[-1] * n)
+        return tuple(s[::-1])
+
+
+def plans(cache, rows=3, seqs=2, pages=4):
+    k, v, q, out = (Array((rows, h, 64), "bf16") for h in (2, 2, 4, 4))
+    slots = Array((rows,), "i32")
+    return [cache.plan_write(k, v, slots), cache.plan_read(slots, k, v),
+            cache.plan_attention(q, out, Array((seqs + 1,), "i32"), Array((seqs,), "i32"), Array((seqs, pages), "i32"))]
+
+
+def test_a_plan_passes_the_handles_of_its_cache_and_context():
+    ctx = context()
+    cache = KVCache(ctx, 8, 2, 64, 4, 32)
+    for plan, name in zip(plans(cache), ("tpuhip_kv_write", "tpuhip_kv_read", "tpuhip_kv_attention")):
+        for _ in range(2):
+            plan()
+            call = ctx.lib.calls[-1]
+            assert call[0] == name and call[1].value == 0x10 and call[2].value == 0x1000
+
+
+@pytest.mark.parametrize("what", ["cache", "context"])
+def test_a_plan_whose_cache_or_context_is_closed_refuses(what):
+    ctx = context()
+    cache = KVCache(ctx, 8, 2, 64, 4, 32)
+    made = plans(cache)
+    (cache if what == "cache" else ctx).close()
+    before = len(ctx.lib.calls)
+    for plan in made:
+        with pytest.raises(capi.TpuHipError, match="closed"):
+            plan()
+    assert len(ctx.lib.calls) == before
+
+
+def test_a_context_that_closes_frees_its_caches_first():
+    ctx = context()
+    kept = KVCache(ctx, 8, 2, 64, 4, 32)
+    gone = KVCache(ctx, 8, 2, 64, 4, 32)
+    gone.close()
+    ctx.close()
+    assert ctx.lib.names().count("tpuhip_kv_cache_destroy") == 2
+    assert ctx.lib.names()[-1] == "tpuhip_ctx_destroy" and ctx.lib.names()[-2] == "tpuhip_kv_cache_destroy"
+    kept.close()
+    assert ctx.lib.names()[-1] == "tpuhip_ctx_destroy"
+
+
+def test_a_plan_whose_array_is_freed_refuses():
+    from tpu_compiler_amd.kv_cache import DeviceArray
+    ctx = context()
+    cache = KVCache(ctx, 8, 2, 64, 4, 32)
+    k, v, slots = DeviceArray(ctx, (3, 2, 64), "bf16"), DeviceArray(ctx, (3, 2, 64), "bf16"), DeviceArray(ctx, (3,), "i32")
+    write = cache.plan_write(k, v, slots)
+    write()
+    v.free()
+    before = len(ctx.lib.calls)
+    with pytest.raises(capi.TpuHipError, match="freed"):
+        write()
+    with pytest.raises(capi.TpuHipError, match="freed"):
+        cache.plan_write(k, v, slots)
+    assert len(ctx.lib.calls) == before

@@ -2,6 +2,7 @@
 conveniences.  Every call goes to the HIP library; nothing here computes."""
 import ctypes as C
 import struct
+import weakref
 
 import numpy as np
 
@@ -422,16 +423,20 @@ class Context:
     one), made by the HIP runtime that the library runs on: in a process with torch, torch's if that was imported first."""
 
     def __init__(self, device=0, stream=None):
-        self.lib = bind()
-        self.device = device
-        h = C.c_void_p()
-        check(self.lib, self.lib.tpuhip_ctx_create(device, C.byref(h)) if stream is None else
-              self.lib.tpuhip_ctx_create_on_stream(device, stream, C.byref(h)))
-        self.h = h
-        self._ops = _Ops(self.lib)
+        lib, h = bind(), C.c_void_p()
+        check(lib, lib.tpuhip_ctx_create(device, C.byref(h)) if stream is None else
+              lib.tpuhip_ctx_create_on_stream(device, stream, C.byref(h)))
+        self._begin(lib, device, h)
+        self._ops = _Ops(lib)
+
+    def _begin(self, lib, device, h):
+        self.lib, self.device, self.h = lib, device, h
+        self.caches = weakref.WeakSet()      # key/value caches made by this context, which end with it
 
     def close(self):
         if self.h:
+            for c in list(self.caches):
+                c.close()
             self.lib.tpuhip_ctx_destroy(self.h)
             self.h = None
 

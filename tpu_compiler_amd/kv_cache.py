@@ -98,14 +98,25 @@ def _ints(x, what, ctx, shape):
 
 
 class _Call:
-    """A checked call, to be made any number of times on the same arrays (it keeps them alive)."""
+    """A checked call, to be made any number of times on the same arrays (it keeps them alive) while these, the cache and its context are
+    there."""
 
     def __init__(self, cache, fn, args, keep):
-        self._cache, self._fn, self._args, self._keep = cache, fn, args, keep
+        self._cache, self._ctx, self._fn, self._args, self._keep = cache, cache.ctx, fn, args, keep
+        self._arrays = [x for x in keep if isinstance(x, DeviceArray)]
+        self._check()
+
+    def _check(self):
+        if not self._cache.h or not self._ctx.h:
+            _refuse("the %s is closed" % ("context" if not self._ctx.h else "cache"))
+        for x in self._arrays:
+            if not x.ptr:
+                _refuse("an array of the call has been freed")
 
     def __call__(self):
-        if rc := self._fn(*self._args):
-            self._cache.ctx._ck(rc)
+        self._check()
+        if rc := self._fn(self._ctx.h, self._cache.h, *self._args):
+            self._ctx._ck(rc)
 
 
 class KVCache:
@@ -118,13 +129,14 @@ class KVCache:
         d = capi.KVDesc(self.pages, self.page_tokens, self.kv_heads, self.head_dim, self.bits)
         self.h = C.c_void_p()
         ctx._ck(ctx.lib.tpuhip_kv_cache_create(ctx.h, C.byref(d), C.byref(self.h)))
+        self._made_by = ctx                  # closes this cache before it ends
+        ctx.caches.add(self)
         self.nbytes = int(ctx.lib.tpuhip_kv_cache_bytes(C.byref(d)))
 
     def close(self):
         if self.h:
             h, self.h = self.h, None
-            if self.ctx.h:
-                self.ctx._ck(self.ctx.lib.tpuhip_kv_cache_destroy(self.ctx.h, h))
+            self._made_by._ck(self._made_by.lib.tpuhip_kv_cache_destroy(self._made_by.h, h))
 
     def __del__(self):
         try:
@@ -140,7 +152,7 @@ class KVCache:
             _refuse("k and v: of one type and length")
         at = _ints(slots, "slots", self.ctx, (tokens,))
         d = capi.KVRows(tokens, TYPES[dtype], k.data_ptr(), v.data_ptr(), *ks, *vs)
-        return _Call(self, fn, (self.ctx.h, self.h, d, at), (k, v, slots))
+        return _Call(self, fn, (d, at), (k, v, slots))
 
     def plan_write(self, k, v, slots):
         """a call that quantises rows k, v [tokens, kv_heads, head_dim] into slots [tokens] (int32; -1: passed over)"""
@@ -167,7 +179,7 @@ class KVCache:
                                  most * self.page_tokens if max_kv is None else int(max_kv), int(window), int(sinks),
                                  int(page_table.stride()[0]) if n > 1 else most,
                                  self.head_dim ** -0.5 if scale is None else float(scale), *qs, *outs)
-        return _Call(self, self.ctx.lib.tpuhip_kv_attention, (self.ctx.h, self.h, d, q.data_ptr(), out.data_ptr(), *args),
+        return _Call(self, self.ctx.lib.tpuhip_kv_attention, (d, q.data_ptr(), out.data_ptr(), *args),
                      (q, out, q_starts, kv_lens, page_table))
 
     def write(self, k, v, slots):
