@@ -107,3 +107,20 @@ def test_a_plan_whose_array_is_freed_refuses():
     with pytest.raises(capi.TpuHipError, match="freed"):
         cache.plan_write(k, v, slots)
     assert len(ctx.lib.calls) == before
+
+
+def attend(cache, table, **how):
+    q, out = (Array((2, 4, 64), "bf16") for _ in range(2))
+    return cache.plan_attention(q, out, Array((table.shape[0] + 1,), "i32"), Array((table.shape[0],), "i32"), table, **how)
+
+
+def test_no_more_tokens_than_a_page_table_lists():
+    """rows of a table may be parts of longer ones: what lies behind them is none of the table's, and past the last row no memory at all"""
+    ctx = context()
+    cache = KVCache(ctx, 8, 2, 64, 4, 32)
+    for table in (Array((2, 4), "i32"), Array((2, 4), "i32", (40, 1)), Array((1, 4), "i32", (40, 1))):
+        attend(cache, table, max_kv=128)()
+        call = ctx.lib.calls[-1]
+        assert call[3].max_kv == 128 and call[3].table_stride == (table.stride()[0] if table.shape[0] > 1 else 4)
+        with pytest.raises(capi.TpuHipError, match="4 pages"):
+            attend(cache, table, max_kv=129)

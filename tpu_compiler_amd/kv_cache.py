@@ -175,8 +175,10 @@ class KVCache:
         n, most = (int(page_table.shape[0]), int(page_table.shape[1])) if len(page_table.shape) == 2 else (0, 0)
         args = [_ints(q_starts, "q_starts", self.ctx, (n + 1,)), _ints(kv_lens, "kv_lens", self.ctx, (n,)),
                 _ints(page_table, "page_table", self.ctx, (n, most))]
-        d = capi.KVAttentionDesc(n, heads, TYPES[dtype], total, total if max_q is None else int(max_q),
-                                 most * self.page_tokens if max_kv is None else int(max_kv), int(window), int(sinks),
+        max_kv = most * self.page_tokens if max_kv is None else int(max_kv)
+        if max_kv > most * self.page_tokens:      # the library sees the distance of the table's rows only, which may be parts of longer ones
+            _refuse("max_kv: %d tokens in %d pages of %d" % (max_kv, most, self.page_tokens))
+        d = capi.KVAttentionDesc(n, heads, TYPES[dtype], total, total if max_q is None else int(max_q), max_kv, int(window), int(sinks),
                                  int(page_table.stride()[0]) if n > 1 else most,
                                  self.head_dim ** -0.5 if scale is None else float(scale), *qs, *outs)
         return _Call(self, self.ctx.lib.tpuhip_kv_attention, (d, q.data_ptr(), out.data_ptr(), *args),
