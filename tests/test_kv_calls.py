@@ -124,3 +124,40 @@ def test_no_more_tokens_than_a_page_table_lists():
         assert call[3].max_kv == 128 and call[3].table_stride == (table.stride()[0] if table.shape[0] > 1 else 4)
         with pytest.raises(capi.TpuHipError, match="4 pages"):
             attend(cache, table, max_kv=129)
+
+
+@pytest.mark.parametrize("n", [2 ** 31, 2 ** 32 + 4, -2 ** 31 - 1, 2 ** 40])
+def test_numbers_that_an_int_does_not_hold_are_refused(n):
+    """and not taken for what is left of them in 32 bits"""
+    ctx = context()
+    for place in range(5):
+        sizes = [8, 2, 64, 4, 32]
+        sizes[place] = n
+        with pytest.raises(capi.TpuHipError, match="int"):
+            KVCache(ctx, *sizes)
+    cache = KVCache(ctx, 8, 2, 64, 4, 32)
+    for name in ("max_q", "max_kv", "window", "sinks"):
+        with pytest.raises(capi.TpuHipError):
+            attend(cache, Array((2, 4), "i32"), **{name: n})
+    with pytest.raises(capi.TpuHipError, match="int"):
+        attend(cache, Array((2, 4), "i32", (n, 1)))
+    if n > 0:
+        with pytest.raises(capi.TpuHipError, match="int"):
+            cache.plan_write(Array((n, 2, 64), "bf16"), Array((n, 2, 64), "bf16"), Array((n,), "i32"))
+
+
+def test_a_table_of_more_pages_than_a_sequence_has():
+    """by default a call looks at no more than 2^30 tokens, the most there may be"""
+    ctx = context()
+    cache = KVCache(ctx, 8, 2, 64, 4, 1 << 20)
+    attend(cache, Array((2, 5000), "i32"))()
+    assert ctx.lib.calls[-1][3].max_kv == 1 << 30
+
+
+@pytest.mark.parametrize("values", [[2 ** 31], [-2 ** 31 - 1], [2 ** 32 + 3]])
+def test_integers_that_do_not_fit_are_not_uploaded(values):
+    from tpu_compiler_amd.kv_cache import DeviceArray
+    ctx = context()
+    with pytest.raises(capi.TpuHipError, match="int"):
+        DeviceArray.of(ctx, values, "i32")
+    DeviceArray.of(ctx, [2 ** 31 - 1, -2 ** 31], "i32")

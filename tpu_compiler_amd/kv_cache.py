@@ -25,7 +25,9 @@ class DeviceArray:
 
     @classmethod
     def of(cls, ctx, values, dtype):
-        """the values, rounded to the type"""
+        """the values, rounded to the type (bf16: of what float32 holds of them)"""
+        if dtype == "i32" and np.size(values) and not (-2 ** 31 <= np.min(values) and np.max(values) < 2 ** 31):
+            _refuse("values: no ints of 32 bits")
         a = cls(ctx, np.shape(values), dtype)
         if dtype == "bf16":
             bits = np.ascontiguousarray(values, np.float32).view(np.uint32).astype(np.uint64)
@@ -59,6 +61,14 @@ class DeviceArray:
 
 def _refuse(message):
     raise capi.TpuHipError(1, message)
+
+
+def _int(n, what):
+    """a number for a C int, which would take the low 32 bits of any"""
+    n = int(n)
+    if not -2 ** 31 <= n < 2 ** 31:
+        _refuse("%s: %d is no int of 32 bits" % (what, n))
+    return n
 
 
 def _type(x, what, allowed):
@@ -124,10 +134,10 @@ class KVCache:
     in slot page * page_tokens + t % page_tokens of the sequence's page number t // page_tokens; which page that is, is the caller's to say."""
 
     def __init__(self, ctx, pages, kv_heads, head_dim, bits=4, page_tokens=64):
-        self.ctx, self.pages, self.kv_heads, self.head_dim = ctx, int(pages), int(kv_heads), int(head_dim)
-        self.bits, self.page_tokens = int(bits), int(page_tokens)
-        d = capi.KVDesc(self.pages, self.page_tokens, self.kv_heads, self.head_dim, self.bits)
         self.h = C.c_void_p()
+        self.ctx, self.pages, self.kv_heads, self.head_dim = ctx, _int(pages, "pages"), _int(kv_heads, "kv_heads"), _int(head_dim, "head_dim")
+        self.bits, self.page_tokens = _int(bits, "bits"), _int(page_tokens, "page_tokens")
+        d = capi.KVDesc(self.pages, self.page_tokens, self.kv_heads, self.head_dim, self.bits)
         ctx._ck(ctx.lib.tpuhip_kv_cache_create(ctx.h, C.byref(d), C.byref(self.h)))
         self._made_by = ctx                  # closes this cache before it ends
         ctx.caches.add(self)
@@ -145,7 +155,7 @@ class KVCache:
             pass
 
     def _rows(self, fn, slots, k, v):
-        tokens = int(k.shape[0])
+        tokens = _int(k.shape[0], "tokens")
         ks, vs = _rows3(k, "k", self.ctx, self.kv_heads, self.head_dim), _rows3(v, "v", self.ctx, self.kv_heads, self.head_dim)
         dtype = _type(k, "k", tuple(TYPES))
         if _type(v, "v", tuple(TYPES)) != dtype or v.shape[0] != tokens:
@@ -175,11 +185,12 @@ class KVCache:
         n, most = (int(page_table.shape[0]), int(page_table.shape[1])) if len(page_table.shape) == 2 else (0, 0)
         args = [_ints(q_starts, "q_starts", self.ctx, (n + 1,)), _ints(kv_lens, "kv_lens", self.ctx, (n,)),
                 _ints(page_table, "page_table", self.ctx, (n, most))]
-        max_kv = most * self.page_tokens if max_kv is None else int(max_kv)
+        max_kv = min(most * self.page_tokens, 1 << 30) if max_kv is None else int(max_kv)   # a sequence has no more
         if max_kv > most * self.page_tokens:      # the library sees the distance of the table's rows only, which may be parts of longer ones
             _refuse("max_kv: %d tokens in %d pages of %d" % (max_kv, most, self.page_tokens))
-        d = capi.KVAttentionDesc(n, heads, TYPES[dtype], total, total if max_q is None else int(max_q), max_kv, int(window), int(sinks),
-                                 int(page_table.stride()[0]) if n > 1 else most,
+        d = capi.KVAttentionDesc(_int(n, "sequences"), _int(heads, "heads"), TYPES[dtype], _int(total, "queries"),
+                                 _int(total if max_q is None else max_q, "max_q"), _int(max_kv, "max_kv"), _int(window, "window"), _int(sinks, "sinks"),
+                                 _int(page_table.stride()[0] if n > 1 else most, "page_table: distance of rows"),
                                  self.head_dim ** -0.5 if scale is None else float(scale), *qs, *outs)
         return _Call(self, self.ctx.lib.tpuhip_kv_attention, (d, q.data_ptr(), out.data_ptr(), *args),
                      (q, out, q_starts, kv_lens, page_table))
