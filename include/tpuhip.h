@@ -553,7 +553,8 @@ typedef struct {
   int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
 } tpuhip_kv_rows;
 /* Quantises rows into the cache, row i at slots[i] (device memory).  A slot outside the cache is passed over (-1 for rows that are
- * padding); of two rows for one slot in a call either may stay. */
+ * padding).  The rows that a call has for one slot have to be the same: threads write them in no order, and what different ones leave
+ * there is a mixture of their codes, steps and offsets, which is neither.  Other slots do not feel it. */
 int tpuhip_kv_write(tpuhip_ctx *ctx, tpuhip_kv_cache *cache, const tpuhip_kv_rows *rows, const int32_t *slots);
 /* Reads rows back: m + s c, rounded once to the type.  Row i from slots[i]; zeros from a slot outside the cache. */
 int tpuhip_kv_read(tpuhip_ctx *ctx, const tpuhip_kv_cache *cache, const tpuhip_kv_rows *rows, const int32_t *slots);

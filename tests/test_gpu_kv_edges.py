@@ -96,3 +96,21 @@ def test_a_row_that_cannot_be_held_shows_whatever_its_weight(ctx, n, at, q_len):
     s.cache.close()
     sees = n - q_len + np.arange(q_len) >= at
     assert np.isnan(got[sees]).all() and not np.isnan(got[~sees]).any()
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("n", [40, 100, 20000])
+def test_a_slot_twice_for_the_same_row(ctx, bits, n):
+    """in one unit's run and outside of it, in one workgroup and in several"""
+    rng = np.random.default_rng(5)
+    cache = KVCache(ctx, -(-n // 32) + 1, 2, 80, bits, 32)
+    x, y = rows(rng, n, 2, 80, "bf16", False), rows(rng, n, 2, 80, "bf16", False)
+    which = np.concatenate([np.arange(n), rng.integers(0, n, n // 2), np.full(9, n // 3), [n - 1]])
+    which = np.concatenate([which[:n // 2], which[n:], which[n // 2:n]])
+    cache.write(array(ctx, x[which], "bf16"), array(ctx, y[which], "bf16"), array(ctx, which, "i32"))
+    got = [DeviceArray(ctx, (n + 8, 2, 80), "bf16") for _ in range(2)]
+    cache.read(array(ctx, np.arange(n + 8), "i32"), *got)
+    for a, b in zip(got, (x, y)):
+        held = a.numpy()
+        assert np.array_equal(held[:n], O.rounded(O.values(b, bits), "bf16")) and not held[n:].any()
+    cache.close()

@@ -165,7 +165,8 @@ class KVCache:
         return _Call(self, fn, (d, at), (k, v, slots))
 
     def plan_write(self, k, v, slots):
-        """a call that quantises rows k, v [tokens, kv_heads, head_dim] into slots [tokens] (int32; -1: passed over)"""
+        """a call that quantises rows k, v [tokens, kv_heads, head_dim] into slots [tokens] (int32; -1: passed over; a slot twice for the same
+        row only)"""
         return self._rows(self.ctx.lib.tpuhip_kv_write, slots, k, v)
 
     def plan_read(self, slots, k, v):
