@@ -1,10 +1,15 @@
 """Attention to the key/value cache where numbers are far apart, and lengths and calls at their ends."""
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 
 import kv_bounds
 import kv_oracle as O
-from test_gpu_kv_cache import Sequences, array, ctx, rows  # noqa: F401 (a fixture)
+from test_gpu_kv_cache import Sequences, Strided, array, ctx, rows  # noqa: F401 (a fixture)
+from tpu_compiler_amd import capi
 from tpu_compiler_amd.kv_cache import DeviceArray, KVCache
 
 pytestmark = pytest.mark.gpu
@@ -114,3 +119,45 @@ def test_a_slot_twice_for_the_same_row(ctx, bits, n):
         held = a.numpy()
         assert np.array_equal(held[:n], O.rounded(O.values(b, bits), "bf16")) and not held[n:].any()
     cache.close()
+
+
+def test_each_refusal_says_what_it_is(ctx):
+    """one thing wrong at a time, beside a call that is taken"""
+    cache = KVCache(ctx, 4, 2, 64, 4, 32)
+    q, out = (DeviceArray(ctx, (3, 4, 64), "bf16") for _ in range(2))
+    starts, lens, table = array(ctx, [0, 3], "i32"), array(ctx, [3], "i32"), array(ctx, [[0, 1]], "i32")
+    good = dict(q=q, out=out, q_starts=starts, kv_lens=lens, page_table=table)
+    other = lambda heads, dtype, n=3: DeviceArray(ctx, (n, heads, 64), dtype)
+    cache.attention(**good)
+    for change, says in ((dict(max_kv=65), "65 tokens in 2 pages"), (dict(max_kv=-1), "of -1 tokens"), (dict(max_q=-1), "at most -1 a sequence"),
+                         (dict(window=-1), "window of -1"), (dict(sinks=-1), "-1 first tokens"), (dict(scale=float("nan")), "not finite"),
+                         (dict(scale=float("inf")), "not finite"), (dict(q=other(5, "bf16"), out=other(5, "bf16")), "5 heads over"),
+                         (dict(q=other(4, "f32"), out=other(4, "f32")), "of type bf16 or f16"), (dict(out=other(4, "f16")), "one type and length"),
+                         (dict(out=other(4, "bf16", 2)), "one type and length"), (dict(out=q), "takes the queries' place"),
+                         (dict(out=other(6, "bf16")), "are wanted"), (dict(kv_lens=array(ctx, [3, 3], "i32")), "kv_lens"),
+                         (dict(q_starts=array(ctx, [0], "i32")), "q_starts"), (dict(q_starts=array(ctx, [0.0, 3.0], "f32")), "of type i32"),
+                         (dict(page_table=array(ctx, [0, 1], "i32")), "q_starts"),
+                         (dict(out=Strided(out, (3, 4, 64), (64, 64, 1), 0)), "overlap"), (dict(q=Strided(q, (3, 4, 64), (-256, 64, 1), 0)), "strides"),
+                         (dict(q=Strided(q, (3, 4, 64), (128, 32, 2), 0)), "lie 2 apart")):
+        with pytest.raises(capi.TpuHipError, match=says):
+            cache.attention(**{**good, **change})
+    rows_of = lambda n, dtype="bf16": DeviceArray(ctx, (n, 2, 64), dtype)
+    slots = array(ctx, np.arange(5), "i32")
+    cache.write(rows_of(5), rows_of(5), slots)
+    for k, v, at, says in ((rows_of(5), rows_of(5, "f16"), slots, "one type and length"), (rows_of(5), rows_of(4), slots, "one type and length"),
+                           (rows_of(4), rows_of(4), slots, "4] int32"), (rows_of(5, "i32"), rows_of(5), slots, "bf16 or f16 or f32"),
+                           (DeviceArray(ctx, (5, 3, 64), "bf16"), rows_of(5), slots, "are wanted"), (rows_of(5), rows_of(5), rows_of(5), "slots"),
+                           (Strided(rows_of(5), (5, 2, 64), (-128, 64, 1), 0), rows_of(5), slots, "strides of the keys")):
+        with pytest.raises(capi.TpuHipError, match=says):
+            cache.write(k, v, at)
+    with pytest.raises(capi.TpuHipError, match="rows of the values overlap"):
+        cache.read(slots, rows_of(5), Strided(rows_of(5), (5, 2, 64), (64, 64, 1), 0))
+    cache.close()
+
+
+def test_torch_tensors():
+    """the cache between torch's own kernels, on torch's stream and on another one, on parts of a tensor: tests/kv_torch.py, in a process of its own,
+    since torch has to be imported before the library"""
+    res = subprocess.run([sys.executable, os.path.join(os.path.dirname(os.path.abspath(__file__)), "kv_torch.py")], stdout=subprocess.PIPE,
+                         stderr=subprocess.STDOUT, text=True, timeout=100)
+    assert res.returncode == 0 and res.stdout.strip().endswith("fine"), res.stdout[-3000:]

@@ -161,3 +161,32 @@ def test_integers_that_do_not_fit_are_not_uploaded(values):
     with pytest.raises(capi.TpuHipError, match="int"):
         DeviceArray.of(ctx, values, "i32")
     DeviceArray.of(ctx, [2 ** 31 - 1, -2 ** 31], "i32")
+
+
+def test_torch_tensors_of_other_devices_types_and_orders():
+    import torch
+    ctx = context()
+    cache = KVCache(ctx, 8, 2, 64, 4, 32)
+
+    class Placed:
+        """a tensor that says it lies on a device"""
+        def __init__(self, x, device):
+            self.x, self.device = x, torch.device(device)
+
+        def __getattr__(self, name):
+            return getattr(self.x, name)
+
+    k, slots = torch.zeros(3, 2, 64, dtype=torch.bfloat16), torch.arange(3, dtype=torch.int32)
+    here = lambda x: Placed(x, "cuda:0")
+    cache.plan_write(here(k), here(k), here(slots))()
+    assert ctx.lib.calls[-1][3].dtype == 0 and ctx.lib.calls[-1][3].k == k.data_ptr() and ctx.lib.calls[-1][4] == slots.data_ptr()
+    part = torch.zeros(3, 7, 70)[:, 2:4, 3:67]
+    cache.plan_write(here(part), here(part), here(slots))()
+    d = ctx.lib.calls[-1][3]
+    assert d.dtype == 2 and (d.k_token_stride, d.k_head_stride) == (490, 70) and d.k == part.data_ptr()
+    for bad, says in ((k, "on cpu"), (Placed(k, "cuda:1"), "on cuda:1"), (here(k.double()), "float64"), (here(k[:, :1]), "are wanted"),
+                      (here(torch.zeros(3, 2, 128, dtype=torch.bfloat16)[:, :, ::2]), "lie 2 apart")):
+        with pytest.raises(capi.TpuHipError, match=says):
+            cache.plan_write(bad, here(k), here(slots))
+    with pytest.raises(capi.TpuHipError, match="int64"):
+        cache.plan_write(here(k), here(k), here(slots.long()))
