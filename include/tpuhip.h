@@ -567,11 +567,14 @@ int tpuhip_kv_read(tpuhip_ctx *ctx, const tpuhip_kv_cache *cache, const tpuhip_k
  * page_table[b * table_stride + t / page_tokens]; a page outside the cache holds nothing to be seen (entries before the
  * window need not be kept).  q_starts (n_seq + 1), kv_lens (n_seq), page_table are device memory; what they say is cut to
  * total_q, max_q queries a sequence, max_kv tokens.  A call has at most 65535 sequences and heads, max_q * heads of 2^29, max_kv of
- * 2^30, and sequences * kv_heads (each sequence once for every 16 to 128 of its (query, shared head) pairs) below 2^24.  Rows of out that belong to no sequence stay as they are; out shares no memory
- * with q (workgroups that split a sequence read the queries again).
+ * 2^30, and sequences * kv_heads (each sequence once for every 16 to 128 of its (query, shared head) pairs) below 2^24.  Rows of out
+ * that belong to no sequence stay as they are; out shares no memory with q (workgroups that split a sequence read the queries
+ * again).
  * Scores, maxima and sums are 32-bit.  Queries are multiplied as float16 numbers times a power of two for each tile of at most 32
- * (query, head) pairs of a sequence, exactly as far as they are within 2^24 of the tile's largest; weights, times the values'
- * steps, are rounded to float16.  Sums are divided by that of the weights at the end: values past 1e30 may overflow them. */
+ * (query, head) pairs of a sequence, exactly as far as they are within 2^24 of the tile's largest.  Weights, times the values'
+ * steps, are rounded to float16: 2^-11 of a term s c (of a float16 result s (c - L / 2)) is lost of it, and 2^-33 of the largest
+ * step that the query sees, times c, where that is more.  Sums are divided by that of the weights at the end: values past 1e30 may
+ * overflow them. */
 typedef struct {
   int n_seq, heads, dtype;            /* dtype of q and out: TPUHIP_BF16 or TPUHIP_F16 */
   int total_q, max_q, max_kv;

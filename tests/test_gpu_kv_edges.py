@@ -161,3 +161,31 @@ def test_torch_tensors():
     res = subprocess.run([sys.executable, os.path.join(os.path.dirname(os.path.abspath(__file__)), "kv_torch.py")], stdout=subprocess.PIPE,
                          stderr=subprocess.STDOUT, text=True, timeout=100)
     assert res.returncode == 0 and res.stdout.strip().endswith("fine"), res.stdout[-3000:]
+
+
+@pytest.mark.parametrize("bits,n,dim,q_len", [(4, 513, 64, 1), (8, 513, 128, 1), (4, 3000, 64, 3), (4, 300, 160, 40)])
+def test_what_cancels_in_a_row_cancels_in_the_result(ctx, bits, n, dim, q_len):
+    """float16 results: values that are small between two large ones have large codes and a large offset.  All weights but the first token's are
+    alike and their rounding to float16 is as large as it gets, so that it adds up; of the small values that is little"""
+    rng = np.random.default_rng(6)
+    v = O.rounded(rng.uniform(-0.05, 0.05, (n, 1, dim)), "bf16")
+    v[:, :, 0], v[:, :, 1] = -1, 1
+    step = float(O.quantise(v, bits)[1][0, 0, 0])
+    x = np.linspace(0.5, 1.5, 2001)                              # weights exp(-x) times the step, as far from a float16 number as can be
+    product = np.exp(-x) * step
+    x = O.rounded(x[np.abs(product.astype(np.float16) / product - 1).argmax()], "bf16").item()
+    k = np.zeros((n, 1, dim), np.float32)
+    k[1:] = -x
+    q = np.zeros((q_len, 2, dim), np.float32)
+    q[:, :, 0] = dim ** 0.5 if dim == 64 else 8
+    k *= np.float32(dim ** 0.5 / q[0, 0, 0])
+    check(ctx, rng, q, [q_len], [O.rounded(k, "bf16")], [v], [n], bits, "f16")
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("kv_lens,q_lens,heads,kv_heads,dim", [([513], [1], 8, 2, 128), ([700, 40], [1, 1], 6, 1, 64), ([300], [40], 4, 2, 80),
+                                                               ([200, 150], [180, 150], 4, 4, 64), ([2000], [3], 4, 1, 256)])
+def test_float16_results_by_the_terms_of_their_rows(ctx, bits, kv_lens, q_lens, heads, kv_heads, dim):
+    rng = np.random.default_rng(7)
+    k, v = ([rows(rng, n, kv_heads, dim, "bf16", False) for n in kv_lens] for _ in "kv")
+    check(ctx, rng, rows(rng, sum(q_lens), heads, dim, "f16", False), q_lens, k, v, kv_lens, bits, "f16")

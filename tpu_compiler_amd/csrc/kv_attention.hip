@@ -162,7 +162,8 @@ constexpr int kJoinWaves = 16;
 // The left operands are the codes themselves: masked out of a dword, two of them are a pair of subnormal float16 numbers
 // c 2^-24 (of a byte's upper half c 2^-20), which the matrix unit takes as they are and multiplies exactly.  Steps and offsets are applied to
 // what is small: x = s_t (q.c_t) + m_t sum(q) to the scores, and P'_t = p_t s_t to the weights, with sum(p_t m_t) added to all channels.
-// Scores, maxima and sums are 32 bits; weights are rounded once, to float16, as the result is (at most 1.4 times its own rounding in all).
+// Scores, maxima and sums are 32 bits.  Weights times steps are rounded to float16, as the matrix unit takes no wider ones at this rate: against 64 bits
+// a result's RMS error is 1.005 times that of its own rounding in bfloat16 and 1.06 times in float16 (a token to 513; to 8192 1.002 and 1.02).
 // Of a workgroup's four waves, WR have rows of their own; the 4 / WR with the same rows take every so manieth unit and join their sums in LDS.
 //
 // Bounds.  Few rows: memory.  A unit of 128 channels in 4 bits is 4352 bytes, read once, straight into the lanes that multiply it (no
@@ -365,8 +366,15 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
   // ---- the sums
   float top[NC], limit[NC], total[NC], offsets[NC];   // limit: a score above it, relative to the maximum, raises that
   float4v o[OB][NC];
+  // The rounding of weights times steps counts as much as the codes do, also where codes and offsets cancel.  For a float16 result it counts by the codes'
+  // distance from their middle: sums of the rounded weights make o that of codes less the middle, which goes to the offsets, whose weights are not
+  // rounded.  Of the RMS error of a token to 513, beside that of the result's own rounding, that leaves 0.35 of 1.03.  For bfloat16, whose own is eight
+  // times as large, it is a tenth of it as it is, and four instructions for eight scores would be for nothing.
+  const float middle = a.bf16 ? 0.0f : U::kLevels / 2.0f;
+  float rounded[NC];
 #pragma unroll
   for (int nc = 0; nc < NC; ++nc) {
+    rounded[nc] = 0;
     top[nc] = 0;
     limit[nc] = -INFINITY;                                      // the row has seen nothing
     total[nc] = offsets[nc] = 0;
@@ -399,77 +407,88 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
       for (int h = 0; h < 2; ++h) *(float4v *)(vs + h * 4) = *(const float4v *)&params[wave][32 + h * 16 + g * 4];
     };
     const bool scaled = size_limit > 0;
-    float seen_size[NC];
+    float lift[NC], v_change = 1;
+    bool sizes = !scaled || ((size > size_limit) & (lane >= 32));
 #pragma unroll
     for (int nc = 0; nc < NC; ++nc) {
-      seen_size[nc] = uneven ? row_size[wave][nc * 16 + col] : __uint_as_float(most_seen);
       high[nc] = column_max(high[nc]);
+      lift[nc] = fmaxf(limit[nc] - kLag, 0);
+      sizes |= limit[nc] < 0 && high[nc] > -INFINITY;           // a row that begins to see
     }
-    const int t = t0 + lane - 32;                               // the lane's token, and whether any row sees it
-    const bool there = lane >= 32 && t <= p_hi && (t > p_lo - window || t < a.sinks);
-    const uint32_t largest = wave_max(there ? __float_as_uint(size) : 0);
-    const auto least = [&] { return ~wave_max(there ? ~__float_as_uint(size) : 0); };
-    if (all || p_lo == p_hi) {                                  // all rows see the same of the unit
-      most_seen = max(most_seen, largest);
+    if (__any(sizes)) {
+      float seen_size[NC];
 #pragma unroll
-      for (int nc = 0; nc < NC; ++nc) seen_size[nc] = fmaxf(seen_size[nc], __uint_as_float(largest));
-    } else if (const uint32_t low = least(); exponent(largest) - exponent(low) < kLeastLift) {   // or about the same, if any: that there is more shows when it is above size_limit
-      uneven = true;
-      most_seen = max(most_seen, largest);
+      for (int nc = 0; nc < NC; ++nc) seen_size[nc] = uneven ? row_size[wave][nc * 16 + col] : __uint_as_float(most_seen);
+      const int t = t0 + lane - 32;                             // the lane's token, and whether any row sees it
+      const bool there = lane >= 32 && t <= p_hi && (t > p_lo - window || t < a.sinks);
+      const uint32_t largest = wave_max(there ? __float_as_uint(size) : 0);
+      const auto least = [&] { return ~wave_max(there ? ~__float_as_uint(size) : 0); };
+      if (all || p_lo == p_hi) {                                // all rows see the same of the unit
+        most_seen = max(most_seen, largest);
 #pragma unroll
-      for (int nc = 0; nc < NC; ++nc) seen_size[nc] = high[nc] > -INFINITY ? fmaxf(seen_size[nc], __uint_as_float(low)) : seen_size[nc];
-    } else {
-      uneven = true;
-      if (scaled) steps(1);
-      uint32_t most = 0;
+        for (int nc = 0; nc < NC; ++nc) seen_size[nc] = fmaxf(seen_size[nc], __uint_as_float(largest));
+      } else if (const uint32_t low = least(); exponent(largest) - exponent(low) < kLeastLift) {
+        uneven = true;                                          // or about the same, if any; that a row sees more shows above size_limit
+        most_seen = max(most_seen, largest);
 #pragma unroll
-      for (int nc = 0; nc < NC; ++nc) {
-        float sees = 0;
+        for (int nc = 0; nc < NC; ++nc) seen_size[nc] = high[nc] > -INFINITY ? fmaxf(seen_size[nc], __uint_as_float(low)) : seen_size[nc];
+      } else {
+        uneven = true;
+        if (scaled) steps(1);
+        uint32_t most = 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sees = s[j / 4][nc][j & 3] > -INFINITY ? fmaxf(sees, size_of(vs[j], vm[j])) : sees;
-        seen_size[nc] = fmaxf(seen_size[nc], column_max(sees));
-        most = max(most, __float_as_uint(seen_size[nc]));
+        for (int nc = 0; nc < NC; ++nc) {
+          float sees = 0;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) sees = s[j / 4][nc][j & 3] > -INFINITY ? fmaxf(sees, size_of(vs[j], vm[j])) : sees;
+          seen_size[nc] = fmaxf(seen_size[nc], column_max(sees));
+          most = max(most, __float_as_uint(seen_size[nc]));
+        }
+        most_seen = max(most_seen, wave_max(most));
       }
-      most_seen = max(most_seen, wave_max(most));
-    }
-    if (uneven)
+      if (most_seen && (!scaled || exponent(most_seen) + v_exp >= kMostSteps)) {
+        const int now = min(8 - exponent(most_seen), 99);
+        v_change = power(now - v_exp);
+        v_exp = now;
+        v_scale = power(now);
+      }
+      if (scaled) {
+        steps(v_scale);
+      } else {
 #pragma unroll
-      for (int nc = 0; nc < NC; ++nc) row_size[wave][nc * 16 + col] = seen_size[nc];
-    float v_change = 1;
-    if (most_seen && (size_limit == 0 || exponent(most_seen) + v_exp >= kMostSteps)) {
-      const int now = min(8 - exponent(most_seen), 99);
-      v_change = power(now - v_exp);
-      v_exp = now;
-      v_scale = power(now);
-    }
-    if (scaled) {
-      steps(v_scale);
-    } else {
+        for (int j = 0; j < 8; ++j) vs[j] *= v_scale;
+      }
+      if (!all) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) vs[j] *= v_scale;
-    }
-    if (!all) {
+        for (int j = 0; j < 8; ++j) vs[j] = fminf(vs[j], 0x1p15f);   // of a hidden one, whose weight is 0
+      }
+      int most_lift = 0;
+      if (uneven) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) vs[j] = fminf(vs[j], 0x1p15f);   // of a hidden one, whose weight is 0
+        for (int nc = 0; nc < NC; ++nc) {
+          row_size[wave][nc * 16 + col] = seen_size[nc];
+          const int by = seen_size[nc] > 0 ? 8 - exponent(__float_as_uint(seen_size[nc])) - v_exp : 0;
+          lift[nc] = by < kLeastLift ? 0.0f : (float)min(by, kMostLift);
+          most_lift = max(most_lift, (int)lift[nc]);
+        }
+        if (__any(most_lift)) most_lift = (int)wave_max(most_lift);
+      }
+      if (most_seen) size_limit = power(kMostSteps - v_exp - __builtin_amdgcn_readfirstlane(most_lift));
     }
-    int most_lift = 0;
 #pragma unroll
     for (int nc = 0; nc < NC; ++nc) {
       const bool first = limit[nc] < 0, some = high[nc] > -INFINITY;
-      int lift = uneven && seen_size[nc] > 0 ? 8 - exponent(__float_as_uint(seen_size[nc])) - v_exp : 0;
-      lift = lift < kLeastLift ? 0 : min(lift, kMostLift);
-      most_lift = max(most_lift, lift);
-      const float up = (first ? some ? high[nc] : 0.0f : fmaxf(high[nc], limit[nc] - kLag)) - (float)lift, change = first ? 1.0f : exp2_fast(-up);
-      limit[nc] = some || !first ? kLag + (float)lift : limit[nc];
+      const float up = (first ? some ? high[nc] : 0.0f : fmaxf(high[nc], limit[nc] - kLag)) - lift[nc], change = first ? 1.0f : exp2_fast(-up);
+      limit[nc] = some || !first ? kLag + lift[nc] : limit[nc];
       top[nc] += up;
       total[nc] *= change;
       offsets[nc] *= change;
+      rounded[nc] *= change * v_change;
 #pragma unroll
       for (int j = 0; j < 8; ++j) s[j / 4][nc][j & 3] -= up;
 #pragma unroll
       for (int b = 0; b < OB; ++b) o[b][nc] *= change * v_change;
     }
-    if (most_seen) size_limit = power(kMostSteps - v_exp - (__any(most_lift) ? (int)wave_max(most_lift) : 0));
   };
   const auto softmax = [&](int t0, float step, float size, float (&ks)[8], float (&km)[8], float (&vs)[8], float (&vm)[8], float4v (&s)[2][NC], uint4v (&p)[NC]) {
     const bool all = t0 + kUnitTokens - 1 <= p_lo && (t0 > p_hi - window || t0 + kUnitTokens - 1 < a.sinks);
@@ -523,6 +542,14 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
       for (int j = 0; j < 8; ++j) w[j] *= vs[j];
       p[nc] = (uint4v){pack_f16(w[0], w[1]), pack_f16(w[2], w[3]), pack_f16(w[4], w[5]), pack_f16(w[6], w[7])};
     }
+    if (!a.bf16)
+#pragma unroll
+      for (int nc = 0; nc < NC; ++nc)
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          const uint32_t pair = p[nc][d];
+          rounded[nc] = __builtin_amdgcn_fdot2(__builtin_bit_cast(half2v, pair), (half2v){1, 1}, rounded[nc], false);   // takes subnormal ones as they are
+        }
   };
 
   for (; i < end; i += WK) {
@@ -536,6 +563,8 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
     if (lane < 32) {
       step *= step_scale;
       offset *= offset_scale;
+    } else {
+      offset = __builtin_fmaf(step, middle, offset);
     }
     params[wave][lane] = lane < 32 ? step : step * v_scale;
     params[wave][64 + lane] = offset;
@@ -608,7 +637,7 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
     const int lift = limit[nc] > 0 ? (int)(limit[nc] - kLag) : 0;
     const float down = power(-lift), back = ldexpf(1.0f, 24 - v_exp - lift);
     total[nc] = column_sum(total[nc]) * down;
-    offsets[nc] = column_sum(offsets[nc]) * down;
+    offsets[nc] = __builtin_fmaf(column_sum(rounded[nc]), -middle * 0x1p-24f * back, column_sum(offsets[nc]) * down);
     top[nc] = limit[nc] < 0 ? kNothing : top[nc] + (float)lift;
 #pragma unroll
     for (int b = 0; b < OB; ++b) {
