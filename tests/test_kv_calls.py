@@ -190,3 +190,25 @@ def test_torch_tensors_of_other_devices_types_and_orders():
             cache.plan_write(bad, here(k), here(slots))
     with pytest.raises(capi.TpuHipError, match="int64"):
         cache.plan_write(here(k), here(k), here(slots.long()))
+
+
+@pytest.mark.parametrize("prompts", [[], [[1, 2], []]])
+def test_the_example_refuses_prompts_without_a_token(prompts):
+    """there is nothing to continue, and the logits of another sequence would be taken for its own"""
+    from tpu_compiler_amd import kv_example
+    ctx = context()
+    with pytest.raises(ValueError, match="token"):
+        kv_example.generate(ctx, kv_example.Model(), prompts, 3)
+    assert not ctx.lib.calls
+
+
+def test_the_example_gives_out_pages_until_there_are_no_more():
+    from tpu_compiler_amd import kv_example
+    ctx = context()
+    s = kv_example.Sequences(ctx, 1, 8, 2, 64, 4, pages=3, page_tokens=32)
+    s.begin([40, 20])
+    with pytest.raises(ValueError, match="pages"):
+        s.begin([30, 0])
+    assert s.lens == [40, 20] and len(s.pages[0]) == 2
+    s.begin([24, 12])                            # what fits is taken all the same
+    assert s.lens == [64, 32]

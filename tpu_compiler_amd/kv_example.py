@@ -27,6 +27,9 @@ class Sequences:
         while len(self.lens) < len(new_tokens):
             self.pages.append([])
             self.lens.append(0)
+        more = [max(0, -(-(have + n) // self.page_tokens) - len(pages)) for have, n, pages in zip(self.lens, new_tokens, self.pages)]
+        if sum(more) > len(self.free):
+            raise ValueError("%d pages are wanted, %d are free" % (sum(more), len(self.free)))
         slots = []
         for i, n in enumerate(new_tokens):
             at = np.arange(self.lens[i], self.lens[i] + n)
@@ -86,6 +89,8 @@ class Model:
 
 def generate(ctx, model, prompts, tokens, bits=4, window=0, sinks=0, page_tokens=64):
     """continues each prompt by `tokens` tokens, the likeliest one each time -> (lists of tokens, logits of every step, bytes of the cache)"""
+    if not len(prompts) or not all(len(p) for p in prompts):
+        raise ValueError("a prompt has a token at least")
     need = sum(-(-(len(p) + tokens) // page_tokens) for p in prompts)
     s = Sequences(ctx, len(model.qkv), model.heads, model.kv_heads, model.head_dim, bits, need, page_tokens, window, sinks)
     answers, steps, new = [[] for _ in prompts], [], [list(p) for p in prompts]
