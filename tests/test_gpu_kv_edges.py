@@ -189,3 +189,19 @@ def test_float16_results_by_the_terms_of_their_rows(ctx, bits, kv_lens, q_lens, 
     rng = np.random.default_rng(7)
     k, v = ([rows(rng, n, kv_heads, dim, "bf16", False) for n in kv_lens] for _ in "kv")
     check(ctx, rng, rows(rng, sum(q_lens), heads, dim, "f16", False), q_lens, k, v, kv_lens, bits, "f16")
+
+
+def test_a_cache_that_there_is_no_memory_for(ctx):
+    """is refused, and what comes after it is not"""
+    with pytest.raises(capi.TpuHipError) as refused:
+        KVCache(ctx, 1 << 20, 64, 256, 8, 32)                    # 1.1 TB
+    assert refused.value.status == 3 and "memory" in str(refused.value)
+    cache = KVCache(ctx, 2, 2, 64, 4, 32)
+    x, slots = array(ctx, np.ones((3, 2, 64)), "bf16"), array(ctx, np.arange(3), "i32")
+    with pytest.raises(capi.TpuHipError):
+        KVCache(ctx, 1 << 20, 64, 256, 8, 32)
+    cache.write(x, x, slots)
+    with pytest.raises(capi.TpuHipError):
+        KVCache(ctx, 1 << 20, 64, 256, 8, 32)
+    cache.read(slots, x, x)
+    cache.close()

@@ -197,8 +197,10 @@ int tpuhip_malloc(tpuhip_ctx *ctx, size_t bytes, void **dptr) {
     if (rc != TPUHIP_ERR_NOMEM) return rc;   // where there is no room for a slab there may be for this
   }
   hipError_t e = hipMalloc(dptr, bytes + 256);
-  if (e == hipErrorOutOfMemory)
+  if (e == hipErrorOutOfMemory) {
+    (void)hipGetLastError();   // or the next launch's check finds it
     return set_error(TPUHIP_ERR_NOMEM, "tpuhip_malloc: out of device memory (%zu bytes)", bytes);
+  }
   TPUHIP_CHECK_HIP(e);
   return TPUHIP_OK;
 }
