@@ -919,8 +919,9 @@ int tpuhip_kv_attention(tpuhip_ctx *ctx, const tpuhip_kv_cache *cache, const tpu
       TPUHIP_REQUIRE(most >= 1, "%s: %d queries of %d sequences over %d heads in one call", what, a.total_q, d->n_seq, kv_heads);
       a.splits = 1;
       if constexpr (WR == 1) {
-        // Two workgroups a CU, without more than are there at a time (three, two with twice the rows or wider ones), and none of more than
-        // 128 units, as lengths may differ; but two units a wave at least, four with twice the rows, for a join takes as long (a wave takes
+        // Two workgroups a CU, without more than are there at a time (three, two with twice the rows or wider ones; heads of 64 have registers for
+        // one more, but with 2, 3 or 4 a batch of 24 single tokens takes 26.5, 23.5 or 23.6 us there, 34.3, 32.7 or 32.5 with heads of 128, and a draft
+        // 20.3, 21.1 or 21.3), and none of more than 128 units, as lengths may differ; but two units a wave at least, four with twice the rows, for a join takes as long (a wave takes
         // 1 us a unit, the join of two splits 1.6), and so few splits that the last one can join them rather than another kernel, where
         // these have six units a wave at most.
         const int64_t units = units_of(R), there = (NC == 1 && U::kDim <= 128 ? 3 : 2) * num_cu;
@@ -955,18 +956,33 @@ int tpuhip_kv_attention(tpuhip_ctx *ctx, const tpuhip_kv_cache *cache, const tpu
     };
     // The form of the kernel: 16 NC rows a wave, WR of the four waves with rows of their own.  Wide waves unpack codes less often, waves
     // with the same rows end a long list sooner, and there have to be workgroups for the CUs, more than two at a time where tiles differ.
-    // Microseconds of 4 sequences of n tokens, causal, heads of 128 in 4 bits by fours (NC, WR; the chosen one in brackets):
+    // Microseconds of 4 sequences of n tokens, causal, heads of 128 in 4 bits by fours (NC, WR; the chosen one in brackets; those of WR 1 with
+    // their splits, the others have none):
     //    n  heads  rows a CU    2, 4     2, 2     2, 1     1, 4     1, 1
-    //    64    4        16       9.4      9.0      8.2      7.6     [6.5]
-    //   512    4        32      21.5     15.9     11.8     16.1     [9.8]
-    //  1088    4        68      37.4     24.8    [19.4]    27.6     20.6
-    //    64  128       128      11.6     12.8     19.9    [10.1]    19.8
-    //   512   16       128      24.3    [21.0]    24.8     21.4     24.6
-    //   256   64       256     [22.6]    27.1     38.0     23.6     37.0
-    //  1088   64      1088    [125.5]   158.5    209.9    139.6    212.8
-    // and of 64 queries of each behind 4096 tokens of 8 heads 115.8, 65.9, 24.0, 84.6 and [19.3]; of one prompt of 2176 of 32 heads (272 rows a
-    // CU) 76.8, [67.1], 77.2, 65.8 and 79.0; of a draft, 24 sequences of 12 to 28 rows of 80 channels in 8 bits, 130, 75, [23.9], 102 and 27.1.
-    // Rows of more than 128 channels have one block of 16 a wave, as two do not fit into registers.
+    //    64    4        16       9.2      8.8      8.4      6.8     [6.3]
+    //   512    4        32      21.2     15.4     11.8     16.4    [10.4]
+    //  1088    4        68      37.5     25.0    [20.6]    29.2     23.4
+    //    64  128       128      11.2     12.7     20.1     [9.9]    20.6
+    //   512   16       128      24.1    [21.4]    24.8     21.2     25.4
+    //   256   64       256     [22.8]    26.5     38.2     23.3     37.3
+    //  1088   64      1088    [129.4]   156.0    208.1    142.9    213.3
+    // and of 64 queries of each behind 4096 tokens of 8 heads 116.5, 63.6, 23.5, 88.1 and [18.9]; of one prompt of 2176 of 32 heads (272 rows a
+    // CU) 77.4, [70.3], 77.8, 71.0 and 80.4; of a draft, 24 sequences of 12 to 28 rows of 80 channels in 8 bits, 132.6, 74.3, [24.6], 107.4 and 27.1.
+    // Rows of more than 128 channels have one block of 16 a wave, as two do not fit into registers.  Of 4 sequences with q queries each at the end of
+    // n tokens, heads of 192 in 4 bits by fours (those of 256 take 1.1 to 1.3 times as long in all forms):
+    //     q     n  heads  rows a CU    1, 4     1, 2     1, 1
+    //    64    64    4        16        7.9      7.5     [7.3]
+    //   512   512    4        32       19.6     13.7    [12.6]
+    //    64  4096   32        32      109.9     61.0    [46.4]
+    //    64  1000   64        64       34.3    [25.6]    31.3
+    //   128  4096   32        64      111.0    [74.1]    80.8
+    //  1088  1088    4        68       36.8    [27.0]    29.1
+    //    64    64  128       128      [13.3]    18.7     29.8
+    //   128  4096   64       128      137.2   [140.4]   150.6
+    //   600  2000   16       150      104.1    [92.7]
+    //   300   300   32       150      [22.5]    26.6     38.4
+    //  1088  1088   16       272      [68.9]    68.0     91.6
+    //  1088  1088   64      1088     [212.8]   252.3    344.0
     using std::integral_constant;
     const integral_constant<int, 1> one;
     const integral_constant<int, 2> two;
@@ -981,8 +997,8 @@ int tpuhip_kv_attention(tpuhip_ctx *ctx, const tpuhip_kv_cache *cache, const tpu
       if (!enough(seen <= 40 ? 255 : 511)) return run(two, two);
       return run(two, four);
     } else {
-      if (rows_max <= 16 || !enough(31)) return run(one, one);
-      if (!enough(255)) return run(one, two);
+      if (rows_max <= 16 || !enough(48)) return run(one, one);
+      if (!enough(units_of(16) <= 20 ? 100 : 255)) return run(one, two);
       return run(one, four);
     }
   });
