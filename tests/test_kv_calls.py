@@ -212,3 +212,17 @@ def test_the_example_gives_out_pages_until_there_are_no_more():
     assert s.lens == [40, 20] and len(s.pages[0]) == 2
     s.begin([24, 12])                            # what fits is taken all the same
     assert s.lens == [64, 32]
+
+
+def test_a_cache_that_could_not_be_freed_can_be_closed_again():
+    ctx = context()
+    cache = KVCache(ctx, 8, 2, 64, 4, 32)
+    status = [2]
+    ctx.lib.tpuhip_kv_cache_destroy = lambda *a: status[0]
+    ctx.lib.tpuhip_last_error = lambda: b"a stream is being captured"
+    with pytest.raises(capi.TpuHipError, match="captured"):
+        cache.close()
+    status[0] = 0
+    assert cache.h
+    cache.close()
+    assert not cache.h

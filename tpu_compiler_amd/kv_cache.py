@@ -145,8 +145,8 @@ class KVCache:
 
     def close(self):
         if self.h:
-            h, self.h = self.h, None
-            self._made_by._ck(self._made_by.lib.tpuhip_kv_cache_destroy(self._made_by.h, h))
+            self._made_by._ck(self._made_by.lib.tpuhip_kv_cache_destroy(self._made_by.h, self.h))
+            self.h = None
 
     def __del__(self):
         try:
