@@ -544,6 +544,7 @@ enum { TPUHIP_BF16 = 0, TPUHIP_F16 = 1, TPUHIP_F32 = 2 };
 /* device memory a cache takes, 0 if its sizes are refused */
 size_t tpuhip_kv_cache_bytes(const tpuhip_kv_desc *desc);
 int tpuhip_kv_cache_create(tpuhip_ctx *ctx, const tpuhip_kv_desc *desc, tpuhip_kv_cache **out);
+/* refused, like create, while the context's stream is being captured */
 int tpuhip_kv_cache_destroy(tpuhip_ctx *ctx, tpuhip_kv_cache *cache);
 
 /* keys and values [tokens, kv_heads, head_dim] of one type, strides in elements, a head's numbers next to each other */

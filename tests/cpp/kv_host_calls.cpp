@@ -170,13 +170,33 @@ void many_rows() {
   notes.clear();
   check(attend(few.ctx, few.cache, attention(65535, 4, 1, 1, 1 << 20, 64)));   // all but one of them without a query
 }
+
+// while the context's stream is being recorded, a cache is neither made nor freed, and the recording is not touched; calls are recorded, and
+// take no memory
+void recording() {
+  Cache c(0);
+  tpuhip_ctx *fresh = nullptr;
+  check(tpuhip_ctx_create(0, &fresh));
+  capturing = true;
+  notes.clear();
+  const tpuhip_kv_desc d = {4, 32, 2, 64, 4};
+  tpuhip_kv_cache *other = nullptr;
+  expect(tpuhip_kv_cache_create(c.ctx, &d, &other) == TPUHIP_ERR_INVALID && !other, "a cache was made");
+  expect(tpuhip_kv_cache_destroy(c.ctx, c.cache) == TPUHIP_ERR_INVALID, "a cache was freed");
+  expect(notes.empty(), "the runtime was asked for something");
+  check(attend(c.ctx, c.cache, attention(1, 4, 1, 1, 4096, 64)));
+  check(attend(fresh, c.cache, attention(1, 4, 1, 1, 4096, 64)));
+  expect(count("launch") == notes.size(), "more than launches");
+  capturing = false;
+  check(tpuhip_ctx_destroy(fresh));
+}
 }  // namespace
 
 int main(int argc, char **argv) {
   const struct {
     const char *name;
     std::function<void()> run;
-  } cases[] = {{"no_tokens", no_tokens}, {"workspace_device", workspace_device}, {"pages_are_clear", pages_are_clear}, {"many_rows", many_rows}};
+  } cases[] = {{"no_tokens", no_tokens}, {"workspace_device", workspace_device}, {"pages_are_clear", pages_are_clear}, {"many_rows", many_rows}, {"recording", recording}};
   try {
     for (auto &c : cases)
       if (argc == 2 && !strcmp(argv[1], c.name)) {

@@ -549,6 +549,7 @@ int tpuhip_kv_cache_create(tpuhip_ctx *ctx, const tpuhip_kv_desc *desc, tpuhip_k
 int tpuhip_kv_cache_destroy(tpuhip_ctx *ctx, tpuhip_kv_cache *cache) {
   TPUHIP_REQUIRE(ctx, "tpuhip_kv_cache_destroy: NULL context");
   if (!cache) return TPUHIP_OK;
+  if (int rc = not_captured(ctx, "tpuhip_kv_cache_destroy")) return rc;   // a wait would end the recording
   if (int rc = tpuhip_free(ctx, cache->data)) return rc;
   delete cache;
   return TPUHIP_OK;
