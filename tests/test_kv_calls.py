@@ -1,6 +1,7 @@
 """The Python side of the key/value cache: what calls are made with, and which are refused.  A stand-in for the library notes its calls, so
 no device is needed."""
 import ctypes as C
+import gc
 
 import pytest
 
@@ -226,3 +227,16 @@ def test_a_cache_that_could_not_be_freed_can_be_closed_again():
     assert cache.h
     cache.close()
     assert not cache.h
+
+
+def test_a_cache_that_is_collected_while_it_cannot_be_freed_is_freed_with_its_context():
+    ctx = context()
+    cache = KVCache(ctx, 8, 2, 64, 4, 32)
+    freed = []
+    ctx.lib.tpuhip_last_error = lambda: b"a stream is being captured"
+    ctx.lib.tpuhip_kv_cache_destroy = lambda *a: 1
+    del cache
+    gc.collect()
+    ctx.lib.tpuhip_kv_cache_destroy = lambda c, h: freed.append(h.value) or 0
+    ctx.close()
+    assert freed == [0x1000]

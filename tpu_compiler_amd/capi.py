@@ -431,12 +431,14 @@ class Context:
 
     def _begin(self, lib, device, h):
         self.lib, self.device, self.h = lib, device, h
-        self.caches = weakref.WeakSet()      # key/value caches made by this context, which end with it
+        self.caches = weakref.WeakSet()      # key/value caches made by this context, which end with it,
+        self.unfreed = []                    # and those that nobody holds but could not be freed yet
 
     def close(self):
         if self.h:
-            for c in list(self.caches):
+            for c in list(self.caches) + self.unfreed:
                 c.close()
+            self.unfreed = []
             self.lib.tpuhip_ctx_destroy(self.h)
             self.h = None
 

@@ -151,8 +151,8 @@ class KVCache:
     def __del__(self):
         try:
             self.close()
-        except Exception:       # the process ends
-            pass
+        except Exception:       # its context's stream is being recorded, or the process ends
+            self._made_by.unfreed.append(self)
 
     def _rows(self, fn, slots, k, v):
         tokens = _int(k.shape[0], "tokens")
