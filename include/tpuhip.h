@@ -524,8 +524,9 @@ int tpuhip_dequant_i8_to_f32(tpuhip_ctx *ctx, const void *x, void *y_nchw_f32, i
  * A row x of D numbers is held as integers c of 0..L, L = 2^bits - 1, with an offset m and a step s in bfloat16:
  *   m = the largest bfloat16 <= min(x),  s = the smallest bfloat16 >= (max(x) - m) / L (0 below 2^-126),
  *   c = rint((x - m) / s), a tie to the even one, at most L,
- * in 32-bit arithmetic, and stands for m + s c: every element comes back within s / 2.  A row that holds an infinity or a NaN, or
- * whose range 32 bits do not hold, comes back as NaN as a whole, and is harmless where a mask hides it.
+ * in 32-bit arithmetic, and stands for m + s c: every element comes back within s / 2 (of float32 rows within s (1 / 2 + 2^-14), of a
+ * row whose step is below 2^-126 within its range).  A row that holds an infinity or a NaN, or whose range 32 bits do not hold,
+ * comes back as NaN as a whole, and is harmless where a mask hides it.
  *
  * The cache is an array of pages of page_tokens tokens each, for all kv_heads heads.  Token positions are the caller's to
  * give out: slot = page * page_tokens + place names one of them, and a page table lists the pages of a sequence in order.

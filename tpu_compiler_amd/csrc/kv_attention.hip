@@ -167,11 +167,11 @@ constexpr int kJoinWaves = 16;
 // Of a workgroup's four waves, WR have rows of their own; the 4 / WR with the same rows take every so manieth unit and join their sums in LDS.
 //
 // Bounds.  Few rows: memory.  A unit of 128 channels in 4 bits is 4352 bytes, read once, straight into the lanes that multiply it (no
-// barrier in the loop): one token for each of 64 sequences of 61 to 8192, 288 MB, takes 67 us, 4.3 TB/s (a copy moves 4.8, reading alone reaches
+// barrier in the loop): one token for each of 64 sequences of 61 to 8192, 288 MB, takes 68 us, 4.3 TB/s (a copy moves 4.8, reading alone reaches
 // 6.0); for one of 131072, 143 MB, 28 us and 4.5 for the join.  Many rows: the vector ALU.  A unit costs a wave 80 instructions to unpack and
-// 7 a score (two fused products, half a maximum, an exponential, a sum, a step, an offset, half a conversion), 235 for 32 rows against 32
-// matrix instructions of 16 cycles; 8192 tokens of 32 heads, causal, 0.55 TFLOP, take 590 us, 930 TFLOP/s, 76 % of a large float16 product,
-// with the vector ALU busy for 80 % of the time and the matrix unit for 36 %.  More rows a wave would amortise unpacking, but 48 of 128 channels need the queries in LDS,
+// 7 a score (two fused products, half a maximum, an exponential, a sum, a step, an offset, half a conversion), 238 for 32 rows against 32
+// matrix instructions of 16 cycles; 8192 tokens of 32 heads, causal, 0.55 TFLOP, take 588 us, 935 TFLOP/s, 77 % of a large float16 product,
+// with the vector ALU busy for 83 % of the time and the matrix unit for 37 %.  More rows a wave would amortise unpacking, but 48 of 128 channels need the queries in LDS,
 // all registers, and gained 2 %; fewer, 16, have three waves a SIMD and take 709 us.
 // In between, latency: a SIMD with one wave issues a vector instruction every eight clocks instead of four to five, and a unit of 32 rows takes it
 // 0.95 us, where two waves take 1.13 for one each.  Multiplying the next unit's keys before this one's scores, and handing on its params, took nothing
@@ -604,7 +604,7 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
     load_k(u);
     in_order();
     // bound by the vector ALU: a wave with scores to work on goes before one that feeds the matrix unit, and products of values, which
-    // end its unit, before those of keys (a prompt of 8192 tokens: 595 us without, 582 with)
+    // end its unit, before those of keys (a prompt of 8192 tokens: 598 us without, 585 with; parts of prompts 34.4 and 32.9)
     __builtin_amdgcn_s_setprio(2);
     uint4v p[NC];
     softmax(t0, step, size, ks, km, vs, vm, s, p);
