@@ -205,3 +205,19 @@ def test_a_cache_that_there_is_no_memory_for(ctx):
         KVCache(ctx, 1 << 20, 64, 256, 8, 32)
     cache.read(slots, x, x)
     cache.close()
+
+
+@pytest.mark.parametrize("far", [1e6, 1e9])
+@pytest.mark.parametrize("near", [30, 250, 900])
+@pytest.mark.parametrize("bits,dim,heads", [(4, 64, 1), (8, 128, 2), (4, 160, 1), (4, 96, 4)])
+def test_large_values_that_some_queries_see_and_larger_ones_that_few_see(ctx, bits, dim, heads, near, far):
+    """the first queries' windows hold a value that the others have behind them, and the last ones see tokens `near` times their other ones; all
+    with the same weight, so that each of these counts in full"""
+    rng = np.random.default_rng(9)
+    n, q_len, window = 320, 24, 130
+    k, v = (rows(rng, n, 1, dim, "bf16", False) for _ in "kv")
+    first = n - q_len
+    v[first - window + 3] = O.rounded(v[first - window + 3] * far, "bf16")     # seen by the first three queries
+    v[[n - 20, n - 7]] = O.rounded(v[[n - 20, n - 7]] * near, "bf16")
+    q = np.zeros((q_len, heads, dim), np.float32)
+    check(ctx, rng, q, [q_len], [k], [v], [n], bits, "bf16", window=window)

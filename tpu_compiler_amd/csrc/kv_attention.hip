@@ -427,8 +427,8 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
         most_seen = max(most_seen, largest);
 #pragma unroll
         for (int nc = 0; nc < NC; ++nc) seen_size[nc] = fmaxf(seen_size[nc], __uint_as_float(largest));
-      } else if (const uint32_t low = least(); exponent(largest) - exponent(low) < kLeastLift) {
-        uneven = true;                                          // or about the same, if any; that a row sees more shows above size_limit
+      } else if (const uint32_t low = least(); exponent(max(most_seen, largest)) - exponent(low) < kLeastLift) {
+        uneven = true;                                          // or about the same, if any, and so near the largest that no row which does is lifted
         most_seen = max(most_seen, largest);
 #pragma unroll
         for (int nc = 0; nc < NC; ++nc) seen_size[nc] = high[nc] > -INFINITY ? fmaxf(seen_size[nc], __uint_as_float(low)) : seen_size[nc];
