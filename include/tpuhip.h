@@ -575,7 +575,7 @@ int tpuhip_kv_read(tpuhip_ctx *ctx, const tpuhip_kv_cache *cache, const tpuhip_k
  * Scores, maxima and sums are 32-bit.  Queries are multiplied as float16 numbers times a power of two for each tile of at most 32
  * (query, head) pairs of a sequence, exactly as far as they are within 2^24 of the tile's largest; from 2^104 on they are
  * infinities, which harm their own results alone.  Weights, times the values'
- * steps, are rounded to float16: 2^-11 of a term s c (of a float16 result s (c - L / 2)) is lost of it, and 2^-33 of the largest
+ * steps, are rounded to float16: 2^-11 of a term s c (of a float16 result s (c - L / 2)) is lost of it, and 2^-30 of the largest
  * step that the query sees, times c, where that is more.  Sums are divided by that of the weights at the end: values past 1e30 may
  * overflow them. */
 typedef struct {

@@ -18,7 +18,7 @@ def attention(q, k, v, bits, q_lens, kv_lens, scale, dtype, window=0, sinks=0):
       a score     at most D + 8 of 32 bits, each of T or less, and one of the largest score, which is taken off: the weight is that much off,
                   and its share of the result with it: p ((D + 8) u T + 4 u max|x| + 8 u) (|V| + |out|), 8 u the exponential and products
       a weight    times its step to float16, 2^-11 of its term: p s c, or for a float16 result p s |c - L / 2|; one that is small beside the
-                  largest step S loses at most 2^-33 S c (the largest is held as 2^8 or more, where float16 ends at 2^-25)
+                  largest step S loses at most 2^-30 S c (that is held as 2^5 or more, where float16 ends at 2^-25)
       the sums    32 bits, no more than n / 16 + 64 additions one after the other, of the terms p |m| and p s c
       the result  half a unit of 8 or 11 bits: bfloat16 numbers from 1 on lie 2^-7 apart, float16 numbers 2^-10"""
     heads, dim = q.shape[1:]
@@ -43,7 +43,7 @@ def attention(q, k, v, bits, q_lens, kv_lens, scale, dtype, window=0, sinks=0):
                 rounded = w @ (vs[t, g] * np.abs(c - (2 ** bits - 1) / 2)) if dtype == "f16" else part
                 want[row, h] = out
                 limit[row, h] = unit * np.abs(out) + off @ (np.abs(offsets + codes) + np.abs(out)) + 2.0 ** -11 * rounded + \
-                    2.0 ** -33 * vs[t, g].max() * c.sum(0) * w.max() + (len(t) / 16 + 64) * u * (w @ np.abs(offsets) + part) + 2.0 ** -126
+                    2.0 ** -30 * vs[t, g].max() * c.sum(0) * w.max() + (len(t) / 16 + 64) * u * (w @ np.abs(offsets) + part) + 2.0 ** -126
                 if dtype == "f16":
                     limit[row, h] += 2.0 ** -25
             row += 1

@@ -383,7 +383,8 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
   }
   // Steps of the values are taken times a power of two, the same for a wave: 2^8 to 2^10 for the largest that any row has seen.  Weights up
   // to 2^5 (of a maximum that lags) times these are below float16's 65504.  A row that has seen only far smaller ones, as the large ones
-  // are hidden from it, has a maximum that is lower by its `lift`, so that its weights are larger by a power of two (limit: kLag and that).
+  // are hidden from it, has a maximum that is lower by its `lift`, so that its weights are larger by a power of two (limit: kLag and that):
+  // a row's own largest step is 2^5 or more, with what float16 loses of subnormal weights 2^-30 of it.
   // An offset counts as a step of 2^-14 of it: what is rounded beside it is far below its own rounding, and its sum stays in bounds.
   const auto power = [](int e) { return __uint_as_float((uint32_t)min(max(e + 127, 0), 254) << 23); };
   const auto exponent = [](uint32_t bits) { return (int)(bits >> 23) - 127; };
@@ -392,7 +393,7 @@ __global__ __launch_bounds__(64 * kAttentionWaves, 2) void kv_attention_kernel(A
   float v_scale = 1, size_limit = 0;                            // size_limit: a token above it may not fit; 0: none so far
   uint32_t most_seen = 0;                                       // by any row; numbers that are not negative are in order as integers
   bool uneven = false;                                          // whether rows have seen different ones: the largest of each is in row_size
-  constexpr int kMostSteps = 10, kLeastLift = 10, kMostLift = 100;
+  constexpr int kMostSteps = 10, kLeastLift = 4, kMostLift = 100;
   constexpr float kLag = 5;
 
   __shared__ __attribute__((aligned(16))) float params[kAttentionWaves][128];
