@@ -221,3 +221,37 @@ def test_large_values_that_some_queries_see_and_larger_ones_that_few_see(ctx, bi
     v[[n - 20, n - 7]] = O.rounded(v[[n - 20, n - 7]] * near, "bf16")
     q = np.zeros((q_len, heads, dim), np.float32)
     check(ctx, rng, q, [q_len], [k], [v], [n], bits, "bf16", window=window)
+
+
+@pytest.mark.parametrize("bits,heads,dim", [(4, 1, 64), (8, 3, 96), (4, 2, 100), (8, 1, 128), (4, 1, 256)])
+@pytest.mark.parametrize("seed", range(6))
+def test_runs_of_slots_of_every_kind(ctx, bits, heads, dim, seed):
+    """pieces in order that begin and end anywhere in a unit, whole units, single slots, slots in reverse and none, one after the other: written and
+    read back by other such pieces"""
+    rng = np.random.default_rng(seed)
+    total = 32 * (40 if seed < 3 else 400)
+
+    def pieces():
+        order, at = [], 0
+        cuts = rng.choice(np.arange(1, total), rng.integers(1, 60), replace=False)
+        cuts = np.unique(np.where(rng.random(len(cuts)) < 0.5, cuts // 32 * 32, cuts))
+        parts = [np.arange(a, b) for a, b in zip(np.r_[0, cuts], np.r_[cuts, total]) if a < b]
+        parts = [p[::-1] if rng.random() < 0.15 else rng.permutation(p) if rng.random() < 0.15 else p for p in parts]
+        rng.shuffle(parts)
+        for p in parts:
+            order += [np.full(rng.integers(0, 3), -1), p]
+        return np.concatenate(order)[:rng.integers(total // 2, total + 40)]
+
+    cache = KVCache(ctx, total // 32, heads, dim, bits, 32)
+    to = pieces()
+    assert len(np.unique(to[to >= 0])) == (to >= 0).sum()        # each slot once
+    x, y = (rows(rng, len(to), heads, dim, "bf16", False) for _ in "kv")
+    cache.write(array(ctx, x, "bf16"), array(ctx, y, "bf16"), array(ctx, to, "i32"))
+    back = pieces()
+    got = [DeviceArray.of(ctx, np.full((len(back), heads, dim), 7.0), "bf16") for _ in range(2)]
+    cache.read(array(ctx, back, "i32"), *got)
+    for a, b in zip(got, (x, y)):
+        held = np.zeros((total + 1, heads, dim), np.float32)     # the last one: of slots that are none
+        held[to[to >= 0]] = O.rounded(O.values(b, bits), "bf16")[to >= 0]
+        assert np.array_equal(a.numpy(), held[back])
+    cache.close()
