@@ -589,6 +589,72 @@ typedef struct {
 int tpuhip_kv_attention(tpuhip_ctx *ctx, const tpuhip_kv_cache *cache, const tpuhip_kv_attention_desc *desc, const void *q,
                         void *out, const int32_t *q_starts, const int32_t *kv_lens, const int32_t *page_table);
 
+/* The pages that the sequences of a batch have in a cache, kept on the device: a step's lengths in, page table, slots and starts of its queries
+ * out, as tpuhip_kv_write and tpuhip_kv_attention take them, with nothing read back in between, so that a recorded step goes on by
+ * itself.  All arrays are int32 in device memory and the caller's: lens (n_seq), the tokens that each sequence holds; table (n_seq rows of
+ * max_pages, table_stride apart), its pages, -1 behind the last; free_pages (pages) and n_free (1), a stack of pages that nobody has, the
+ * last of the first *n_free the next to go.  A page belongs to one sequence.  What the arrays say is cut to what there is: a length to
+ * max_pages * page_tokens and 2^30, a page that does not exist gives slots of -1. */
+typedef struct {
+  int n_seq, pages, page_tokens;      /* 1..65535 sequences; pages and page_tokens as the cache's */
+  int max_pages, table_stride;
+  int32_t *lens, *table, *free_pages, *n_free;
+} tpuhip_kv_pages;
+/* no tokens, all pages free: page 0 is the first to go */
+int tpuhip_kv_pages_clear(tpuhip_ctx *ctx, const tpuhip_kv_pages *pages);
+/* new_tokens[b] more tokens (none if negative) for each sequence b, in order: pages are taken off the stack for those that its last page has no
+ * room for, lens grows, q_starts (n_seq + 1) are the sums of what the sequences before each one got, slots[q_starts[b] + i] the slot of
+ * sequence b's new token i, and -1 behind the last one up to `capacity`, the entries of slots.  A sequence gets all of its tokens or none: none
+ * if its row of the table, or 2^30 tokens, are not enough; if the new tokens of all sequences up to it (but for those whose row is not enough)
+ * are more than `capacity`; or if it needs pages and those up to it need more than are free.  refused (1; may be NULL) counts the sequences
+ * that wanted tokens and got none.  What new_tokens, q_starts, slots and refused hold shares no memory with the batch's arrays. */
+int tpuhip_kv_pages_grow(tpuhip_ctx *ctx, const tpuhip_kv_pages *pages, const int32_t *new_tokens, int capacity, int32_t *q_starts,
+                         int32_t *slots, int32_t *refused);
+/* keep[b] tokens of sequence b stay (all, if it has no more; none if negative): the end of a draft, or of a sequence.  The pages behind them are
+ * free, their entries of the table -1, and the stack is as if they had never been taken: the next to grow get the same ones in the
+ * same order.  The rows of what stays are as they were. */
+int tpuhip_kv_pages_trim(tpuhip_ctx *ctx, const tpuhip_kv_pages *pages, const int32_t *keep);
+
+/* ---- Microscaled 4-bit floating point ----------------------------------------
+ * Rows of numbers in 4 bits with a scale for each 32 (the OCP microscaling format MXFP4), and their products: a language model's weights as they
+ * are stored, its activations as they are multiplied.  The reference quantises to INT8 and bfloat16 only; the products take the place of its
+ * fully connected layers' (core/fullyconnected.cpp) where these are too wide.
+ *
+ * A row of `cols` numbers is blocks of 32 columns, the last one filled up with zeros.  A block has a scale 2^e, held as the byte e + 127, and
+ * 16 bytes of codes, column 2i in the low half of byte i: a sign and one of 0, 0.5, 1, 1.5, 2, 3, 4, 6.  tpuhip_mx_quantize makes
+ *   e = floor(log2(max |x|)) - 2, at least -127 (zeros: -127),   code = the nearest to x / 2^e, a tie to the even one, at most 6,
+ * and of a block that holds an infinity or a NaN the byte 255, which makes a NaN of all its numbers.  Row i's codes begin at codes + i *
+ * codes_stride, its scales at scales + i * scales_stride; codes and codes_stride are multiples of 16 bytes, scales lie anywhere.  Codes past the
+ * last column are zeros: quantising writes them so, and codes from elsewhere have to be.
+ *
+ * Memory is the caller's, on the context's device; calls can be captured into a graph and allocate nothing, but for the 32 MiB of partial sums
+ * that a context has (see above). */
+typedef struct {
+  int rows, cols;           /* cols: 1..2^24 */
+  void *codes, *scales;
+  int64_t codes_stride, scales_stride;   /* bytes */
+} tpuhip_mx_matrix;
+/* x [rows, cols] of TPUHIP_BF16, TPUHIP_F16 or TPUHIP_F32, rows x_stride elements apart, a row's numbers next to each other */
+int tpuhip_mx_quantize(tpuhip_ctx *ctx, const tpuhip_mx_matrix *m, const void *x, int dtype, int64_t x_stride);
+/* the numbers that a matrix stands for, rounded once to the type */
+int tpuhip_mx_read(tpuhip_ctx *ctx, const tpuhip_mx_matrix *m, void *x, int dtype, int64_t x_stride);
+
+/* y = x w^T (+ bias) (+ residual): x has y's rows, w a row for each of y's columns, both as many columns.  bias: float32, one a column of y, or
+ * NULL; residual: like y, of its type, or NULL, and may be y itself.  Products are exact and summed in 32 bits (terms below 2^-126 may
+ * count as 0), and what the sum, the bias and the residual come to is rounded once.  The order of the sums depends on sizes alone, unless
+ * a context has no memory for partial sums (it gets it with its first product or cache outside of a recording). */
+typedef struct {
+  int dtype;                          /* of y and residual: TPUHIP_BF16, TPUHIP_F16 or TPUHIP_F32 */
+  int64_t y_stride, residual_stride;  /* elements */
+  const float *bias;
+  const void *residual;
+} tpuhip_mx_product_desc;
+int tpuhip_mx_product(tpuhip_ctx *ctx, const tpuhip_mx_product_desc *desc, const tpuhip_mx_matrix *x, const tpuhip_mx_matrix *w, void *y);
+/* The same with x quantised in the call: elements of x_dtype, as tpuhip_mx_quantize takes them.  room: a matrix of x's size, memory that the call
+ * may work in; what it holds afterwards is not said. */
+int tpuhip_mx_linear(tpuhip_ctx *ctx, const tpuhip_mx_product_desc *desc, const void *x, int x_dtype, int64_t x_stride,
+                     const tpuhip_mx_matrix *room, const tpuhip_mx_matrix *w, void *y);
+
 /* ---- module interpreter ------------------------------------------------------ */
 
 /* Flat view of the C++ ModuleInterpreter (include/tpuhip/interpreter.hpp), which

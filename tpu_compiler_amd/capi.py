@@ -77,6 +77,20 @@ class KVAttentionDesc(C.Structure):
         [("scale", C.c_float)] + [(k, C.c_int64) for k in ("q_token_stride", "q_head_stride", "out_token_stride", "out_head_stride")]
 
 
+class KVPagesDesc(C.Structure):
+    _fields_ = [(k, C.c_int) for k in ("n_seq", "pages", "page_tokens", "max_pages", "table_stride")] + \
+        [(k, C.c_void_p) for k in ("lens", "table", "free_pages", "n_free")]
+
+
+class MXMatrixDesc(C.Structure):
+    _fields_ = [("rows", C.c_int), ("cols", C.c_int), ("codes", C.c_void_p), ("scales", C.c_void_p), ("codes_stride", C.c_int64),
+                ("scales_stride", C.c_int64)]
+
+
+class MXProductDesc(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("y_stride", C.c_int64), ("residual_stride", C.c_int64), ("bias", C.c_void_p), ("residual", C.c_void_p)]
+
+
 ALGO_AUTO, ALGO_DIRECT, ALGO_MFMA, ALGO_DEPTHWISE, ALGO_DEPTHWISE_DOT, ALGO_STEM = 0, 1, 2, 3, 4, 5
 
 # name -> (restype, argtypes); every symbol include/tpuhip.h declares
@@ -262,6 +276,14 @@ PROTOTYPES.update({
     "tpuhip_kv_write": (C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(KVRows), C.c_void_p]),
     "tpuhip_kv_read": (C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(KVRows), C.c_void_p]),
     "tpuhip_kv_attention": (C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(KVAttentionDesc)] + [C.c_void_p] * 5),
+    "tpuhip_kv_pages_clear": (C.c_int, [C.c_void_p, C.POINTER(KVPagesDesc)]),
+    "tpuhip_kv_pages_grow": (C.c_int, [C.c_void_p, C.POINTER(KVPagesDesc), C.c_void_p, C.c_int] + [C.c_void_p] * 3),
+    "tpuhip_kv_pages_trim": (C.c_int, [C.c_void_p, C.POINTER(KVPagesDesc), C.c_void_p]),
+    "tpuhip_mx_quantize": (C.c_int, [C.c_void_p, C.POINTER(MXMatrixDesc), C.c_void_p, C.c_int, C.c_int64]),
+    "tpuhip_mx_read": (C.c_int, [C.c_void_p, C.POINTER(MXMatrixDesc), C.c_void_p, C.c_int, C.c_int64]),
+    "tpuhip_mx_product": (C.c_int, [C.c_void_p, C.POINTER(MXProductDesc), C.POINTER(MXMatrixDesc), C.POINTER(MXMatrixDesc), C.c_void_p]),
+    "tpuhip_mx_linear": (C.c_int, [C.c_void_p, C.POINTER(MXProductDesc), C.c_void_p, C.c_int, C.c_int64, C.POINTER(MXMatrixDesc),
+                                   C.POINTER(MXMatrixDesc), C.c_void_p]),
 })
 
 
@@ -433,12 +455,16 @@ class Context:
         self.lib, self.device, self.h = lib, device, h
         self.caches = weakref.WeakSet()      # key/value caches made by this context, which end with it,
         self.unfreed = []                    # and those that nobody holds but could not be freed yet
+        self.rooms = []                      # memory that products work in (mx.py), which ends with it too
 
     def close(self):
         if self.h:
             for c in list(self.caches) + self.unfreed:
                 c.close()
             self.unfreed = []
+            for r in self.rooms:
+                r.free()
+            self.rooms = []
             self.lib.tpuhip_ctx_destroy(self.h)
             self.h = None
 

@@ -10,12 +10,12 @@ import numpy as np
 from . import capi
 
 TYPES = {"bf16": 0, "f16": 1, "f32": 2}
-_SIZES = {"bf16": 2, "f16": 2, "f32": 4, "i32": 4}
-_NAMES = {"bfloat16": "bf16", "float16": "f16", "float32": "f32", "int32": "i32"}
+_SIZES = {"bf16": 2, "f16": 2, "f32": 4, "i32": 4, "u8": 1}
+_NAMES = {"bfloat16": "bf16", "float16": "f16", "float32": "f32", "int32": "i32", "uint8": "u8"}
 
 
 class DeviceArray:
-    """A dense array in device memory: "bf16" (numpy holds it as uint16), "f16", "f32" or "i32"."""
+    """A dense array in device memory: "bf16" (numpy holds it as uint16), "f16", "f32", "i32" or "u8"."""
 
     def __init__(self, ctx, shape, dtype):
         self.ctx, self.shape, self.dtype = ctx, tuple(int(n) for n in shape), dtype
@@ -28,20 +28,23 @@ class DeviceArray:
         """the values, rounded to the type (bf16: of what float32 holds of them)"""
         if dtype == "i32" and np.size(values) and not (-2 ** 31 <= np.min(values) and np.max(values) < 2 ** 31):
             _refuse("values: no ints of 32 bits")
+        if dtype == "u8" and np.size(values) and not (0 <= np.min(values) and np.max(values) < 256):
+            _refuse("values: no bytes")
         a = cls(ctx, np.shape(values), dtype)
         if dtype == "bf16":
             bits = np.ascontiguousarray(values, np.float32).view(np.uint32).astype(np.uint64)
             nan = (bits & 0x7FFFFFFF) > 0x7F800000
             host = np.where(nan, 0x7FC0, bits + 0x7FFF + (bits >> 16 & 1) >> 16).astype(np.uint16)
         else:
-            host = np.ascontiguousarray(values, {"f16": np.float16, "f32": np.float32, "i32": np.int32}[dtype])
+            host = np.ascontiguousarray(values, {"f16": np.float16, "f32": np.float32, "i32": np.int32, "u8": np.uint8}[dtype])
         if a.nbytes:
             ctx.upload(a.ptr, host)
         return a
 
     def numpy(self):
         """its values: float32 of bf16"""
-        host = self.ctx.download(self.ptr, self.shape, {"bf16": np.uint16, "f16": np.float16, "f32": np.float32, "i32": np.int32}[self.dtype])
+        types = {"bf16": np.uint16, "f16": np.float16, "f32": np.float32, "i32": np.int32, "u8": np.uint8}
+        host = self.ctx.download(self.ptr, self.shape, types[self.dtype])
         return (host.astype(np.uint32) << 16).view(np.float32) if self.dtype == "bf16" else host
 
     def data_ptr(self):
@@ -107,21 +110,38 @@ def _ints(x, what, ctx, shape):
     return x.data_ptr()
 
 
-class _Call:
-    """A checked call, to be made any number of times on the same arrays (it keeps them alive) while these, the cache and its context are
-    there."""
+class _Plan:
+    """A checked call, to be made any number of times on the same arrays (it keeps them alive) while these and its context are there."""
 
-    def __init__(self, cache, fn, args, keep):
-        self._cache, self._ctx, self._fn, self._args, self._keep = cache, cache.ctx, fn, args, keep
+    def __init__(self, ctx, fn, args, keep):
+        self._ctx, self._fn, self._args, self._keep = ctx, fn, args, keep
         self._arrays = [x for x in keep if isinstance(x, DeviceArray)]
         self._check()
 
     def _check(self):
-        if not self._cache.h or not self._ctx.h:
-            _refuse("the %s is closed" % ("context" if not self._ctx.h else "cache"))
+        if not self._ctx.h:
+            _refuse("the context is closed")
         for x in self._arrays:
             if not x.ptr:
                 _refuse("an array of the call has been freed")
+
+    def __call__(self):
+        self._check()
+        if rc := self._fn(self._ctx.h, *self._args):
+            self._ctx._ck(rc)
+
+
+class _Call(_Plan):
+    """one that is made on a cache"""
+
+    def __init__(self, cache, fn, args, keep):
+        self._cache = cache
+        super().__init__(cache.ctx, fn, args, keep)
+
+    def _check(self):
+        if not self._cache.h or not self._ctx.h:
+            _refuse("the %s is closed" % ("context" if not self._ctx.h else "cache"))
+        super()._check()
 
     def __call__(self):
         self._check()
@@ -204,3 +224,54 @@ class KVCache:
 
     def attention(self, q, out, q_starts, kv_lens, page_table, **how):
         self.plan_attention(q, out, q_starts, kv_lens, page_table, **how)()
+
+
+class KVPages:
+    """Which pages the sequences of a batch have in a cache (any number of caches whose pages are alike), kept on the device: arrays of int32,
+    lens [sequences], table [sequences, max_pages], free [pages], n_free [1], made here or the caller's, whose state they are.  `clear`
+    begins; `grow` gives new tokens pages and slots, `trim` takes tokens off."""
+
+    def __init__(self, ctx, pages, sequences, max_pages, page_tokens=64, lens=None, table=None, free=None, n_free=None):
+        given = [x is not None for x in (lens, table, free, n_free)]
+        if any(given) and not all(given):
+            _refuse("lens, table, free and n_free: all of them or none")
+        self.ctx, self.pages, self.sequences, self.max_pages = ctx, _int(pages, "pages"), _int(sequences, "sequences"), _int(max_pages, "max_pages")
+        self.page_tokens = _int(page_tokens, "page_tokens")
+        for n, what in ((self.pages, "pages"), (self.sequences, "sequences"), (self.max_pages, "max_pages")):
+            if n < 1:
+                _refuse("%s: %d" % (what, n))
+        shapes = (self.sequences,), (self.sequences, self.max_pages), (self.pages,), (1,)
+        if not any(given):
+            lens, table, free, n_free = (DeviceArray(ctx, shape, "i32") for shape in shapes)
+        self.lens, self.table, self.free, self.n_free = self._keep = lens, table, free, n_free
+        at = [_ints(x, what, ctx, shape) for x, what, shape in zip(self._keep, ("lens", "table", "free", "n_free"), shapes)]
+        stride = table.stride()[0] if self.sequences > 1 else self.max_pages
+        self._d = capi.KVPagesDesc(self.sequences, self.pages, self.page_tokens, self.max_pages, _int(stride, "table: distance of rows"), *at)
+        if not any(given):
+            self.clear()
+
+    def _plan(self, fn, args, keep):
+        return _Plan(self.ctx, fn, (self._d,) + args, self._keep + keep)
+
+    def clear(self):
+        """no tokens, all pages free, page 0 the first to go"""
+        self._plan(self.ctx.lib.tpuhip_kv_pages_clear, (), ())()
+
+    def plan_grow(self, new, q_starts, slots, refused=None):
+        """A call that gives sequence b new[b] more tokens: lens and table as they are afterwards, q_starts [sequences + 1], slots (-1 behind the last
+        token), refused [1]: how many sequences got none as there is no room for all of theirs."""
+        n = self.sequences
+        capacity = _int(slots.shape[0] if len(slots.shape) == 1 else -1, "slots")
+        args = (_ints(new, "new", self.ctx, (n,)), capacity, _ints(q_starts, "q_starts", self.ctx, (n + 1,)),
+                _ints(slots, "slots", self.ctx, (capacity,)), None if refused is None else _ints(refused, "refused", self.ctx, (1,)))
+        return self._plan(self.ctx.lib.tpuhip_kv_pages_grow, args, (new, q_starts, slots, refused))
+
+    def plan_trim(self, keep):
+        """a call that leaves sequence b its first keep[b] tokens: the pages behind them are free"""
+        return self._plan(self.ctx.lib.tpuhip_kv_pages_trim, (_ints(keep, "keep", self.ctx, (self.sequences,)),), (keep,))
+
+    def grow(self, new, q_starts, slots, refused=None):
+        self.plan_grow(new, q_starts, slots, refused)()
+
+    def trim(self, keep):
+        self.plan_trim(keep)()
