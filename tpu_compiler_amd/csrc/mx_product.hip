@@ -33,20 +33,45 @@ __device__ __forceinline__ void four_times(F f) {
   f(std::integral_constant<int, 3>{});
 }
 
-// The scales of a lane for 512 numbers of its row, blocks 16 chunk + 4 s + g, s = 0..3: byte s of a dword.  Past the row's end they are 0, 2^-127:
-// what such numbers of both operands make is below 2^-200, nothing in 32 bits, whatever the codes are.
-__device__ __forceinline__ uint32_t mx_scales(const uint8_t *row, int chunk, int blocks, int g) {
+// Scales 16 chunk .. 16 chunk + 15 of a row.  Past the row's end they are 0, 2^-127: what such numbers of both operands make is below 2^-200, nothing
+// in 32 bits, whatever the codes are.
+__device__ __forceinline__ uint4m mx_scales16(const uint8_t *row, int chunk, int blocks) {
+  typedef uint32_t dword_any __attribute__((aligned(1)));
+  typedef uint16_t half_any __attribute__((aligned(1)));
   const uint8_t *at = row + chunk * 16;
-  if (chunk * 16 + 16 <= blocks) {
-    const uint4m v = *(const uint4m_any *)at;
-    const uint32_t pick = 0x0C0C0400u + 0x0101u * (uint32_t)g;   // byte g of the second operand, byte g of the first
-    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(v[3], v[2], pick), __builtin_amdgcn_perm(v[1], v[0], pick), 0x05040100);
+  const int rest = blocks - chunk * 16;
+  if (rest >= 16) return *(const uint4m_any *)at;
+  uint4m v = {0, 0, 0, 0};
+  if (rest <= 0) return v;
+  uint64_t few = 0;                                            // of the rest, what is beyond eight
+  int shift = 0;
+  if (rest & 8) {
+    const uint2m first = *(const uint2m_any *)at;
+    v[0] = first[0], v[1] = first[1];
+    at += 8;
   }
-  uint32_t v = 0;
-#pragma unroll
-  for (int s = 0; s < 4; ++s)
-    if (chunk * 16 + 4 * s + g < blocks) v |= (uint32_t)at[4 * s + g] << 8 * s;
+  if (rest & 4) {
+    few = *(const dword_any *)at;
+    at += 4;
+    shift = 32;
+  }
+  if (rest & 2) {
+    few |= (uint64_t)*(const half_any *)at << shift;
+    at += 2;
+    shift += 16;
+  }
+  if (rest & 1) few |= (uint64_t)*at << shift;
+  if (rest & 8)
+    v[2] = (uint32_t)few, v[3] = (uint32_t)(few >> 32);
+  else
+    v[0] = (uint32_t)few, v[1] = (uint32_t)(few >> 32);
   return v;
+}
+// of them those of blocks 4 s + g, s = 0..3: byte s of a dword
+__device__ __forceinline__ uint32_t mx_scales(const uint8_t *row, int chunk, int blocks, int g) {
+  const uint4m v = mx_scales16(row, chunk, blocks);
+  const uint32_t pick = 0x0C0C0400u + 0x0101u * (uint32_t)g;   // byte g of the second operand, byte g of the first
+  return __builtin_amdgcn_perm(__builtin_amdgcn_perm(v[3], v[2], pick), __builtin_amdgcn_perm(v[1], v[0], pick), 0x05040100);
 }
 
 // four neighbours of a row of y
@@ -122,6 +147,183 @@ __global__ __launch_bounds__(64 * WAVES) void mx_stream_kernel(MxProductArgs a) 
   }
 }
 
+// Many rows of x: a workgroup of WM x WN waves has a tile of BM rows and BN columns of y.  256 numbers of the tile's rows
+// of both operands, a stage, come to LDS past the registers while the stage before is multiplied; a wave reads the operands of the next 64
+// numbers while it multiplies those that it has, so that the matrix unit waits for neither, and there is one barrier a stage.
+//   Order in LDS: rows of 128 bytes, block c of a row in place c ^ row % 8, so that eight lanes that read the same block of rows next to each other
+// use all banks.  Lane (r, g) has blocks 4g..4g + 3 of a stage: its scales are four bytes, a dword in LDS.
+constexpr int kMxStage = 8;   // blocks of a stage
+
+typedef __attribute__((address_space(1))) const uint8_t mx_global;
+typedef __attribute__((address_space(3))) uint8_t mx_lds;
+typedef float float16m __attribute__((ext_vector_type(16)));
+
+// 32 x 32 products of 64 numbers: lane (r, g) has row r's block g, and gets rows 8 i + 4 g + 0..3, i = 0..3, of column r
+template <int S>
+__device__ __forceinline__ float16m mx_mfma32(uint4m a, uint4m b, float16m c, uint32_t sa, uint32_t sb) {
+  const int8m va = {(int)a[0], (int)a[1], (int)a[2], (int)a[3]}, vb = {(int)b[0], (int)b[1], (int)b[2], (int)b[3]};
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(va, vb, c, 4, 4, S, (int)sa, S, (int)sb);
+}
+
+template <int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxProductArgs a) {
+  constexpr int WAVES = WM * WN, THREADS = 64 * WAVES, ROWS = BM + BN;
+  constexpr int MF = BM / WM / 32, NF = BN / WN / 32, L = ROWS / 8 / WAVES;  // fragments of a wave; pieces of 8 rows that it brings
+  constexpr int SR = ROWS / THREADS;                                         // rows whose scales a thread brings
+  static_assert(ROWS % THREADS == 0 && BM % (8 * WAVES) == 0 && MF % NF == 0);
+  __shared__ __attribute__((aligned(128))) uint8_t stage0[ROWS * 128];
+  __shared__ __attribute__((aligned(128))) uint8_t stage1[ROWS * 128];
+  __shared__ uint32_t scales[2][4][ROWS];                      // of two stages, four bytes each: [of which two][stage, g][row]
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 31, g = lane >> 5;
+  // Tiles: consecutive workgroups go to different XCDs; those of one have neighbouring tiles, four rows of tiles at a time, so that its L2 holds what
+  // they share
+  const int tiles_m = (a.rows + BM - 1) / BM, tiles_n = (a.cols + BN - 1) / BN, tiles = tiles_m * tiles_n;
+  const int per = tiles / 8, more = tiles % 8, xcd = (int)blockIdx.x % 8;
+  const int tile = xcd * per + min(xcd, more) + (int)blockIdx.x / 8;
+  const int group = tile / (4 * tiles_n), in_group = tile % (4 * tiles_n), high = min(4, tiles_m - 4 * group);
+  const int m0 = (4 * group + in_group % high) * BM, n0 = in_group / high * BN;
+  const int wm = wave % WM * (BM / WM), wn = wave / WM * (BN / WN);
+  // what a lane brings of a piece of 8 rows: a row, as an offset from the tile's first row, and a block
+  uint32_t from[L];
+#pragma unroll
+  for (int i = 0; i < L; ++i) {
+    const int row = (i * WAVES + wave) * 8 + (lane >> 3);
+    from[i] = i * WAVES * 8 < BM ? (uint32_t)min(row, a.rows - 1 - m0) * (uint32_t)a.x_stride : (uint32_t)min(row - BM, a.cols - 1 - n0) * (uint32_t)a.w_stride;
+  }
+  const int block = (lane & 7) ^ (lane >> 3);
+  const uint8_t *x0 = a.x + (int64_t)m0 * a.x_stride, *w0 = a.w + (int64_t)n0 * a.w_stride;
+  const int stages = (a.blocks + kMxStage - 1) / kMxStage;
+  const auto load = [&](int t, uint8_t *stage) {
+    t = min(t, stages - 1);                                    // no branch here: products would be moved past it
+    const uint32_t at = (uint32_t)(min(block, a.blocks - 1 - t * kMxStage) * kMxBytes);   // past the row's end, its last block again: its scales are 0
+#pragma unroll
+    for (int i = 0; i < L; ++i)
+      __builtin_amdgcn_global_load_lds((mx_global *)((i * WAVES * 8 < BM ? x0 : w0) + t * (kMxStage * kMxBytes) + (from[i] + at)),
+                                       (mx_lds *)(stage + (i * WAVES + wave) * 1024), 16, 0, 0);
+  };
+  const uint8_t *scale_rows[SR];
+#pragma unroll
+  for (int i = 0; i < SR; ++i) {
+    const int row = i * THREADS + threadIdx.x;
+    scale_rows[i] = row < BM ? a.xs + (int64_t)min(m0 + row, a.rows - 1) * a.xs_stride : a.ws + (int64_t)min(n0 + row - BM, a.cols - 1) * a.ws_stride;
+  }
+  uint4m next_scales[SR];
+  const auto load_scales = [&](int chunk) {                    // of the last stages they may be others': see below
+#pragma unroll
+    for (int i = 0; i < SR; ++i) next_scales[i] = *(const uint4m_any *)(scale_rows[i] + min(chunk * 16, a.blocks - 16));
+  };
+  const auto put_scales = [&](int chunk) {
+#pragma unroll
+    for (int i = 0; i < SR; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) scales[chunk & 1][k][i * THREADS + threadIdx.x] = next_scales[i][k];
+  };
+  struct Operands {
+    uint4m x[MF], w[NF];
+  };
+  struct Scales {
+    uint32_t x[MF], w[NF];
+  };
+  const auto read_scales = [&](Scales &s, int t) {
+    const uint32_t *at = scales[t >> 1 & 1][(t & 1) * 2 + g];
+#pragma unroll
+    for (int f = 0; f < MF; ++f) s.x[f] = at[wm + f * 32 + r];
+#pragma unroll
+    for (int f = 0; f < NF; ++f) s.w[f] = at[BM + wn + f * 32 + r];
+  };
+  const int at_x = (wm + r) * 128, at_w = (BM + wn + r) * 128, at_block = ((4 * g) ^ (r & 7)) * 16;   // of step 0; others by ^ 16 step
+  const auto read = [&](Operands &o, const uint8_t *stage, int s, int f) {   // one of w's fragments and as many parts of x's
+#pragma unroll
+    for (int i = f * MF / NF; i < (f + 1) * MF / NF; ++i) o.x[i] = *(const uint4m *)(stage + at_x + (at_block ^ s * 16) + i * 32 * 128);
+    o.w[f] = *(const uint4m *)(stage + at_w + (at_block ^ s * 16) + f * 32 * 128);
+  };
+  float16m acc[NF][MF] = {};
+  // multiplies `now` while the operands of step s of a stage are read
+  const auto step = [&](auto byte, auto reads, const Scales &sc, const Operands &now, Operands &next, const uint8_t *stage, int s) {
+    constexpr int S = decltype(byte)::value;
+#pragma unroll
+    for (int j = 0; j < NF; ++j) {
+      if constexpr (decltype(reads)::value) read(next, stage, s, j);
+#pragma unroll
+      for (int i = 0; i < MF; ++i) acc[j][i] = mx_mfma32<S>(now.w[j], now.x[i], acc[j][i], sc.w[j], sc.x[i]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  constexpr std::integral_constant<int, 0> b0{};
+  constexpr std::integral_constant<int, 1> b1{};
+  constexpr std::integral_constant<int, 2> b2{};
+  constexpr std::integral_constant<int, 3> b3{};
+  Operands p, q;
+  Scales sa, sb;                                               // of two stages
+  load(0, stage0);
+  load_scales(0);                                              // there are sixteen at least
+  put_scales(0);
+  __builtin_amdgcn_s_waitcnt(0x0F70);                          // vmcnt(0)
+  __syncthreads();
+  read_scales(sa, 0);                                          // before loads into LDS are on their way: the compiler has it wait for them
+  read_scales(sb, 1);
+  load(1, stage1);
+#pragma unroll
+  for (int f = 0; f < NF; ++f) read(p, stage0, 0, f);
+  const auto two_stages = [&](auto last, int chunk) {
+    constexpr bool LAST = decltype(last)::value;
+    const int t = chunk * 2;
+    if (!LAST) load_scales(chunk + 1);
+    step(b0, std::true_type{}, sa, p, q, stage0, 1);
+    step(b1, std::true_type{}, sa, q, p, stage0, 2);
+    step(b2, std::true_type{}, sa, p, q, stage0, 3);
+    __builtin_amdgcn_s_waitcnt(0x0F70);
+    __syncthreads();                                           // the next stage is there, this one has been read
+    if (!LAST) load(t + 2, stage0);
+    step(b3, std::true_type{}, sa, q, p, stage1, 0);
+    if (!LAST) put_scales(chunk + 1);
+    step(b0, std::true_type{}, sb, p, q, stage1, 1);
+    step(b1, std::true_type{}, sb, q, p, stage1, 2);
+    step(b2, std::true_type{}, sb, p, q, stage1, 3);
+    __builtin_amdgcn_s_waitcnt(0x0F70);
+    __syncthreads();
+    const Scales now = sb;
+    if (!LAST) {
+      read_scales(sa, t + 2);
+      read_scales(sb, t + 3);
+      load(t + 3, stage1);
+    }
+    step(b3, std::bool_constant<!LAST>{}, now, q, p, stage0, 0);
+  };
+  const int chunks = (stages + 1) / 2;
+  for (int chunk = 0; chunk < chunks - 1; ++chunk) two_stages(std::false_type{}, chunk);
+  if (a.blocks % 16) {                                         // the last scales, zeros past the end; out of the loop, as products would be moved past a branch
+#pragma unroll
+    for (int i = 0; i < SR; ++i) next_scales[i] = mx_scales16(scale_rows[i], chunks - 1, a.blocks);
+    __syncthreads();                                           // those that are there have been read
+    put_scales(chunks - 1);
+    __syncthreads();
+    read_scales(sa, chunks * 2 - 2);
+    read_scales(sb, chunks * 2 - 1);
+  }
+  two_stages(std::true_type{}, chunks - 1);
+  // Results go through LDS, a wave's by itself, 32 rows at a time: then a lane has four neighbours of a row, and FOURS lanes a row of the wave's.
+  // Four numbers c of row m lie in place c ^ m % 8.  All loads into LDS have been waited for, and all waves have read the last stage.
+  constexpr int FOURS = NF * 8;
+  static_assert(WAVES * 32 * FOURS * 16 <= ROWS * 128);
+  float4m *mine = (float4m *)stage0 + wave * 32 * FOURS;
+#pragma unroll
+  for (int i = 0; i < MF; ++i) {
+#pragma unroll
+    for (int j = 0; j < NF; ++j)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        mine[r * FOURS + ((j * 8 + 2 * k + g) ^ (r & 7))] = (float4m){acc[j][i][4 * k], acc[j][i][4 * k + 1], acc[j][i][4 * k + 2], acc[j][i][4 * k + 3]};
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+    for (int k = lane; k < 32 * FOURS; k += 64) {
+      const int row = k / FOURS, four = k % FOURS, m = m0 + wm + i * 32 + row, n = n0 + wn + 4 * four;
+      if (m < a.rows && n < a.cols) mx_result(a, m, n, mine[row * FOURS + (four ^ (row & 7))]);
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
 static int mx_product_args(tpuhip_ctx *ctx, const tpuhip_mx_product_desc *d, const tpuhip_mx_matrix *x, const tpuhip_mx_matrix *w, void *y,
                            const char *what, MxProductArgs *a) {
   TPUHIP_REQUIRE(ctx && d, "%s: NULL argument", what);
@@ -156,7 +358,20 @@ static int mx_product_args(tpuhip_ctx *ctx, const tpuhip_mx_product_desc *d, con
   return TPUHIP_OK;
 }
 
+template <int BM, int BN, int WM, int WN>
+static void mx_launch_tiles(tpuhip_ctx *ctx, const MxProductArgs &a) {
+  launch(ctx, mx_tile_kernel<BM, BN, WM, WN>, dim3((unsigned)(ceil_div64(a.rows, BM) * ceil_div64(a.cols, BN))), dim3(64 * WM * WN), a);
+}
+
 static int mx_multiply(tpuhip_ctx *ctx, const MxProductArgs &a) {
+  if (a.rows > 128 && a.blocks >= 16) {
+    if (ceil_div64(a.rows, 256) * ceil_div64(a.cols, 256) >= ctx->num_cu / 2)
+      mx_launch_tiles<256, 256, 2, 4>(ctx, a);
+    else
+      mx_launch_tiles<128, 128, 2, 2>(ctx, a);
+    TPUHIP_CHECK_HIP(hipGetLastError());
+    return TPUHIP_OK;
+  }
   launch(ctx, mx_stream_kernel<1, 1, 8>, dim3((unsigned)ceil_div64(a.cols, 16), (unsigned)ceil_div64(a.rows, 16)), dim3(512), a);
   TPUHIP_CHECK_HIP(hipGetLastError());
   return TPUHIP_OK;
