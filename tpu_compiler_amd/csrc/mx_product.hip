@@ -150,8 +150,8 @@ __global__ __launch_bounds__(64 * WAVES) void mx_stream_kernel(MxProductArgs a) 
 // Many rows of x: a workgroup of WM x WN waves has a tile of BM rows and BN columns of y.  256 numbers of the tile's rows
 // of both operands, a stage, come to LDS past the registers while the stage before is multiplied; a wave reads the operands of the next 64
 // numbers while it multiplies those that it has, so that the matrix unit waits for neither, and there is one barrier a stage.
-//   Order in LDS: rows of 128 bytes, block c of a row in place c ^ row % 8, so that eight lanes that read the same block of rows next to each other
-// use all banks.  Lane (r, g) has blocks 4g..4g + 3 of a stage: its scales are four bytes, a dword in LDS.
+//   Order in LDS: rows of 128 bytes, block c of a row in place c ^ row / 2 % 8, so that sixteen lanes that read the same block of rows next to each
+// other use all 64 banks (with row % 8 each read took twice the time).  Lane (r, g) has blocks 4g..4g + 3 of a stage: its scales are four bytes, a dword in LDS.
 constexpr int kMxStage = 8;   // blocks of a stage
 
 typedef __attribute__((address_space(1))) const uint8_t mx_global;
@@ -170,7 +170,7 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxProductArgs a) 
   constexpr int WAVES = WM * WN, THREADS = 64 * WAVES, ROWS = BM + BN;
   constexpr int MF = BM / WM / 32, NF = BN / WN / 32, L = ROWS / 8 / WAVES;  // fragments of a wave; pieces of 8 rows that it brings
   constexpr int SR = ROWS / THREADS;                                         // rows whose scales a thread brings
-  static_assert(ROWS % THREADS == 0 && BM % (8 * WAVES) == 0 && MF % NF == 0);
+  static_assert(ROWS % THREADS == 0 && BM % (8 * WAVES) == 0 && WAVES % 2 == 0 && MF % NF == 0);
   __shared__ __attribute__((aligned(128))) uint8_t stage0[ROWS * 128];
   __shared__ __attribute__((aligned(128))) uint8_t stage1[ROWS * 128];
   __shared__ uint32_t scales[2][4][ROWS];                      // of two stages, four bytes each: [of which two][stage, g][row]
@@ -190,7 +190,7 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxProductArgs a) 
     const int row = (i * WAVES + wave) * 8 + (lane >> 3);
     from[i] = i * WAVES * 8 < BM ? (uint32_t)min(row, a.rows - 1 - m0) * (uint32_t)a.x_stride : (uint32_t)min(row - BM, a.cols - 1 - n0) * (uint32_t)a.w_stride;
   }
-  const int block = (lane & 7) ^ (lane >> 3);
+  const int block = (lane & 7) ^ ((wave & 1) * 4 + (lane >> 4));
   const uint8_t *x0 = a.x + (int64_t)m0 * a.x_stride, *w0 = a.w + (int64_t)n0 * a.w_stride;
   const int stages = (a.blocks + kMxStage - 1) / kMxStage;
   const auto load = [&](int t, uint8_t *stage) {
@@ -231,7 +231,7 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxProductArgs a) 
 #pragma unroll
     for (int f = 0; f < NF; ++f) s.w[f] = at[BM + wn + f * 32 + r];
   };
-  const int at_x = (wm + r) * 128, at_w = (BM + wn + r) * 128, at_block = ((4 * g) ^ (r & 7)) * 16;   // of step 0; others by ^ 16 step
+  const int at_x = (wm + r) * 128, at_w = (BM + wn + r) * 128, at_block = ((4 * g) ^ (r >> 1 & 7)) * 16;   // of step 0; others by ^ 16 step
   const auto read = [&](Operands &o, const uint8_t *stage, int s, int f) {   // one of w's fragments and as many parts of x's
 #pragma unroll
     for (int i = f * MF / NF; i < (f + 1) * MF / NF; ++i) o.x[i] = *(const uint4m *)(stage + at_x + (at_block ^ s * 16) + i * 32 * 128);
@@ -302,26 +302,55 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxProductArgs a) 
     read_scales(sb, chunks * 2 - 1);
   }
   two_stages(std::true_type{}, chunks - 1);
-  // Results go through LDS, a wave's by itself, 32 rows at a time: then a lane has four neighbours of a row, and FOURS lanes a row of the wave's.
-  // Four numbers c of row m lie in place c ^ m % 8.  All loads into LDS have been waited for, and all waves have read the last stage.
-  constexpr int FOURS = NF * 8;
+  // Results go through LDS, a wave's by itself, 32 rows at a time: then a lane has four neighbours of a row, the same ones of every row, and FOURS lanes
+  // have a row of the wave's.  Four numbers c of row m lie in place c ^ m % 16.  All loads into LDS have been waited for, and all waves have read the last
+  // stage.
+  constexpr int FOURS = NF * 8, PASS = 64 / FOURS, PASSES = 32 / PASS;
   static_assert(WAVES * 32 * FOURS * 16 <= ROWS * 128);
   float4m *mine = (float4m *)stage0 + wave * 32 * FOURS;
+  const int four = lane % FOURS, row0 = lane / FOURS, n = n0 + wn + 4 * four;
+  const float4m bias = a.bias && n + 4 <= a.cols ? mx_load4(a.bias, n, TPUHIP_F32) : (float4m){0, 0, 0, 0};
+  const auto results = [&](auto type) {
+    constexpr int TYPE = decltype(type)::value;
 #pragma unroll
-  for (int i = 0; i < MF; ++i) {
+    for (int i = 0; i < MF; ++i) {
 #pragma unroll
-    for (int j = 0; j < NF; ++j)
+      for (int j = 0; j < NF; ++j)
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        mine[r * FOURS + ((j * 8 + 2 * k + g) ^ (r & 7))] = (float4m){acc[j][i][4 * k], acc[j][i][4 * k + 1], acc[j][i][4 * k + 2], acc[j][i][4 * k + 3]};
-    __builtin_amdgcn_wave_barrier();
-#pragma unroll 1
-    for (int k = lane; k < 32 * FOURS; k += 64) {
-      const int row = k / FOURS, four = k % FOURS, m = m0 + wm + i * 32 + row, n = n0 + wn + 4 * four;
-      if (m < a.rows && n < a.cols) mx_result(a, m, n, mine[row * FOURS + (four ^ (row & 7))]);
+        for (int k = 0; k < 4; ++k)
+          mine[r * FOURS + ((j * 8 + 2 * k + g) ^ (r & 15))] = (float4m){acc[j][i][4 * k], acc[j][i][4 * k + 1], acc[j][i][4 * k + 2], acc[j][i][4 * k + 3]};
+      __builtin_amdgcn_wave_barrier();
+      float4m v[PASSES];
+#pragma unroll
+      for (int k = 0; k < PASSES; ++k) {
+        const int row = k * PASS + row0;
+        v[k] = mine[row * FOURS + (four ^ (row & 15))];
+      }
+      __builtin_amdgcn_wave_barrier();
+      const int first = m0 + wm + i * 32 + row0;
+      if (n + 4 <= a.cols) {
+#pragma unroll
+        for (int k = 0; k < PASSES; ++k) v[k] += bias;
+        if (a.residual)
+#pragma unroll
+          for (int k = 0; k < PASSES; ++k)
+            if (first + k * PASS < a.rows) v[k] += mx_load4(a.residual, (int64_t)(first + k * PASS) * a.residual_stride + n, TYPE);
+#pragma unroll
+        for (int k = 0; k < PASSES; ++k)
+          if (first + k * PASS < a.rows) mx_store4(a.y, (int64_t)(first + k * PASS) * a.y_stride + n, TYPE, v[k]);
+      } else if (n < a.cols) {
+#pragma unroll
+        for (int k = 0; k < PASSES; ++k)
+          if (first + k * PASS < a.rows) mx_result(a, first + k * PASS, n, v[k]);
+      }
     }
-    __builtin_amdgcn_wave_barrier();
-  }
+  };
+  if (a.dtype == TPUHIP_BF16)
+    results(std::integral_constant<int, TPUHIP_BF16>{});
+  else if (a.dtype == TPUHIP_F16)
+    results(std::integral_constant<int, TPUHIP_F16>{});
+  else
+    results(std::integral_constant<int, TPUHIP_F32>{});
 }
 
 static int mx_product_args(tpuhip_ctx *ctx, const tpuhip_mx_product_desc *d, const tpuhip_mx_matrix *x, const tpuhip_mx_matrix *w, void *y,
