@@ -624,7 +624,8 @@ int tpuhip_kv_pages_trim(tpuhip_ctx *ctx, const tpuhip_kv_pages *pages, const in
  * 16 bytes of codes, column 2i in the low half of byte i: a sign and one of 0, 0.5, 1, 1.5, 2, 3, 4, 6.  tpuhip_mx_quantize makes
  *   e = floor(log2(max |x|)) - 2, at least -127 (zeros: -127),   code = the nearest to x / 2^e, a tie to the even one, at most 6,
  * and of a block that holds an infinity or a NaN the byte 255, which makes a NaN of all its numbers.  Row i's codes begin at codes + i *
- * codes_stride, its scales at scales + i * scales_stride; codes and codes_stride are multiples of 16 bytes, scales lie anywhere.  Codes past the
+ * codes_stride, its scales at scales + i * scales_stride; codes and codes_stride are multiples of 16 bytes (of a product's matrices below 2^24), scales
+ * lie anywhere.  Codes past the
  * last column are zeros: quantising writes them so, and codes from elsewhere have to be.
  *
  * Memory is the caller's, on the context's device; calls can be captured into a graph and allocate nothing, but for the 32 MiB of partial sums

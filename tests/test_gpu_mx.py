@@ -166,6 +166,41 @@ def test_sums_that_32_bits_hold_come_out_as_they_are(ctx, rows, cols, n):
     assert np.array_equal(out.numpy(), want)
 
 
+# sizes that take tiles of each size; sums of 256 numbers and of several times as many, whole and with a rest
+@pytest.mark.parametrize("rows,n", [(60, 1000), (250, 4096), (500, 4090), (770, 4096), (512, 16380), (2048, 8190)])
+@pytest.mark.parametrize("cols", [256, 512, 600, 768, 1024, 1250, 2304])
+def test_tiles_of_every_size_come_out_as_they_are_each_time(ctx, rows, cols, n):
+    if rows * cols * n > 2 ** 34.5:
+        pytest.skip("more of the same")
+    rng = np.random.default_rng(rows + cols + n)
+    x, w = codes_of(rng, rows, cols, 127, 128), codes_of(rng, n, cols, 126, 127)
+    xv, wv = O.values(*x, cols).astype(np.float32), O.values(*w, cols).astype(np.float32)
+    assert cols * 72 < 2 ** 24 / 8                     # in units of 2^-3, in any order
+    want = xv @ wv.T
+    a, b = matrix(ctx, *x, cols), matrix(ctx, *w, cols)
+    for _ in range(3):
+        out = DeviceArray.of(ctx, np.full((rows, n), 7.0), "f32")
+        mx.product(ctx, a, b, out)
+        assert np.array_equal(out.numpy(), want)
+        out.free()
+    for m in (a, b):
+        m.free()
+
+
+# long sums, shared by workgroups
+@pytest.mark.parametrize("rows,cols,n", [(1, 16384, 100), (2, 20000, 64), (17, 16384, 200), (40, 16384, 1000), (64, 8192, 4096), (128, 16384, 2048), (16, 30000, 512)])
+def test_long_sums(ctx, rows, cols, n):
+    rng = np.random.default_rng(cols)
+    x, w = codes_of(rng, rows, cols, 127, 127), codes_of(rng, n, cols, 127, 127)
+    want, _ = O.product(O.values(*x, cols), O.values(*w, cols))
+    assert cols * 36 < 2 ** 24 / 4
+    a, b = matrix(ctx, *x, cols), matrix(ctx, *w, cols)
+    for _ in range(3):
+        out = DeviceArray.of(ctx, np.full((rows, n), 7.0), "f32")
+        mx.product(ctx, a, b, out)
+        assert np.array_equal(out.numpy(), want)
+
+
 @pytest.mark.parametrize("ready", [False, True])
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("rows,cols,n", SHAPES)

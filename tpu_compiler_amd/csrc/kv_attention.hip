@@ -818,9 +818,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void kv_join_kernel(AttentionArgs 
   dst[c] = (uint16_t)store16(sum != 0 ? x / sum : 0.0f, a.bf16);
 }
 
-// Splits' sums: a split of 16 rows of 128 channels takes 8 KiB, three of them on each of 256 CUs 6 MiB.
-constexpr size_t kJoinBytes = 32 << 20;
-constexpr int kCounters = 16384, kJoinInKernel = 16;   // tiles with a counter; splits up to which the last workgroup joins them
+constexpr int kJoinInKernel = 16;   // splits up to which the last workgroup joins them
 
 int attention_workspace(tpuhip_ctx *ctx) {
   if (ctx->join) return TPUHIP_OK;

@@ -74,6 +74,10 @@ int kv_dispatch(const tpuhip_kv_cache *c, F f) {
   return set_error(TPUHIP_ERR_INVALID, "kv cache: no kernels for a head size of %d", c->desc.head_dim);
 }
 
+// ctx->join: counters of tiles, then splits' sums: of attention, where a split of 16 rows of 128 channels takes 8 KiB, three of them on each of 256
+// CUs 6 MiB, and of products (mx_product.hip).  All counters are 0 between launches.
+constexpr size_t kJoinBytes = 32 << 20;
+constexpr int kCounters = 16384;
 // kv_attention.hip: makes ctx->join if it can
 int attention_workspace(tpuhip_ctx *ctx);
 

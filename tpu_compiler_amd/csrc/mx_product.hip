@@ -1,4 +1,5 @@
 // Products of rows of microscaled 4-bit numbers: y = x w^T (+ bias) (+ residual).
+#include "kv_cache.hpp"
 #include "mx.hpp"
 
 #include <algorithm>
@@ -14,6 +15,10 @@ struct MxProductArgs {
   void *y;
   int64_t y_stride, residual_stride;
   int rows, cols, blocks, dtype;
+  int depth;                        // numbers of a row, where x is elements; x_stride counts those then
+  int splits, split_chunks;         // of the sums over 512 numbers each, among workgroups: of each tile; of them
+  float *part;                      // their sums
+  int *counters;                    // of each tile: splits that have ended
 };
 
 typedef int int8m __attribute__((ext_vector_type(8)));
@@ -68,11 +73,11 @@ __device__ __forceinline__ uint4m mx_scales16(const uint8_t *row, int chunk, int
   return v;
 }
 // of them those of blocks 4 s + g, s = 0..3: byte s of a dword
-__device__ __forceinline__ uint32_t mx_scales(const uint8_t *row, int chunk, int blocks, int g) {
-  const uint4m v = mx_scales16(row, chunk, blocks);
+__device__ __forceinline__ uint32_t mx_picked(uint4m v, int g) {
   const uint32_t pick = 0x0C0C0400u + 0x0101u * (uint32_t)g;   // byte g of the second operand, byte g of the first
   return __builtin_amdgcn_perm(__builtin_amdgcn_perm(v[3], v[2], pick), __builtin_amdgcn_perm(v[1], v[0], pick), 0x05040100);
 }
+__device__ __forceinline__ uint32_t mx_scales(const uint8_t *row, int chunk, int blocks, int g) { return mx_picked(mx_scales16(row, chunk, blocks), g); }
 
 // four neighbours of a row of y
 __device__ __forceinline__ void mx_result(const MxProductArgs &a, int m, int n, float4m v) {
@@ -92,69 +97,141 @@ __device__ __forceinline__ void mx_result(const MxProductArgs &a, int m, int n, 
   }
 }
 
-// Few rows of x: a workgroup has 16 NT columns of y (rows of w) and 16 MT rows; its waves take every so manieth 512 numbers of the sums, operands
-// come from memory as they lie, and the waves' sums meet in LDS, added in the waves' order.
-template <int NT, int MT, int WAVES>
+// A few rows of x, 16 at most: they lie in LDS as codes while a workgroup goes from 16 columns of y (rows of w) to the next.  Its waves take every
+// so manieth 512 numbers of the sums, a chunk; w comes from memory as it lies, a chunk ahead, whichever columns that belongs to; the waves' sums meet in LDS,
+// added in the waves' order.
+//   TYPE: of x's elements, which the workgroup quantises for itself, eight numbers a lane; kMxCodes: x is a matrix.
+constexpr int kMxCodes = -1, kMxFew = 16;
+constexpr int kMxFewPieces = 32;   // of x, 512 numbers of a row each
+
+template <int TYPE>
+struct MxRaw {                       // what a lane brings of 512 numbers of a row
+  uint4m v[TYPE == TPUHIP_F32 ? 2 : 1];
+};
+
+template <int WAVES, int TYPE>
 __global__ __launch_bounds__(64 * WAVES) void mx_stream_kernel(MxProductArgs a) {
-  __shared__ float4m sums[WAVES][NT * MT][64];
+  __shared__ uint4m rows[kMxFewPieces * 17];                   // [chunk][row][17]: 16 blocks of codes, their scales
+  __shared__ float4m sums[2][WAVES][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
-  const int n0 = (int)blockIdx.x * 16 * NT, m0 = (int)blockIdx.y * 16 * MT;
-  const uint8_t *w[NT], *ws[NT], *x[MT], *xs[MT];
+  const int chunks = (a.blocks + 15) / 16, tiles = (a.cols + 15) / 16, count = a.rows * chunks;
+  struct Chunk {
+    uint4m w[4];
+    uint32_t s;
+  };
+  const auto load = [&](Chunk &c, int tile, int chunk) {
+    const int64_t n = min(tile * 16 + r, a.cols - 1);          // past the end, the last row again
+    const uint8_t *w = a.w + n * a.w_stride;
 #pragma unroll
-  for (int j = 0; j < NT; ++j) {                               // past the end, the last row again
-    const int64_t n = min(n0 + 16 * j + r, a.cols - 1);
-    w[j] = a.w + n * a.w_stride;
-    ws[j] = a.ws + n * a.ws_stride;
+    for (int s = 0; s < 4; ++s) c.w[s] = *(const uint4m *)(w + (int64_t)min(chunk * 16 + 4 * s + g, a.blocks - 1) * kMxBytes);
+    c.s = mx_scales(a.ws + n * a.ws_stride, chunk, a.blocks, g);
+  };
+  Chunk now;
+  int tile = (int)blockIdx.x;
+  constexpr int BATCH = 4;
+  for (int first = wave; first < max(count, 1 + wave); first += BATCH * WAVES) {
+    MxRaw<TYPE> raw[BATCH];
+    const auto item = [&](int b, int &m, int &chunk) {         // rows of a chunk follow each other
+      const int i = first + b * WAVES;
+      chunk = i / a.rows;
+      m = i % a.rows;
+      return i < count;
+    };
+#pragma unroll
+    for (int b = 0; b < BATCH; ++b) {
+      int m, chunk;
+      if (!item(b, m, chunk)) continue;
+      if constexpr (TYPE == kMxCodes) {
+        const int block = chunk * 16 + lane / 4;
+        const bool there = block < a.blocks;
+        raw[b].v[0][0] = there ? ((const uint32_t *)(a.x + m * a.x_stride + (int64_t)block * kMxBytes))[lane & 3] : 0;
+        raw[b].v[0][1] = there ? a.xs[m * a.xs_stride + block] : 0;
+      } else {
+        const int col = chunk * 512 + lane * 8;
+        const int64_t at = m * a.x_stride + col;
+        if (chunk * 512 + 512 <= a.depth) {
+          if constexpr (TYPE == TPUHIP_F32) {
+            raw[b].v[0] = *(const uint4m_any *)((const float *)a.x + at);
+            raw[b].v[1] = *(const uint4m_any *)((const float *)a.x + at + 4);
+          } else {
+            raw[b].v[0] = *(const uint4m_any *)((const uint16_t *)a.x + at);
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const bool there = col + k < a.depth;
+            if constexpr (TYPE == TPUHIP_F32)
+              raw[b].v[k / 4][k % 4] = there ? ((const uint32_t *)a.x)[at + k] : 0;
+            else
+              raw[b].v[0][k / 2] = (k % 2 ? raw[b].v[0][k / 2] : 0) | (there ? (uint32_t)((const uint16_t *)a.x)[at + k] : 0u) << 16 * (k % 2);
+          }
+        }
+      }
+    }
+    if (first == wave && wave < chunks) load(now, min(tile, tiles - 1), wave);   // behind x, which is waited for first
+#pragma unroll
+    for (int b = 0; b < BATCH; ++b) {
+      int m, chunk;
+      if (!item(b, m, chunk)) continue;
+      uint32_t code, byte;
+      if constexpr (TYPE == kMxCodes) {
+        code = raw[b].v[0][0];
+        byte = raw[b].v[0][1];
+      } else {
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          if constexpr (TYPE == TPUHIP_F32) {
+            v[k] = __uint_as_float(raw[b].v[k / 4][k % 4]);
+          } else {
+            const uint32_t pair = raw[b].v[0][k / 2];
+            v[k] = TYPE == TPUHIP_BF16 ? __uint_as_float(k % 2 ? pair & 0xFFFF0000u : pair << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)(pair >> 16 * (k % 2)));
+          }
+        }
+        code = mx_quantised8(v, byte);
+      }
+      uint4m *at = rows + (chunk * a.rows + m) * 17;
+      ((uint32_t *)at)[lane] = code;
+      if ((lane & 3) == 0) ((uint8_t *)(at + 16))[lane >> 2] = (uint8_t)byte;
+    }
   }
-#pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    const int64_t m = min(m0 + 16 * i + r, a.rows - 1);
-    x[i] = a.x + m * a.x_stride;
-    xs[i] = a.xs + m * a.xs_stride;
-  }
-  float4m acc[NT][MT] = {};
-  for (int chunk = wave; chunk * 16 < a.blocks; chunk += WAVES) {
-    uint32_t sw[NT], sx[MT];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) sw[j] = mx_scales(ws[j], chunk, a.blocks, g);
-#pragma unroll
-    for (int i = 0; i < MT; ++i) sx[i] = mx_scales(xs[i], chunk, a.blocks, g);
-    four_times([&](auto s) {
-      constexpr int S = decltype(s)::value;
-      const int64_t at = (int64_t)min(chunk * 16 + 4 * S + g, a.blocks - 1) * kMxBytes;
-      uint4m vw[NT], vx[MT];
-#pragma unroll
-      for (int j = 0; j < NT; ++j) vw[j] = *(const uint4m *)(w[j] + at);
-#pragma unroll
-      for (int i = 0; i < MT; ++i) vx[i] = *(const uint4m *)(x[i] + at);
-#pragma unroll
-      for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int i = 0; i < MT; ++i) acc[j][i] = mx_mfma<S>(vw[j], vx[i], acc[j][i], sw[j], sx[i]);
-    });
-  }
-#pragma unroll
-  for (int j = 0; j < NT; ++j)
-#pragma unroll
-    for (int i = 0; i < MT; ++i) sums[wave][j * MT + i][lane] = acc[j][i];
   __syncthreads();
-  for (int k = threadIdx.x; k < NT * MT * 64; k += 64 * WAVES) {
-    float4m v = sums[0][k / 64][k % 64];
+  const uint4m *mine = rows + min(r, a.rows - 1) * 17;         // behind the last row it again: its results go nowhere
+  for (int turn = 0; tile < tiles; tile += (int)gridDim.x, ++turn) {
+    float4m acc = {};
+    for (int chunk = wave; chunk < chunks; chunk += WAVES) {
+      const bool last = chunk + WAVES >= chunks;
+      Chunk next;
+      load(next, min(last ? tile + (int)gridDim.x : tile, tiles - 1), last ? wave : chunk + WAVES);
+      const uint4m *x = mine + chunk * a.rows * 17;
+      const uint32_t sx = mx_picked(x[16], g);
+      four_times([&](auto s) {
+        constexpr int S = decltype(s)::value;
+        acc = mx_mfma<S>(now.w[S], x[4 * S + g], acc, now.s, sx);
+      });
+      now = next;
+    }
+    sums[turn & 1][wave][lane] = acc;
+    __syncthreads();
+    // a wave adds them while the others go on; it is there again before they are written the time after the next
+    if (wave == turn % WAVES) {
+      const int n = tile * 16 + g * 4;
+      float4m v = sums[turn & 1][0][lane];
 #pragma unroll
-    for (int i = 1; i < WAVES; ++i) v += sums[i][k / 64][k % 64];
-    const int m = m0 + k / 64 % MT * 16 + k % 16, n = n0 + k / 64 / MT * 16 + k % 64 / 16 * 4;
-    if (m < a.rows && n < a.cols) mx_result(a, m, n, v);
+      for (int i = 1; i < WAVES; ++i) v += sums[turn & 1][i][lane];
+      if (r < a.rows && n < a.cols) mx_result(a, r, n, v);
+    }
   }
 }
 
-// Many rows of x: a workgroup of WM x WN waves has a tile of BM rows and BN columns of y.  256 numbers of the tile's rows
-// of both operands, a stage, come to LDS past the registers while the stage before is multiplied; a wave reads the operands of the next 64
-// numbers while it multiplies those that it has, so that the matrix unit waits for neither, and there is one barrier a stage.
+// Many rows of x: a workgroup of WM x WN waves has a tile of BM rows and BN columns of y.  256 numbers of the tile's rows of both operands, a stage, come
+// to LDS past the registers, S stages' room in turn; a wave reads the operands of the next 64 numbers while it multiplies those that it has.  Before a
+// stage's last products all waves have read it and the next one has come (one barrier a stage), and its room is filled anew.
 //   Order in LDS: rows of 128 bytes, block c of a row in place c ^ row / 2 % 8, so that sixteen lanes that read the same block of rows next to each
-// other use all 64 banks (with row % 8 each read took twice the time).  Lane (r, g) has blocks 4g..4g + 3 of a stage: its scales are four bytes, a dword in LDS.
+// other use all 64 banks (with row % 8 each read took twice the time).  Lane (r, g) has blocks 4g..4g + 3 of a stage: its scales are four bytes.
+// Scales come by way of registers, two stages' at a time, and are written in the odd stages, behind the data that are being multiplied: an access to LDS waits for the loads that are on their way to the same array, and one to an array that has none for all of them.
 constexpr int kMxStage = 8;   // blocks of a stage
 
-typedef __attribute__((address_space(1))) const uint8_t mx_global;
 typedef __attribute__((address_space(3))) uint8_t mx_lds;
 typedef float float16m __attribute__((ext_vector_type(16)));
 
@@ -165,58 +242,89 @@ __device__ __forceinline__ float16m mx_mfma32(uint4m a, uint4m b, float16m c, ui
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(va, vb, c, 4, 4, S, (int)sa, S, (int)sb);
 }
 
-template <int BM, int BN, int WM, int WN>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t mx_buffer(const uint8_t *first, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(first), 0, bytes, 0x00020000);
+}
+// sixteen bytes a lane, from `at` + the lane's `from`, past the registers to LDS, a lane's behind the other's; zeros from behind the buffer's end
+__device__ __forceinline__ void mx_to_lds(__amdgpu_buffer_rsrc_t buffer, uint8_t *to, uint32_t from, int at) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer, (mx_lds *)to, 16, (int)from, at, 0, 0);
+}
+
+template <int BM, int BN, int WM, int WN, int S>
 __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxProductArgs a) {
   constexpr int WAVES = WM * WN, THREADS = 64 * WAVES, ROWS = BM + BN;
   constexpr int MF = BM / WM / 32, NF = BN / WN / 32, L = ROWS / 8 / WAVES;  // fragments of a wave; pieces of 8 rows that it brings
-  constexpr int SR = ROWS / THREADS;                                         // rows whose scales a thread brings
-  static_assert(ROWS % THREADS == 0 && BM % (8 * WAVES) == 0 && WAVES % 2 == 0 && MF % NF == 0);
-  __shared__ __attribute__((aligned(128))) uint8_t stage0[ROWS * 128];
-  __shared__ __attribute__((aligned(128))) uint8_t stage1[ROWS * 128];
-  __shared__ uint32_t scales[2][4][ROWS];                      // of two stages, four bytes each: [of which two][stage, g][row]
+  constexpr int SR = (ROWS + THREADS - 1) / THREADS;                         // rows whose scales a thread brings
+  constexpr int SCALES = ROWS * 128, SIZE = SCALES + ROWS * 16;              // where they lie, and a stage's room
+  static_assert(BM % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0 && WAVES % 2 == 0 && (S == 2 || S == 4));
+  __shared__ __attribute__((aligned(128))) uint8_t room0[SIZE];
+  __shared__ __attribute__((aligned(128))) uint8_t room1[SIZE];
+  __shared__ __attribute__((aligned(128))) uint8_t room2[S > 2 ? SIZE : 16];
+  __shared__ __attribute__((aligned(128))) uint8_t room3[S > 2 ? SIZE : 16];
+  const auto room = [&](auto u) -> uint8_t * {
+    constexpr int U = decltype(u)::value % S;
+    if constexpr (U == 0) return room0;
+    if constexpr (U == 1) return room1;
+    if constexpr (U == 2) return room2;
+    return room3;
+  };
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 31, g = lane >> 5;
   // Tiles: consecutive workgroups go to different XCDs; those of one have neighbouring tiles, four rows of tiles at a time, so that its L2 holds what
   // they share
-  const int tiles_m = (a.rows + BM - 1) / BM, tiles_n = (a.cols + BN - 1) / BN, tiles = tiles_m * tiles_n;
-  const int per = tiles / 8, more = tiles % 8, xcd = (int)blockIdx.x % 8;
-  const int tile = xcd * per + min(xcd, more) + (int)blockIdx.x / 8;
+  const int tiles_m = (a.rows + BM - 1) / BM, tiles_n = (a.cols + BN - 1) / BN;
+  const int per = (int)gridDim.x / 8, more = (int)gridDim.x % 8, xcd = (int)blockIdx.x % 8;
+  const int work = xcd * per + min(xcd, more) + (int)blockIdx.x / 8, tile = work / a.splits, split = work % a.splits;
   const int group = tile / (4 * tiles_n), in_group = tile % (4 * tiles_n), high = min(4, tiles_m - 4 * group);
   const int m0 = (4 * group + in_group % high) * BM, n0 = in_group / high * BN;
   const int wm = wave % WM * (BM / WM), wn = wave / WM * (BN / WN);
-  // what a lane brings of a piece of 8 rows: a row, as an offset from the tile's first row, and a block
+  // What a lane brings of a piece of 8 rows: a row and a block, as an offset from the tile's first row.  Past a row's end, where scales are 0, that is
+  // anything: the next row, or zeros behind the last one, which the buffers' sizes end at.
   uint32_t from[L];
 #pragma unroll
   for (int i = 0; i < L; ++i) {
     const int row = (i * WAVES + wave) * 8 + (lane >> 3);
-    from[i] = i * WAVES * 8 < BM ? (uint32_t)min(row, a.rows - 1 - m0) * (uint32_t)a.x_stride : (uint32_t)min(row - BM, a.cols - 1 - n0) * (uint32_t)a.w_stride;
+    from[i] = (i * WAVES * 8 < BM ? (uint32_t)min(row, a.rows - 1 - m0) * (uint32_t)a.x_stride : (uint32_t)min(row - BM, a.cols - 1 - n0) * (uint32_t)a.w_stride) +
+              ((lane & 7) ^ ((wave & 1) * 4 + (lane >> 4))) * kMxBytes;
   }
-  const int block = (lane & 7) ^ ((wave & 1) * 4 + (lane >> 4));
-  const uint8_t *x0 = a.x + (int64_t)m0 * a.x_stride, *w0 = a.w + (int64_t)n0 * a.w_stride;
-  const int stages = (a.blocks + kMxStage - 1) / kMxStage;
-  const auto load = [&](int t, uint8_t *stage) {
-    t = min(t, stages - 1);                                    // no branch here: products would be moved past it
-    const uint32_t at = (uint32_t)(min(block, a.blocks - 1 - t * kMxStage) * kMxBytes);   // past the row's end, its last block again: its scales are 0
+  const auto bytes = [&](int rows, int64_t stride) { return (uint32_t)(rows - 1) * (uint32_t)stride + (uint32_t)(a.blocks * kMxBytes); };
+  const uint8_t *const x0 = a.x + (int64_t)m0 * a.x_stride, *const w0 = a.w + (int64_t)n0 * a.w_stride;
+  const uint32_t x_bytes = bytes(min(BM, a.rows - m0), a.x_stride), w_bytes = bytes(min(BN, a.cols - n0), a.w_stride);
+  const int chunk0 = split * a.split_chunks, stage0 = chunk0 * 2;             // this one's
+  const int stages = min((a.blocks + kMxStage - 1) / kMxStage, stage0 + a.split_chunks * 2) - stage0;
+  const auto load = [&](int t, uint8_t *to) {                  // behind the last stage, of nothing; no branch here: products would be moved past it
+    const bool there = t < stages;
+    const auto x = mx_buffer(x0, there ? x_bytes : 0), w = mx_buffer(w0, there ? w_bytes : 0);
+    const int at = there ? (stage0 + t) * (kMxStage * kMxBytes) : 0;
 #pragma unroll
-    for (int i = 0; i < L; ++i)
-      __builtin_amdgcn_global_load_lds((mx_global *)((i * WAVES * 8 < BM ? x0 : w0) + t * (kMxStage * kMxBytes) + (from[i] + at)),
-                                       (mx_lds *)(stage + (i * WAVES + wave) * 1024), 16, 0, 0);
+    for (int i = 0; i < L; ++i) mx_to_lds(i * WAVES * 8 < BM ? x : w, to + (i * WAVES + wave) * 1024, from[i], at);
+  };
+  // scales 16 chunk .. 16 chunk + 15 of a thread's rows.  Without a branch: sixteen that there are, and a shift by bytes; rows of fewer have one
+  // chunk, whose scales are not brought here.
+  const auto scale_row = [&](int row) {
+    return row < BM ? a.xs + (int64_t)min(m0 + row, a.rows - 1) * a.xs_stride : a.ws + (int64_t)min(n0 + row - BM, a.cols - 1) * a.ws_stride;
   };
   const uint8_t *scale_rows[SR];
 #pragma unroll
-  for (int i = 0; i < SR; ++i) {
-    const int row = i * THREADS + threadIdx.x;
-    scale_rows[i] = row < BM ? a.xs + (int64_t)min(m0 + row, a.rows - 1) * a.xs_stride : a.ws + (int64_t)min(n0 + row - BM, a.cols - 1) * a.ws_stride;
-  }
+  for (int i = 0; i < SR; ++i) scale_rows[i] = a.blocks >= 16 ? scale_row(min(i * THREADS + (int)threadIdx.x, ROWS - 1)) : a.w;
   uint4m next_scales[SR];
-  const auto load_scales = [&](int chunk) {                    // of the last stages they may be others': see below
+  const auto load_scales = [&](int chunk) {
 #pragma unroll
-    for (int i = 0; i < SR; ++i) next_scales[i] = *(const uint4m_any *)(scale_rows[i] + min(chunk * 16, a.blocks - 16));
+    for (int i = 0; i < SR; ++i) next_scales[i] = *(const uint4m_any *)(scale_rows[i] + max(min(chunk * 16, a.blocks - 16), 0));
   };
-  const auto put_scales = [&](int chunk) {
+  const auto put_scales = [&](int chunk, uint8_t *to) {
+    const int drop = min(chunk * 16 - min(chunk * 16, a.blocks - 16), 15);
+    const uint32_t one = drop & 4 ? ~0u : 0u, two = drop & 8 ? ~0u : 0u, bytes = drop & 3;
+    const auto pick = [](uint32_t mask, uint32_t x, uint32_t y) { return (x & mask) | (y & ~mask); };
 #pragma unroll
-    for (int i = 0; i < SR; ++i)
+    for (int i = 0; i < SR; ++i) {
+      uint4m v = next_scales[i];
+      v = (uint4m){pick(one, v[1], v[0]), pick(one, v[2], v[1]), pick(one, v[3], v[2]), v[3] & ~one};
+      v = (uint4m){pick(two, v[2], v[0]), pick(two, v[3], v[1]), v[2] & ~two, v[3] & ~two};
+      v = (uint4m){__builtin_amdgcn_alignbyte(v[1], v[0], bytes), __builtin_amdgcn_alignbyte(v[2], v[1], bytes),
+                   __builtin_amdgcn_alignbyte(v[3], v[2], bytes), __builtin_amdgcn_alignbyte(0, v[3], bytes)};
 #pragma unroll
-      for (int k = 0; k < 4; ++k) scales[chunk & 1][k][i * THREADS + threadIdx.x] = next_scales[i][k];
+      for (int k = 0; k < 4; ++k) ((uint32_t *)(to + SCALES))[k * ROWS + min(i * THREADS + (int)threadIdx.x, ROWS - 1)] = v[k];   // some threads have the same row
+    }
   };
   struct Operands {
     uint4m x[MF], w[NF];
@@ -224,90 +332,170 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxProductArgs a) 
   struct Scales {
     uint32_t x[MF], w[NF];
   };
-  const auto read_scales = [&](Scales &s, int t) {
-    const uint32_t *at = scales[t >> 1 & 1][(t & 1) * 2 + g];
+  Scales sa, sb;                                               // of two stages
+  const auto read_scales = [&](const uint8_t *from) {
+    const uint32_t *at = (const uint32_t *)(from + SCALES) + g * ROWS;
 #pragma unroll
-    for (int f = 0; f < MF; ++f) s.x[f] = at[wm + f * 32 + r];
+    for (int f = 0; f < MF; ++f) sa.x[f] = at[wm + f * 32 + r], sb.x[f] = at[2 * ROWS + wm + f * 32 + r];
 #pragma unroll
-    for (int f = 0; f < NF; ++f) s.w[f] = at[BM + wn + f * 32 + r];
+    for (int f = 0; f < NF; ++f) sa.w[f] = at[BM + wn + f * 32 + r], sb.w[f] = at[2 * ROWS + BM + wn + f * 32 + r];
   };
   const int at_x = (wm + r) * 128, at_w = (BM + wn + r) * 128, at_block = ((4 * g) ^ (r >> 1 & 7)) * 16;   // of step 0; others by ^ 16 step
-  const auto read = [&](Operands &o, const uint8_t *stage, int s, int f) {   // one of w's fragments and as many parts of x's
+  const auto read = [&](Operands &o, const uint8_t *from, int s, int f) {   // one of w's fragments and as many parts of x's
 #pragma unroll
-    for (int i = f * MF / NF; i < (f + 1) * MF / NF; ++i) o.x[i] = *(const uint4m *)(stage + at_x + (at_block ^ s * 16) + i * 32 * 128);
-    o.w[f] = *(const uint4m *)(stage + at_w + (at_block ^ s * 16) + f * 32 * 128);
+    for (int i = f * MF / NF; i < (f + 1) * MF / NF; ++i) o.x[i] = *(const uint4m *)(from + at_x + (at_block ^ s * 16) + i * 32 * 128);
+    o.w[f] = *(const uint4m *)(from + at_w + (at_block ^ s * 16) + f * 32 * 128);
   };
   float16m acc[NF][MF] = {};
   // multiplies `now` while the operands of step s of a stage are read
-  const auto step = [&](auto byte, auto reads, const Scales &sc, const Operands &now, Operands &next, const uint8_t *stage, int s) {
-    constexpr int S = decltype(byte)::value;
+  const auto step = [&](auto byte, auto reads, const Scales &sc, const Operands &now, Operands &next, const uint8_t *from, int s) {
+    constexpr int B = decltype(byte)::value;
 #pragma unroll
     for (int j = 0; j < NF; ++j) {
-      if constexpr (decltype(reads)::value) read(next, stage, s, j);
+      if constexpr (decltype(reads)::value) read(next, from, s, j);
 #pragma unroll
-      for (int i = 0; i < MF; ++i) acc[j][i] = mx_mfma32<S>(now.w[j], now.x[i], acc[j][i], sc.w[j], sc.x[i]);
+      for (int i = 0; i < MF; ++i) acc[j][i] = mx_mfma32<B>(now.w[j], now.x[i], acc[j][i], sc.w[j], sc.x[i]);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  constexpr std::integral_constant<int, 0> b0{};
-  constexpr std::integral_constant<int, 1> b1{};
-  constexpr std::integral_constant<int, 2> b2{};
-  constexpr std::integral_constant<int, 3> b3{};
-  Operands p, q;
-  Scales sa, sb;                                               // of two stages
-  load(0, stage0);
-  load_scales(0);                                              // there are sixteen at least
-  put_scales(0);
-  __builtin_amdgcn_s_waitcnt(0x0F70);                          // vmcnt(0)
-  __syncthreads();
-  read_scales(sa, 0);                                          // before loads into LDS are on their way: the compiler has it wait for them
-  read_scales(sb, 1);
-  load(1, stage1);
-#pragma unroll
-  for (int f = 0; f < NF; ++f) read(p, stage0, 0, f);
-  const auto two_stages = [&](auto last, int chunk) {
-    constexpr bool LAST = decltype(last)::value;
-    const int t = chunk * 2;
-    if (!LAST) load_scales(chunk + 1);
-    step(b0, std::true_type{}, sa, p, q, stage0, 1);
-    step(b1, std::true_type{}, sa, q, p, stage0, 2);
-    step(b2, std::true_type{}, sa, p, q, stage0, 3);
-    __builtin_amdgcn_s_waitcnt(0x0F70);
-    __syncthreads();                                           // the next stage is there, this one has been read
-    if (!LAST) load(t + 2, stage0);
-    step(b3, std::true_type{}, sa, q, p, stage1, 0);
-    if (!LAST) put_scales(chunk + 1);
-    step(b0, std::true_type{}, sb, p, q, stage1, 1);
-    step(b1, std::true_type{}, sb, q, p, stage1, 2);
-    step(b2, std::true_type{}, sb, p, q, stage1, 3);
-    __builtin_amdgcn_s_waitcnt(0x0F70);
-    __syncthreads();
-    const Scales now = sb;
-    if (!LAST) {
-      read_scales(sa, t + 2);
-      read_scales(sb, t + 3);
-      load(t + 3, stage1);
-    }
-    step(b3, std::bool_constant<!LAST>{}, now, q, p, stage0, 0);
+  // Waits for a stage, of which `behind` loads may still be on their way, and for all waves to have read what they asked for.  vmcnt counts loads in
+  // their order; at least so many have to have been issued behind the stage's own.
+  const auto turn = [&](auto behind) {
+    constexpr int N = decltype(behind)::value;
+    static_assert(N < 64);
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 0x70);   // vmcnt(N) lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
   };
-  const int chunks = (stages + 1) / 2;
-  for (int chunk = 0; chunk < chunks - 1; ++chunk) two_stages(std::false_type{}, chunk);
-  if (a.blocks % 16) {                                         // the last scales, zeros past the end; out of the loop, as products would be moved past a branch
+  Operands p, q;
+  load(0, room0);                                              // what is waited for first, first
+  const auto first_scales = [&](auto get) {
+    const auto of = [&](int row, uint32_t &even, uint32_t &odd) {
+      const uint4m v = get(scale_row(row));
+      even = g ? v[1] : v[0];
+      odd = g ? v[3] : v[2];
+    };
 #pragma unroll
-    for (int i = 0; i < SR; ++i) next_scales[i] = mx_scales16(scale_rows[i], chunks - 1, a.blocks);
-    __syncthreads();                                           // those that are there have been read
-    put_scales(chunks - 1);
-    __syncthreads();
-    read_scales(sa, chunks * 2 - 2);
-    read_scales(sb, chunks * 2 - 1);
+    for (int f = 0; f < MF; ++f) of(wm + f * 32 + r, sa.x[f], sb.x[f]);
+#pragma unroll
+    for (int f = 0; f < NF; ++f) of(BM + wn + f * 32 + r, sa.w[f], sb.w[f]);
+  };
+  if (chunk0 * 16 + 16 <= a.blocks)
+    first_scales([&](const uint8_t *row) { return *(const uint4m_any *)(row + chunk0 * 16); });
+  else
+    first_scales([&](const uint8_t *row) { return mx_scales16(row, chunk0, a.blocks); });
+  load_scales(chunk0 + 1);
+  __builtin_amdgcn_sched_barrier(0);
+  four_times([&](auto u) {
+    if constexpr (decltype(u)::value > 0 && decltype(u)::value < S) load(decltype(u)::value, room(u));
+  });
+  turn(std::integral_constant<int, (S - 1) * L>{});
+#pragma unroll
+  for (int f = 0; f < NF; ++f) read(p, room0, 0, f);
+  // A stage; MORE: with the loads of the one S behind it; NEXT: there is a next one.  Behind that one's loads come those of S - 2 stages.
+  constexpr std::integral_constant<int, (S - 2) * L> others{};
+  const auto stage = [&](auto u, auto behind, auto more, auto next, int t) {
+    constexpr int U = decltype(u)::value;
+    constexpr bool MORE = decltype(more)::value, NEXT = decltype(next)::value;
+    uint8_t *const here = room(u), *const there = room(std::integral_constant<int, U + 1>{});
+    constexpr std::integral_constant<int, 0> b0{};
+    constexpr std::integral_constant<int, 1> b1{};
+    constexpr std::integral_constant<int, 2> b2{};
+    constexpr std::integral_constant<int, 3> b3{};
+    const Scales now = U % 2 ? sb : sa;
+    step(b0, std::true_type{}, now, p, q, here, 1);
+    if constexpr (NEXT && U % 2 == 1) put_scales(chunk0 + t / 2 + 1, here);
+    __builtin_amdgcn_sched_barrier(0);
+    step(b1, std::true_type{}, now, q, p, here, 2);
+    step(b2, std::true_type{}, now, p, q, here, 3);
+    if constexpr (NEXT) {
+      turn(behind);
+      if constexpr (U % 2 == 1) {
+        read_scales(here);
+        if constexpr (MORE) load_scales(chunk0 + t / 2 + 2);   // before the data: what is in registers has come when the data before it have
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (MORE) load(t + S, here);
+    }
+    step(b3, next, now, q, p, there, 0);
+  };
+  constexpr std::integral_constant<int, 0> u0{};
+  constexpr std::integral_constant<int, 1> u1{};
+  constexpr std::integral_constant<int, 2> u2{};
+  constexpr std::integral_constant<int, 3> u3{};
+  constexpr std::true_type yes{};
+  constexpr std::false_type no{};
+  // No way out of a loop in between: the compiler would have it wait for loads on that way.
+  int t = 0;
+  if constexpr (S == 2) {                                      // in pairs; behind the last stage come scales of 0
+    for (; t + 2 < stages; t += 2) {
+      stage(u0, others, yes, yes, t);
+      stage(u1, others, yes, yes, t + 1);
+    }
+    stage(u0, others, no, yes, t);
+    stage(u1, others, no, no, t + 1);
+  } else {                                                     // one to three are left, of four that have been asked for (those that there are not: zeros)
+    for (; t + 4 <= stages; t += 4) {
+      stage(u0, others, yes, yes, t);
+      stage(u1, others, yes, yes, t + 1);
+      stage(u2, others, yes, yes, t + 2);
+      stage(u3, others, yes, yes, t + 3);
+    }
+    if (t < stages) stage(u0, std::integral_constant<int, 2 * L>{}, no, yes, t);
+    if (t + 1 < stages) stage(u1, std::integral_constant<int, L>{}, no, yes, t + 1);
+    if (t + 2 < stages) stage(u2, std::integral_constant<int, 0>{}, no, yes, t + 2);
   }
-  two_stages(std::true_type{}, chunks - 1);
+  turn(std::integral_constant<int, 0>{});                      // nothing is on its way to LDS any more
+  if (a.splits > 1) {
+    // Splits meet in memory, past the caches that a device's XCDs have of their own, as their lanes have them; the last of a tile's to end adds them
+    // in their order
+    constexpr int PARTS = NF * MF * 8;                         // pairs of a lane
+    const int64_t between = (int64_t)PARTS * THREADS;
+    uint64_t *part = (uint64_t *)a.part + (int64_t)tile * a.splits * between + threadIdx.x;
+#pragma unroll
+    for (int j = 0; j < NF; ++j)
+#pragma unroll
+      for (int i = 0; i < MF; ++i)
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          __hip_atomic_store(part + split * between + ((j * MF + i) * 8 + k) * THREADS,
+                             __builtin_bit_cast(uint64_t, (float2m){acc[j][i][2 * k], acc[j][i][2 * k + 1]}), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __shared__ int last;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      const int before = __hip_atomic_fetch_add(a.counters + tile, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      last = before == a.splits - 1;
+      if (last) __hip_atomic_store(a.counters + tile, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // for the next call
+    }
+    __syncthreads();
+    if (!last) return;
+#pragma unroll
+    for (int j = 0; j < NF; ++j)
+#pragma unroll
+      for (int i = 0; i < MF; ++i) acc[j][i] = (float16m){};
+    for (int p = 0; p < a.splits; ++p)
+#pragma unroll
+      for (int j = 0; j < NF; ++j)
+#pragma unroll
+        for (int i = 0; i < MF; ++i)
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const float2m v = __builtin_bit_cast(float2m, __hip_atomic_load(part + p * between + ((j * MF + i) * 8 + k) * THREADS, __ATOMIC_RELAXED,
+                                                                            __HIP_MEMORY_SCOPE_AGENT));
+            acc[j][i][2 * k] += v[0];
+            acc[j][i][2 * k + 1] += v[1];
+          }
+  }
   // Results go through LDS, a wave's by itself, 32 rows at a time: then a lane has four neighbours of a row, the same ones of every row, and FOURS lanes
-  // have a row of the wave's.  Four numbers c of row m lie in place c ^ m % 16.  All loads into LDS have been waited for, and all waves have read the last
-  // stage.
+  // have a row of the wave's.  Four numbers c of row m lie in place c ^ key(m).
   constexpr int FOURS = NF * 8, PASS = 64 / FOURS, PASSES = 32 / PASS;
   static_assert(WAVES * 32 * FOURS * 16 <= ROWS * 128);
-  float4m *mine = (float4m *)stage0 + wave * 32 * FOURS;
+  float4m *mine = (float4m *)room0 + wave * 32 * FOURS;
+  const auto key = [](int row) { return FOURS == 8 ? row >> 1 & 7 : row & (FOURS < 16 ? FOURS - 1 : 15); };   // sixteen rows in all banks
   const int four = lane % FOURS, row0 = lane / FOURS, n = n0 + wn + 4 * four;
   const float4m bias = a.bias && n + 4 <= a.cols ? mx_load4(a.bias, n, TPUHIP_F32) : (float4m){0, 0, 0, 0};
   const auto results = [&](auto type) {
@@ -318,13 +506,13 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxProductArgs a) 
       for (int j = 0; j < NF; ++j)
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          mine[r * FOURS + ((j * 8 + 2 * k + g) ^ (r & 15))] = (float4m){acc[j][i][4 * k], acc[j][i][4 * k + 1], acc[j][i][4 * k + 2], acc[j][i][4 * k + 3]};
+          mine[r * FOURS + ((j * 8 + 2 * k + g) ^ key(r))] = (float4m){acc[j][i][4 * k], acc[j][i][4 * k + 1], acc[j][i][4 * k + 2], acc[j][i][4 * k + 3]};
       __builtin_amdgcn_wave_barrier();
       float4m v[PASSES];
 #pragma unroll
       for (int k = 0; k < PASSES; ++k) {
         const int row = k * PASS + row0;
-        v[k] = mine[row * FOURS + (four ^ (row & 15))];
+        v[k] = mine[row * FOURS + (four ^ key(row))];
       }
       __builtin_amdgcn_wave_barrier();
       const int first = m0 + wm + i * 32 + row0;
@@ -337,7 +525,7 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxProductArgs a) 
             if (first + k * PASS < a.rows) v[k] += mx_load4(a.residual, (int64_t)(first + k * PASS) * a.residual_stride + n, TYPE);
 #pragma unroll
         for (int k = 0; k < PASSES; ++k)
-          if (first + k * PASS < a.rows) mx_store4(a.y, (int64_t)(first + k * PASS) * a.y_stride + n, TYPE, v[k]);
+          if (first + k * PASS < a.rows) mx_store4<(BM >= 256)>(a.y, (int64_t)(first + k * PASS) * a.y_stride + n, TYPE, v[k]);
       } else if (n < a.cols) {
 #pragma unroll
         for (int k = 0; k < PASSES; ++k)
@@ -364,8 +552,9 @@ static int mx_product_args(tpuhip_ctx *ctx, const tpuhip_mx_product_desc *d, con
   if (d->residual)
     if (int rc = mx_check_rows(x->rows, w->rows, d->residual, d->dtype, d->residual_stride, false, "the residual", what)) return rc;
   TPUHIP_REQUIRE((uintptr_t)d->bias % 4 == 0, "%s: the bias does not begin at an element", what);
-  // a launch has fewer than 2^32 threads by the columns, and 65535 workgroups by the rows
-  TPUHIP_REQUIRE(x->rows <= 16 * 65535 && w->rows <= 1 << 26, "%s: %d rows of %d columns in one call", what, x->rows, w->rows);
+  TPUHIP_REQUIRE(x->rows <= 1 << 30 && w->rows <= 1 << 30, "%s: %d rows, %d columns", what, x->rows, w->rows);
+  for (const tpuhip_mx_matrix *m : {x, w})                     // a tile's rows are reached by 32 bits
+    TPUHIP_REQUIRE(m->rows == 1 || m->codes_stride < 1 << 24, "%s: rows of codes lie %lld bytes apart", what, (long long)m->codes_stride);
   *a = MxProductArgs{};
   a->x = (const uint8_t *)x->codes;
   a->xs = (const uint8_t *)x->scales;
@@ -387,23 +576,95 @@ static int mx_product_args(tpuhip_ctx *ctx, const tpuhip_mx_product_desc *d, con
   return TPUHIP_OK;
 }
 
-template <int BM, int BN, int WM, int WN>
-static void mx_launch_tiles(tpuhip_ctx *ctx, const MxProductArgs &a) {
-  launch(ctx, mx_tile_kernel<BM, BN, WM, WN>, dim3((unsigned)(ceil_div64(a.rows, BM) * ceil_div64(a.cols, BN))), dim3(64 * WM * WN), a);
+// Workgroups whose tiles are too few for the device share the sums of each
+// Forms of the tile kernel, and what a call takes in each, in microseconds: some for the first loads and the results, some a stage with a workgroup on
+// each CU; a CU has room for `at_once` of them.  Sums of 4096 numbers, 16 stages, as measured and as worked out here:
+//   x 64 .. 777 rows, w 4096:       32 x 64   7.0  9.5 (256 rows) 30 | 7.0 10.5 25     64 x 64  7.8  8.6 12.8 23 | 8.6  8.6 13 19
+//                                  64 x 128   9.4 10.3 11.8 20       | 11 11 11 22   128 x 128 12.2 13.0 13.6 15.5 | 13 13 13 13
+//   x 512 and 777 rows, w 16384:   128 x 128, two at once 27 45 | 27 43                256 x 256  34 40 | 37 37
+struct MxForm {
+  int rows, cols, at_once;
+  float base, stage;
+};
+constexpr MxForm kMxForms[] = {{32, 64, 4, 3.5f, 0.22f},   {64, 64, 2, 3.8f, 0.30f},   {64, 128, 1, 4.1f, 0.42f},
+                               {128, 128, 1, 5.2f, 0.50f}, {128, 128, 2, 5.0f, 0.70f}, {256, 256, 1, 9.0f, 1.75f}};
+constexpr int kMxFormCount = sizeof(kMxForms) / sizeof(kMxForms[0]);
+
+struct MxChoice {
+  int form, splits;
+};
+// Sums in parts cost their joining, 2.0 to 2.5 us for two and 4.5 for four: x 64, w 4096 rows of 16384 numbers take 64 x 64 tiles 19.9, 14.6 or 12.7 us
+// in 1, 2 or 4 parts, of 4096 numbers 7.8, 8.3 or 9.0.
+static MxChoice mx_choose(int64_t rows, int64_t cols, int blocks, int num_cu) {
+  MxChoice best = {0, 1};
+  float least = 0;
+  const int stages = (blocks + kMxStage - 1) / kMxStage;
+  for (int f = 0; f < kMxFormCount; ++f) {
+    const MxForm &form = kMxForms[f];
+    const int64_t tiles = ceil_div64(rows, form.rows) * ceil_div64(cols, form.cols);
+    for (int splits = 1; splits <= 8 && (splits == 1 || (tiles * splits <= num_cu && splits * 2 <= stages)); splits *= 2) {
+      const float turns = form.at_once == 1 ? (float)ceil_div64(tiles * splits, num_cu) : std::max(1.0f, (float)tiles * splits / num_cu);
+      const float part = form.stage * ((stages + splits - 1) / splits);
+      const float cost = (form.at_once == 1 ? (form.base + part) * turns : form.base + part * turns) + (splits > 1 ? 1.2f + 0.8f * splits : 0.0f);
+      if ((f == 0 && splits == 1) || cost < least) {
+        least = cost;
+        best = {f, splits};
+      }
+    }
+  }
+  return best;
 }
 
-static int mx_multiply(tpuhip_ctx *ctx, const MxProductArgs &a) {
-  if (a.rows > 128 && a.blocks >= 16) {
-    if (ceil_div64(a.rows, 256) * ceil_div64(a.cols, 256) >= ctx->num_cu / 2)
-      mx_launch_tiles<256, 256, 2, 4>(ctx, a);
-    else
-      mx_launch_tiles<128, 128, 2, 2>(ctx, a);
-    TPUHIP_CHECK_HIP(hipGetLastError());
-    return TPUHIP_OK;
+// Workgroups whose tiles are too few for the device share the sums of each
+template <int BM, int BN, int WM, int WN, int S>
+static int mx_launch_tiles(tpuhip_ctx *ctx, MxProductArgs a, int splits) {
+  const int64_t tiles = ceil_div64(a.rows, BM) * ceil_div64(a.cols, BN);
+  TPUHIP_REQUIRE(tiles <= UINT32_MAX / (64 * WM * WN), "a product of %d rows and %d columns in one call", a.rows, a.cols);   // a launch has fewer than 2^32 threads
+  const int chunks = (a.blocks + 15) / 16;
+  if (splits > 1 && (tiles > kCounters || tiles * splits * BM * BN * 4 > (int64_t)kJoinBytes)) splits = 1;
+  if (splits > 1) {
+    if (int rc = attention_workspace(ctx)) return rc;
+    if (!ctx->join) splits = 1;
   }
-  launch(ctx, mx_stream_kernel<1, 1, 8>, dim3((unsigned)ceil_div64(a.cols, 16), (unsigned)ceil_div64(a.rows, 16)), dim3(512), a);
+  a.split_chunks = (int)ceil_div64(chunks, splits);
+  a.splits = (int)ceil_div64(chunks, a.split_chunks);
+  a.counters = (int *)ctx->join;
+  a.part = (float *)((char *)ctx->join + kCounters * 4);
+  launch(ctx, mx_tile_kernel<BM, BN, WM, WN, S>, dim3((unsigned)(tiles * a.splits)), dim3(64 * WM * WN), a);
   TPUHIP_CHECK_HIP(hipGetLastError());
   return TPUHIP_OK;
+}
+
+static int64_t mx_chunks(const MxProductArgs &a) { return (a.blocks + 15) / 16; }
+
+// Rows of x that a workgroup quantises or copies for itself, 512 numbers of a row at a time: from some number of those on, quantising x in a launch
+// of its own and the tile kernel are quicker.  x, w of 4096 x 4096, float16: 1 row 4.8 and 9.3 us, 4 rows 6.5 and 9.3, 16 rows 12.4 and 9.3.
+static bool mx_streams(const MxProductArgs &a) { return a.rows <= kMxFew && a.rows * mx_chunks(a) <= kMxFewPieces; }
+
+// Up to two workgroups a CU, each of which goes from columns to columns: of 16384 columns one row takes 9.1 us so, 10.0 with four a CU.  Eight waves
+// where sums are long (16384 numbers: 10.7 us, with four 12.3) or columns many (65536: 26.6 and 30.1), otherwise four (4096 x 4096: 4.7 us, with eight 5.0).
+template <int WAVES>
+static int mx_launch_stream(tpuhip_ctx *ctx, const MxProductArgs &a, int type) {
+  const int64_t tiles = ceil_div64(a.cols, 16), turns = ceil_div64(tiles, 2 * ctx->num_cu);
+  const auto kernel = type == kMxCodes ? mx_stream_kernel<WAVES, kMxCodes> : type == TPUHIP_BF16 ? mx_stream_kernel<WAVES, TPUHIP_BF16>
+                      : type == TPUHIP_F16 ? mx_stream_kernel<WAVES, TPUHIP_F16> : mx_stream_kernel<WAVES, TPUHIP_F32>;
+  launch(ctx, kernel, dim3((unsigned)ceil_div64(tiles, turns)), dim3(64 * WAVES), a);
+  TPUHIP_CHECK_HIP(hipGetLastError());
+  return TPUHIP_OK;
+}
+
+// type: of x's elements where mx_streams(), or kMxCodes: x is a matrix
+static int mx_multiply(tpuhip_ctx *ctx, const MxProductArgs &a, int type) {
+  if (mx_streams(a)) return mx_chunks(a) > 8 || a.cols > 128 * ctx->num_cu ? mx_launch_stream<8>(ctx, a, type) : mx_launch_stream<4>(ctx, a, type);
+  const MxChoice c = mx_choose(a.rows, a.cols, a.blocks, ctx->num_cu);
+  switch (c.form) {
+    case 0: return mx_launch_tiles<32, 64, 1, 2, 4>(ctx, a, c.splits);
+    case 1: return mx_launch_tiles<64, 64, 2, 2, 4>(ctx, a, c.splits);
+    case 2: return mx_launch_tiles<64, 128, 1, 4, 4>(ctx, a, c.splits);
+    case 3: return mx_launch_tiles<128, 128, 2, 2, 4>(ctx, a, c.splits);
+    case 4: return mx_launch_tiles<128, 128, 2, 2, 2>(ctx, a, c.splits);
+    default: return mx_launch_tiles<256, 256, 2, 4, 2>(ctx, a, c.splits);
+  }
 }
 
 }  // namespace tpuhip
@@ -417,7 +678,7 @@ int tpuhip_mx_product(tpuhip_ctx *ctx, const tpuhip_mx_product_desc *desc, const
   if (int rc = mx_product_args(ctx, desc, x, w, y, "tpuhip_mx_product", &a)) return rc;
   if (a.rows == 0) return TPUHIP_OK;
   TPUHIP_CHECK_HIP(hipSetDevice(ctx->device));
-  return mx_multiply(ctx, a);
+  return mx_multiply(ctx, a, kMxCodes);
 }
 
 int tpuhip_mx_linear(tpuhip_ctx *ctx, const tpuhip_mx_product_desc *desc, const void *x, int x_dtype, int64_t x_stride,
@@ -428,8 +689,14 @@ int tpuhip_mx_linear(tpuhip_ctx *ctx, const tpuhip_mx_product_desc *desc, const 
   if (int rc = mx_check_rows(a.rows, room->cols, x, x_dtype, x_stride, false, "x", what)) return rc;
   if (a.rows == 0) return TPUHIP_OK;
   TPUHIP_CHECK_HIP(hipSetDevice(ctx->device));
+  if (mx_streams(a)) {                                         // quantised on the way
+    a.x = (const uint8_t *)x;
+    a.x_stride = x_stride;
+    a.depth = room->cols;
+    return mx_multiply(ctx, a, x_dtype);
+  }
   if (int rc = mx_quantize(ctx, room, x, x_dtype, x_stride, what)) return rc;
-  return mx_multiply(ctx, a);
+  return mx_multiply(ctx, a, kMxCodes);
 }
 
 }  // extern "C"

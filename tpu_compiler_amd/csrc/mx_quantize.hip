@@ -15,11 +15,6 @@ struct MxRowsArgs {
 // Four threads a block, eight numbers each.
 constexpr int kMxThreads = 256, kMxThreadsBlock = 4;
 
-template <int CTRL>
-__device__ __forceinline__ float dpp_max(float v) {
-  return __builtin_elementwise_maximum(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true)));
-}
-
 __global__ __launch_bounds__(kMxThreads) void mx_quantize_kernel(MxRowsArgs a) {
   const uint32_t at = blockIdx.x * (kMxThreads / kMxThreadsBlock) + threadIdx.x / kMxThreadsBlock, t = threadIdx.x % kMxThreadsBlock;
   if (at >= a.blocks) return;                                  // the four threads of a block together
@@ -33,13 +28,8 @@ __global__ __launch_bounds__(kMxThreads) void mx_quantize_kernel(MxRowsArgs a) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = col + i < a.cols ? mx_load(a.x, row * a.x_stride + col + i, a.dtype) : 0.0f;
   }
-  float top = 0;                                               // a NaN stays
-#pragma unroll
-  for (int i = 0; i < 8; ++i) top = __builtin_elementwise_maximum(top, __builtin_fabsf(v[i]));
-  top = dpp_max<0x4E>(dpp_max<0xB1>(top));
-  const uint32_t byte = mx_scale_byte(top), none = byte == 255;
-  const uint32_t c = mx_codes8(v, mx_scale(none ? 127 : byte));
-  *(uint32_t *)(a.codes + row * a.codes_stride + (int64_t)block * kMxBytes + t * 4) = none ? 0 : c;
+  uint32_t byte;
+  *(uint32_t *)(a.codes + row * a.codes_stride + (int64_t)block * kMxBytes + t * 4) = mx_quantised8(v, byte);
   if (t == 0) a.scales[row * a.scales_stride + block] = (uint8_t)byte;
 }
 
