@@ -18,7 +18,7 @@ struct KvPagesArgs {
   int n_seq, pages, capacity;
 };
 
-constexpr int kPagesMost = 64;   // workgroups of a launch
+constexpr int kPagesMost = 128;   // workgroups of a launch
 
 // Sums over a workgroup's threads, of those up to and with each one.  They stop at 2^32 - 1, which no number they are compared with reaches.
 template <int CTRL, int ROWS>
@@ -130,8 +130,12 @@ __global__ __launch_bounds__(THREADS) void kv_grow_kernel(KvPagesArgs a) {
     pages += all[0];
     refused += all[2];
   };
+  int more = 0, new_len = 0;                                   // of this thread's sequence, where there is one
   for (int base = 0; base < a.n_seq; base += THREADS)
-    sequences(base, [&](int, bool, int len, int have, int got, uint32_t got_pages, uint32_t page_end, uint32_t token_end, uint32_t new_pages, uint32_t new_tokens) {
+    sequences(base, [&](int i, bool there, int len, int have, int got, uint32_t got_pages, uint32_t page_end, uint32_t token_end, uint32_t new_pages, uint32_t new_tokens) {
+      more = there ? got : 0;
+      new_len = len + got;
+      if (blockIdx.x == 0 && there) a.q_starts[i + 1] = (int)(tokens + token_end);
       page_starts[t] = page_end - got_pages;
       token_starts[t] = token_end - (uint32_t)got;
       first_pages[t] = have;
@@ -154,21 +158,23 @@ __global__ __launch_bounds__(THREADS) void kv_grow_kernel(KvPagesArgs a) {
       if (base + THREADS < a.n_seq) __syncthreads();           // the starts are written again
     });
   for (int64_t k = (int64_t)tokens + first; k < a.capacity; k += step) a.slots[k] = -1;
-  const uint32_t taken = pages, none = refused;
+  if (blockIdx.x == 0 && t == 0) {
+    a.q_starts[0] = 0;
+    if (a.refused) a.refused[0] = (int)refused;
+  }
+  const uint32_t taken = pages;
   if (!last_of(a)) return;
-  wanted_pages = wanted_tokens = tokens = pages = 0;
+  if (t == 0) a.n_free[0] = n_free - (int)taken;
+  if (a.n_seq <= THREADS) {
+    if (more) a.lens[t] = new_len;
+    return;
+  }
+  wanted_pages = wanted_tokens = tokens = pages = 0;           // once more, what each of them got
   for (int base = 0; base < a.n_seq; base += THREADS) {
     __syncthreads();
-    sequences(base, [&](int i, bool there, int len, int, int got, uint32_t, uint32_t, uint32_t token_end, uint32_t, uint32_t) {
-      if (!there) return;
-      a.q_starts[i + 1] = (int)(tokens + token_end);
-      if (got) a.lens[i] = len + got;
+    sequences(base, [&](int i, bool there, int len, int, int got, uint32_t, uint32_t, uint32_t, uint32_t, uint32_t) {
+      if (there && got) a.lens[i] = len + got;
     });
-  }
-  if (t == 0) {
-    a.q_starts[0] = 0;
-    a.n_free[0] = n_free - (int)taken;
-    if (a.refused) a.refused[0] = (int)none;
   }
 }
 
@@ -240,7 +246,7 @@ static int launch_pages(tpuhip_ctx *ctx, KvPagesArgs &a, int64_t items, int shar
     a.counter = (int *)ctx->join;
     if (!a.counter) works = 1;
   }
-  if (works == 1 && a.n_seq <= 256 && items <= share / 4)
+  if (works == 1 && a.n_seq <= 256 && items <= 1024)
     launch(ctx, kernel_of(std::integral_constant<int, 256>{}), dim3(1), dim3(256), a);
   else
     launch(ctx, kernel_of(std::integral_constant<int, 1024>{}), dim3((unsigned)works), dim3(1024), a);
@@ -298,7 +304,7 @@ int tpuhip_kv_pages_grow(tpuhip_ctx *ctx, const tpuhip_kv_pages *pages, const in
   a.q_starts = q_starts;
   a.slots = slots;
   a.refused = refused;
-  return launch_pages(ctx, a, capacity, 4096, [](auto threads) { return kv_grow_kernel<decltype(threads)::value>; });
+  return launch_pages(ctx, a, capacity, 2048, [](auto threads) { return kv_grow_kernel<decltype(threads)::value>; });
 }
 
 int tpuhip_kv_pages_trim(tpuhip_ctx *ctx, const tpuhip_kv_pages *pages, const int32_t *keep) {

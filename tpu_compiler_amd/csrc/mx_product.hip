@@ -79,22 +79,29 @@ __device__ __forceinline__ uint32_t mx_picked(uint4m v, int g) {
 }
 __device__ __forceinline__ uint32_t mx_scales(const uint8_t *row, int chunk, int blocks, int g) { return mx_picked(mx_scales16(row, chunk, blocks), g); }
 
+// Four neighbours' biases or residuals.  Past the end the last one again: loads without branches, which do not wait for each other.
+__device__ __forceinline__ float4m mx_four(const void *x, int64_t row, int n, int cols, int dtype) {
+  if (n + 4 <= cols) return mx_load4(x, row + n, dtype);
+  float4m v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = mx_load(x, row + min(n + i, cols - 1), dtype);
+  return v;
+}
+template <bool ONCE = false>
+__device__ __forceinline__ void mx_put_four(void *y, int64_t row, int n, int cols, int dtype, float4m v) {
+  if (n + 4 <= cols) {
+    mx_store4<ONCE>(y, row + n, dtype, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (n + i < cols) mx_store(y, row + n + i, dtype, v[i]);
+  }
+}
 // four neighbours of a row of y
 __device__ __forceinline__ void mx_result(const MxProductArgs &a, int m, int n, float4m v) {
-  const int64_t from = (int64_t)m * a.residual_stride + n, to = (int64_t)m * a.y_stride + n;
-  if (n + 4 <= a.cols) {
-    if (a.bias) v += mx_load4(a.bias, n, TPUHIP_F32);
-    if (a.residual) v += mx_load4(a.residual, from, a.dtype);
-    mx_store4(a.y, to, a.dtype, v);
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (n + i >= a.cols) return;
-    if (a.bias) v[i] += a.bias[n + i];
-    if (a.residual) v[i] += mx_load(a.residual, from + i, a.dtype);
-    mx_store(a.y, to + i, a.dtype, v[i]);
-  }
+  if (a.bias) v += mx_four(a.bias, 0, n, a.cols, TPUHIP_F32);
+  if (a.residual) v += mx_four(a.residual, (int64_t)m * a.residual_stride, n, a.cols, a.dtype);
+  mx_put_four(a.y, (int64_t)m * a.y_stride, n, a.cols, a.dtype, v);
 }
 
 // A few rows of x, 16 at most: they lie in LDS as codes while a workgroup goes from 16 columns of y (rows of w) to the next.  Its waves take every
@@ -251,12 +258,12 @@ __device__ __forceinline__ void mx_to_lds(__amdgpu_buffer_rsrc_t buffer, uint8_t
 }
 
 template <int BM, int BN, int WM, int WN, int S>
-__global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxProductArgs a) {
+__global__ __launch_bounds__(64 * WM * WN, S == 2 ? 2 : 1) void mx_tile_kernel(MxProductArgs a) {
   constexpr int WAVES = WM * WN, THREADS = 64 * WAVES, ROWS = BM + BN;
   constexpr int MF = BM / WM / 32, NF = BN / WN / 32, L = ROWS / 8 / WAVES;  // fragments of a wave; pieces of 8 rows that it brings
   constexpr int SR = (ROWS + THREADS - 1) / THREADS;                         // rows whose scales a thread brings
   constexpr int SCALES = ROWS * 128, SIZE = SCALES + ROWS * 16;              // where they lie, and a stage's room
-  static_assert(BM % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0 && WAVES % 2 == 0 && (S == 2 || S == 4));
+  static_assert(BM % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0 && WAVES % 2 == 0 && (S == 2 || (S == 4 && BM < 256)));
   __shared__ __attribute__((aligned(128))) uint8_t room0[SIZE];
   __shared__ __attribute__((aligned(128))) uint8_t room1[SIZE];
   __shared__ __attribute__((aligned(128))) uint8_t room2[S > 2 ? SIZE : 16];
@@ -436,7 +443,7 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxProductArgs a) 
       stage(u1, others, yes, yes, t + 1);
     }
     stage(u0, others, no, yes, t);
-    stage(u1, others, no, no, t + 1);
+    if (BM >= 256 || t + 1 < stages) stage(u1, others, no, no, t + 1);   // of the largest tiles always: a way around it costs them registers
   } else {                                                     // one to three are left, of four that have been asked for (those that there are not: zeros)
     for (; t + 4 <= stages; t += 4) {
       stage(u0, others, yes, yes, t);
@@ -477,18 +484,30 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxProductArgs a) 
     for (int j = 0; j < NF; ++j)
 #pragma unroll
       for (int i = 0; i < MF; ++i) acc[j][i] = (float16m){};
-    for (int p = 0; p < a.splits; ++p)
+    constexpr int AT_ONCE = NF * MF == 1 ? 4 : NF * MF <= 2 ? 2 : 1;   // splits whose sums are on their way together (one by one: 4.5 us for four of 64 x 64)
+    for (int p0 = 0; p0 < a.splits; p0 += AT_ONCE) {
+      float2m v[AT_ONCE][NF][MF][8];
 #pragma unroll
-      for (int j = 0; j < NF; ++j)
+      for (int p = 0; p < AT_ONCE; ++p)
 #pragma unroll
-        for (int i = 0; i < MF; ++i)
+        for (int j = 0; j < NF; ++j)
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const float2m v = __builtin_bit_cast(float2m, __hip_atomic_load(part + p * between + ((j * MF + i) * 8 + k) * THREADS, __ATOMIC_RELAXED,
-                                                                            __HIP_MEMORY_SCOPE_AGENT));
-            acc[j][i][2 * k] += v[0];
-            acc[j][i][2 * k + 1] += v[1];
-          }
+          for (int i = 0; i < MF; ++i)
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              v[p][j][i][k] = __builtin_bit_cast(float2m, __hip_atomic_load(part + min(p0 + p, a.splits - 1) * between + ((j * MF + i) * 8 + k) * THREADS,
+                                                                            __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+#pragma unroll
+      for (int p = 0; p < AT_ONCE; ++p)
+#pragma unroll
+        for (int j = 0; j < NF; ++j)
+#pragma unroll
+          for (int i = 0; i < MF; ++i)
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) acc[j][i][2 * k + h] += p0 + p < a.splits ? v[p][j][i][k][h] : 0.0f;
+    }
   }
   // Results go through LDS, a wave's by itself, 32 rows at a time: then a lane has four neighbours of a row, the same ones of every row, and FOURS lanes
   // have a row of the wave's.  Four numbers c of row m lie in place c ^ key(m).
@@ -497,7 +516,7 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxProductArgs a) 
   float4m *mine = (float4m *)room0 + wave * 32 * FOURS;
   const auto key = [](int row) { return FOURS == 8 ? row >> 1 & 7 : row & (FOURS < 16 ? FOURS - 1 : 15); };   // sixteen rows in all banks
   const int four = lane % FOURS, row0 = lane / FOURS, n = n0 + wn + 4 * four;
-  const float4m bias = a.bias && n + 4 <= a.cols ? mx_load4(a.bias, n, TPUHIP_F32) : (float4m){0, 0, 0, 0};
+  const float4m bias = a.bias ? mx_four(a.bias, 0, min(n, a.cols - 1), a.cols, TPUHIP_F32) : (float4m){0, 0, 0, 0};
   const auto results = [&](auto type) {
     constexpr int TYPE = decltype(type)::value;
 #pragma unroll
@@ -516,21 +535,19 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_tile_kernel(MxProductArgs a) 
       }
       __builtin_amdgcn_wave_barrier();
       const int first = m0 + wm + i * 32 + row0;
-      if (n + 4 <= a.cols) {
+      if (n >= a.cols) continue;
 #pragma unroll
-        for (int k = 0; k < PASSES; ++k) v[k] += bias;
-        if (a.residual)
+      for (int k = 0; k < PASSES; ++k) v[k] += bias;
+      if (a.residual) {
+        float4m more[PASSES];
 #pragma unroll
-          for (int k = 0; k < PASSES; ++k)
-            if (first + k * PASS < a.rows) v[k] += mx_load4(a.residual, (int64_t)(first + k * PASS) * a.residual_stride + n, TYPE);
+        for (int k = 0; k < PASSES; ++k) more[k] = mx_four(a.residual, (int64_t)min(first + k * PASS, a.rows - 1) * a.residual_stride, n, a.cols, TYPE);
 #pragma unroll
-        for (int k = 0; k < PASSES; ++k)
-          if (first + k * PASS < a.rows) mx_store4<(BM >= 256)>(a.y, (int64_t)(first + k * PASS) * a.y_stride + n, TYPE, v[k]);
-      } else if (n < a.cols) {
-#pragma unroll
-        for (int k = 0; k < PASSES; ++k)
-          if (first + k * PASS < a.rows) mx_result(a, first + k * PASS, n, v[k]);
+        for (int k = 0; k < PASSES; ++k) v[k] += more[k];
       }
+#pragma unroll
+      for (int k = 0; k < PASSES; ++k)
+        if (first + k * PASS < a.rows) mx_put_four<(BM >= 256)>(a.y, (int64_t)(first + k * PASS) * a.y_stride, n, a.cols, TYPE, v[k]);
     }
   };
   if (a.dtype == TPUHIP_BF16)
@@ -576,36 +593,41 @@ static int mx_product_args(tpuhip_ctx *ctx, const tpuhip_mx_product_desc *d, con
   return TPUHIP_OK;
 }
 
-// Workgroups whose tiles are too few for the device share the sums of each
-// Forms of the tile kernel, and what a call takes in each, in microseconds: some for the first loads and the results, some a stage with a workgroup on
-// each CU; a CU has room for `at_once` of them.  Sums of 4096 numbers, 16 stages, as measured and as worked out here:
-//   x 64 .. 777 rows, w 4096:       32 x 64   7.0  9.5 (256 rows) 30 | 7.0 10.5 25     64 x 64  7.8  8.6 12.8 23 | 8.6  8.6 13 19
-//                                  64 x 128   9.4 10.3 11.8 20       | 11 11 11 22   128 x 128 12.2 13.0 13.6 15.5 | 13 13 13 13
-//   x 512 and 777 rows, w 16384:   128 x 128, two at once 27 45 | 27 43                256 x 256  34 40 | 37 37
+// Forms of the tile kernel, and what a call takes in each, in microseconds: some for the first loads and the results, and a stage as much as `low` with one
+// workgroup and `full` with `at_once` of them on each CU, which is as many as have room; more come in turns.  Measured, and as worked out here, with
+// sums of 4096 numbers (16 stages):
+//   32 x 64     64 .. 256 tiles  7.0   7.1 | 6.5  7.8     512   9.5 |  9.5
+//   64 x 64     64 .. 256        7.8   8.6 | 7.7  9.9     512  12.8 | 12.8     2048  42 | 51
+//   64 x 128    32 .. 256        9.4  12.0 | 9.4 12.0     512  20.9 | 24
+//   128 x 128   32 .. 224       12.2  15.8 | 12.6 15.3    344  28.9 | 28.9 (a CU each)
+//   128 x 128   128 .. 256      16.4  18.0 | 15.6 19.2    512  27   | 26       516  37 | 34     896  45 | 48
+//   256 x 256   64 .. 256       27    38.5 | 27.6 38.4    1024 (32 stages)  270 | 275
 struct MxForm {
   int rows, cols, at_once;
-  float base, stage;
+  float base, low, full;
 };
-constexpr MxForm kMxForms[] = {{32, 64, 4, 3.5f, 0.22f},   {64, 64, 2, 3.8f, 0.30f},   {64, 128, 1, 4.1f, 0.42f},
-                               {128, 128, 1, 5.2f, 0.50f}, {128, 128, 2, 5.0f, 0.70f}, {256, 256, 1, 9.0f, 1.75f}};
+constexpr MxForm kMxForms[] = {{32, 64, 2, 3.4f, 0.17f, 0.38f},   {64, 64, 2, 3.8f, 0.20f, 0.56f},   {64, 128, 1, 4.1f, 0.31f, 0.49f},
+                               {128, 128, 1, 5.2f, 0.43f, 0.64f}, {128, 128, 2, 4.0f, 0.50f, 1.40f}, {256, 256, 1, 8.0f, 1.00f, 1.90f}};
 constexpr int kMxFormCount = sizeof(kMxForms) / sizeof(kMxForms[0]);
 
 struct MxChoice {
   int form, splits;
 };
-// Sums in parts cost their joining, 2.0 to 2.5 us for two and 4.5 for four: x 64, w 4096 rows of 16384 numbers take 64 x 64 tiles 19.9, 14.6 or 12.7 us
-// in 1, 2 or 4 parts, of 4096 numbers 7.8, 8.3 or 9.0.
+// Sums in parts cost their joining, measured in two and in four parts: 32 x 64 tiles 2.1 and 3.6 us, 64 x 64 2.9 and 4, 64 x 128 3.6 and 5.3, 128 x 128 6.6
+// and 10.5.
 static MxChoice mx_choose(int64_t rows, int64_t cols, int blocks, int num_cu) {
   MxChoice best = {0, 1};
   float least = 0;
   const int stages = (blocks + kMxStage - 1) / kMxStage;
   for (int f = 0; f < kMxFormCount; ++f) {
     const MxForm &form = kMxForms[f];
-    const int64_t tiles = ceil_div64(rows, form.rows) * ceil_div64(cols, form.cols);
-    for (int splits = 1; splits <= 8 && (splits == 1 || (tiles * splits <= num_cu && splits * 2 <= stages)); splits *= 2) {
-      const float turns = form.at_once == 1 ? (float)ceil_div64(tiles * splits, num_cu) : std::max(1.0f, (float)tiles * splits / num_cu);
-      const float part = form.stage * ((stages + splits - 1) / splits);
-      const float cost = (form.at_once == 1 ? (form.base + part) * turns : form.base + part * turns) + (splits > 1 ? 1.2f + 0.8f * splits : 0.0f);
+    const int64_t tiles = ceil_div64(rows, form.rows) * ceil_div64(cols, form.cols), room = (int64_t)form.at_once * num_cu;
+    for (int splits = 1; splits <= 8 && (splits == 1 || (form.rows < 256 && tiles * splits <= num_cu && splits * 2 <= stages)); splits *= 2) {
+      const int64_t whole = tiles * splits / room, rest = tiles * splits % room;
+      const float each = whole * form.full + (rest ? form.low + (form.full - form.low) * rest / room : 0.0f), size = form.rows * form.cols / 4096.0f;
+      const float join = splits > 1 ? 0.8f + 0.4f * splits + size * (0.7f + 0.3f * splits) : 0.0f;
+      const float starts = form.at_once == 1 ? whole + (rest != 0) : std::max(1.0f, (float)tiles * splits / room);   // with others at work meanwhile
+      const float cost = form.base * starts + each * ((stages + splits - 1) / splits) + join;
       if ((f == 0 && splits == 1) || cost < least) {
         least = cost;
         best = {f, splits};

@@ -25,8 +25,11 @@ __global__ __launch_bounds__(kMxThreads) void mx_quantize_kernel(MxRowsArgs a) {
   if (col + 8 <= a.cols) {
     mx_load8(a.x, row * a.x_stride + col, a.dtype, v);
   } else {
+    // the row's last number in the place of those that are not there: loads without branches, which do not wait for each other
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = col + i < a.cols ? mx_load(a.x, row * a.x_stride + col + i, a.dtype) : 0.0f;
+    for (int i = 0; i < 8; ++i) v[i] = mx_load(a.x, row * a.x_stride + min(col + i, a.cols - 1), a.dtype);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = col + i < a.cols ? v[i] : 0.0f;
   }
   uint32_t byte;
   *(uint32_t *)(a.codes + row * a.codes_stride + (int64_t)block * kMxBytes + t * 4) = mx_quantised8(v, byte);

@@ -129,10 +129,10 @@ def plan_product(ctx, x, w, out, bias=None, residual=None):
     if isinstance(x, MXMatrix):
         return _Plan(ctx, ctx.lib.tpuhip_mx_product, (d, x._d, w._d, out.data_ptr()), keep + (x.codes, x.scales))
     stride, x_type = _rows2(x, "x", ctx, rows, k), _type(x, "x", tuple(TYPES))
-    codes = rows * w.blocks * 16
-    room = _Room.take(ctx, codes + rows * w.blocks)
+    codes, scales = -(-w.blocks // 8) * 128, -(-w.blocks // 16) * 16      # rows that begin at lines of the caches
+    room = _Room.take(ctx, rows * (codes + scales))
     at = room.array.data_ptr()
-    m = capi.MXMatrixDesc(rows, k, at, at + codes, w.blocks * 16, w.blocks)
+    m = capi.MXMatrixDesc(rows, k, at, at + rows * codes, codes, scales)
     return _Linear(ctx, room, ctx.lib.tpuhip_mx_linear, (d, x.data_ptr(), TYPES[x_type], stride, m, w._d, out.data_ptr()), keep + (x, room.array))
 
 
