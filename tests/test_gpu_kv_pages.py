@@ -184,3 +184,48 @@ def test_a_recorded_step_goes_on_by_itself(ctx):
         if step % 20 == 19:
             b.trim([int(v) for v in rng.integers(0, 90, sequences)])
     g.close()
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (40, 4)])
+def test_the_example_answers_the_same_with_pages_from_the_gpu(ctx, window, sinks):
+    """the same pages in the same order: bit for bit"""
+    from tpu_compiler_amd import kv_example
+    model, rng = kv_example.Model(), np.random.default_rng(8)
+    prompts = [rng.integers(0, 512, n) for n in (3, 130, 64, 1)]
+    results = [kv_example.generate(ctx, model, prompts, 6, 4, window, sinks, page_tokens=32, pages_on_gpu=g) for g in (False, True)]
+    assert results[0][0] == results[1][0] and all(np.array_equal(a, b) for a, b in zip(results[0][1], results[1][1]))
+
+
+def test_sequences_end_and_others_take_their_pages(ctx):
+    """a draft that is not taken, a request that ends, one that comes: rows and attention are those of sequences that never saw the others"""
+    from tpu_compiler_amd import kv_example
+    rng = np.random.default_rng(2)
+    sizes = ctx, 1, 4, 2, 64, 8
+    x = {i: rng.standard_normal((300, 8, 64)).astype(np.float32) for i in range(4)}
+    parts = lambda i, a, b: np.split(x[i][a:b], [4, 6], 1)
+
+    def step(s, rows):
+        """rows[b] = (which text, from, to) of sequence b"""
+        s.begin([b - a for _, a, b in rows])
+        q, k, v = (np.concatenate(p) for p in zip(*(parts(*r) for r in rows)))
+        out = s.attend(0, q, k, v)
+        s.end()
+        return np.split(out, np.cumsum([b - a for _, a, b in rows])[:-1])
+
+    s = kv_example.SequencesOnGpu(*sizes, 12, 3, 32)
+    step(s, [(0, 0, 70), (1, 0, 33), (2, 0, 5)])
+    step(s, [(0, 70, 70), (1, 33, 99), (2, 5, 64)])          # six more pages: all twelve but three
+    s.trim([70, 40, 0])                                      # a draft is cut, the last one ends
+    with pytest.raises(ValueError, match="pages"):
+        step(s, [(0, 70, 71), (1, 40, 41), (3, 0, 300)])
+    assert s.lens == [70, 40, 0]
+    got = step(s, [(0, 70, 73), (1, 40, 41), (3, 0, 160)])
+    s.close()
+    for which, a, b in ((0, 70, 73), (1, 40, 41), (3, 0, 160)):
+        alone = kv_example.Sequences(*sizes, 10, 32)
+        if a:
+            step(alone, [(which, 0, a)])
+        want = step(alone, [(which, a, b)])[0]
+        alone.close()
+        # the same rows; sums may be shared otherwise: two roundings of a bfloat16 number of size three at most, and of weights (2^-11 of each)
+        assert np.abs(got.pop(0) - want).max() <= 2.0 ** -5

@@ -304,3 +304,37 @@ def test_no_rows(ctx):
     mx.product(ctx, mx.MXMatrix(ctx, 0, 64).quantize(empty), w, out)
     mx.MXMatrix(ctx, 0, 64).read(empty)
     ctx.sync()
+
+
+def test_the_example_with_weights_in_4_bits(ctx):
+    """prompts and single tokens through a model whose products run here: every one of them is that of its inputs' and weights' values, in 64
+    bits, and the last one's results are the logits that the answers are taken from"""
+    from tpu_compiler_amd import kv_example
+
+    class Noted(kv_example.Model4):
+        def product(self, x, weights, residual=None):
+            y = super().product(x, weights, residual)
+            xv, wv = O.values(*O.quantized(x), weights.cols), O.values(weights.codes.numpy(), weights.scales.numpy(), weights.cols)
+            want, size = O.product(xv, wv, None, None if residual is None else residual.astype(np.float64))
+            assert (np.abs(y - want) <= O.bound(want, size, weights.cols, "f32")).all()
+            self.last = y
+            calls.append(x.shape)
+            return y
+
+    calls = []
+    model, rng = Noted(ctx), np.random.default_rng(4)
+    prompts = [rng.integers(0, 512, n) for n in (9, 70, 1)]
+    answers, steps, _ = kv_example.generate(ctx, model, prompts, 4, 8, page_tokens=32, pages_on_gpu=True)
+    assert [len(a) for a in answers] == [4, 4, 4] and calls[0] == (80, 512) and calls[-1] == (3, 512) and len(calls) == 4 * 7
+    assert np.array_equal(steps[-1], model.last) and [a[-1] for a in answers] == model.last.argmax(-1).tolist()
+    model.close()
+
+
+def test_torch_tensors_and_streams():
+    """in a process of its own, with torch imported first"""
+    import os
+    import subprocess
+    import sys
+    run = subprocess.run([sys.executable, "-u", os.path.join(os.path.dirname(os.path.abspath(__file__)), "mx_torch.py")], stdout=subprocess.PIPE,
+                         stderr=subprocess.STDOUT, text=True, timeout=110)
+    assert run.returncode == 0 and "fine" in run.stdout, run.stdout[-2000:]

@@ -1,16 +1,18 @@
 """A language model that answers from a quantised cache: prompts of different lengths are read into it, then every sequence is continued a
-token at a time.  The model is small and has random weights; its products run on the host, its attention on the GPU:
+token at a time.  The model is small and has random weights; its attention runs on the GPU, its products on the host with float32 weights, or on the
+GPU with weights in 4 bits:
 
-    python -m tpu_compiler_amd.kv_example [--bits 4|8] [--tokens N] [--window W --sinks S]
+    python -m tpu_compiler_amd.kv_example [--bits 4|8] [--tokens N] [--window W --sinks S] [--weights f32|f4] [--pages host|gpu]
 
 What a user of the cache does is in `Sequences`: pages are given out as sequences grow, the new tokens' rows are written to their slots, and
-their queries attend to what the pages hold, prompts and single tokens by the same call."""
+their queries attend to what the pages hold, prompts and single tokens by the same call.  `SequencesOnGpu` gives the pages out on the GPU,
+`Model4` multiplies with weights in microscaled 4-bit floating point, and activations that are quantised on the way."""
 import argparse
 
 import numpy as np
 
-from . import capi
-from .kv_cache import DeviceArray, KVCache
+from . import capi, mx
+from .kv_cache import DeviceArray, KVCache, KVPages
 
 
 class Sequences:
@@ -64,6 +66,44 @@ class Sequences:
             c.close()
 
 
+class SequencesOnGpu(Sequences):
+    """the same for a batch of `sequences`, whose pages, slots and starts are found on the GPU"""
+
+    def __init__(self, ctx, layers, heads, kv_heads, head_dim, bits, pages, sequences, page_tokens=64, window=0, sinks=0):
+        super().__init__(ctx, layers, heads, kv_heads, head_dim, bits, pages, page_tokens, window, sinks)
+        self.batch, self.lens = KVPages(ctx, pages, sequences, pages, page_tokens), [0] * sequences
+
+    def begin(self, new_tokens):
+        put, p = lambda v: DeviceArray.of(self.ctx, v, "i32"), self.batch
+        new, refused = put(new_tokens), DeviceArray(self.ctx, (1,), "i32")
+        self.step = dict(slots=DeviceArray(self.ctx, (sum(new_tokens),), "i32"), starts=DeviceArray(self.ctx, (len(new_tokens) + 1,), "i32"))
+        p.grow(new, self.step["starts"], self.step["slots"], refused)
+        short = int(refused.numpy()[0])              # a loop on the GPU would go on instead, with those that got theirs
+        new.free(), refused.free()
+        if short:
+            self.trim(self.lens)
+            self.end()
+            raise ValueError("pages for %d sequences are not there" % short)
+        self.lens = [a + n for a, n in zip(self.lens, new_tokens)]
+        self.step.update(lens=p.lens, table=p.table, max_q=max(new_tokens), max_kv=max(self.lens))
+
+    def trim(self, keep):
+        """the sequences' tokens behind keep[i] go, and their pages are free"""
+        a = DeviceArray.of(self.ctx, keep, "i32")
+        self.batch.trim(a)
+        a.free()
+        self.lens = [min(have, k) for have, k in zip(self.lens, keep)]
+
+    def end(self):
+        for k in ("slots", "starts"):
+            self.step[k].free()
+
+    def close(self):
+        super().close()
+        for a in (self.batch.lens, self.batch.table, self.batch.free, self.batch.n_free):
+            a.free()
+
+
 class Model:
     """embedding, `layers` of attention with a residual around it, logits"""
 
@@ -77,22 +117,57 @@ class Model:
         self.qkv = [(rng.standard_normal((width, n)) / width ** 0.5).astype(np.float32) for _ in range(layers)]
         self.out = [(rng.standard_normal((width, width)) / width ** 0.5).astype(np.float32) for _ in range(layers)]
 
+    def product(self, x, weights, residual=None):
+        """x times weights (+ residual)"""
+        y = x @ weights
+        return y if residual is None else residual + y
+
     def __call__(self, tokens, attend):
         """tokens [n] -> logits [n, vocabulary]; attend(layer, q, k, v)"""
         x = self.embedding[tokens]
         for layer, (qkv, out) in enumerate(zip(self.qkv, self.out)):
-            y = (x / np.sqrt((x * x).mean(-1, keepdims=True)) @ qkv).reshape(len(x), -1, self.head_dim)
+            y = self.product(x / np.sqrt((x * x).mean(-1, keepdims=True)), qkv).reshape(len(x), -1, self.head_dim)
             q, k, v = np.split(y, [self.heads, self.heads + self.kv_heads], 1)
-            x = x + attend(layer, q, k, v).reshape(len(x), -1) @ out
-        return x / np.sqrt((x * x).mean(-1, keepdims=True)) @ self.logits
+            x = self.product(attend(layer, q, k, v).reshape(len(x), -1), out, x)
+        return self.product(x / np.sqrt((x * x).mean(-1, keepdims=True)), self.logits)
 
 
-def generate(ctx, model, prompts, tokens, bits=4, window=0, sinks=0, page_tokens=64):
+class Model4(Model):
+    """the same with its weights in 4 bits on the GPU, where its products run"""
+
+    def __init__(self, ctx, **sizes):
+        super().__init__(**sizes)
+        self.ctx = ctx
+        self.qkv, self.out, self.logits = [self._quantized(w) for w in self.qkv], [self._quantized(w) for w in self.out], self._quantized(self.logits)
+
+    def _quantized(self, weights):
+        a = DeviceArray.of(self.ctx, weights.T, "f32")
+        m = mx.MXMatrix(self.ctx, *a.shape).quantize(a)
+        a.free()
+        return m
+
+    def product(self, x, weights, residual=None):
+        put = lambda v: DeviceArray.of(self.ctx, v, "f32")
+        a, out = put(x), DeviceArray(self.ctx, (len(x), weights.rows), "f32")
+        more = None if residual is None else put(residual)
+        mx.product(self.ctx, a, weights, out, residual=more)
+        y = out.numpy()
+        for v in (a, out) + (() if more is None else (more,)):
+            v.free()
+        return y
+
+    def close(self):
+        for m in self.qkv + self.out + [self.logits]:
+            m.free()
+
+
+def generate(ctx, model, prompts, tokens, bits=4, window=0, sinks=0, page_tokens=64, pages_on_gpu=False):
     """continues each prompt by `tokens` tokens, the likeliest one each time -> (lists of tokens, logits of every step, bytes of the cache)"""
     if not len(prompts) or not all(len(p) for p in prompts):
         raise ValueError("a prompt has a token at least")
     need = sum(-(-(len(p) + tokens) // page_tokens) for p in prompts)
-    s = Sequences(ctx, len(model.qkv), model.heads, model.kv_heads, model.head_dim, bits, need, page_tokens, window, sinks)
+    sizes = (ctx, len(model.qkv), model.heads, model.kv_heads, model.head_dim, bits, need)
+    s = SequencesOnGpu(*sizes, len(prompts), page_tokens, window, sinks) if pages_on_gpu else Sequences(*sizes, page_tokens, window, sinks)
     answers, steps, new = [[] for _ in prompts], [], [list(p) for p in prompts]
     for _ in range(tokens):
         s.begin([len(n) for n in new])
@@ -114,11 +189,14 @@ def main():
     ap.add_argument("--tokens", type=int, default=16)
     ap.add_argument("--window", type=int, default=0)
     ap.add_argument("--sinks", type=int, default=0)
+    ap.add_argument("--weights", default="f32", choices=("f32", "f4"))
+    ap.add_argument("--pages", default="host", choices=("host", "gpu"))
     a = ap.parse_args()
-    ctx, model = capi.Context(), Model()
+    ctx = capi.Context()
+    model = Model4(ctx) if a.weights == "f4" else Model()
     rng = np.random.default_rng(1)
     prompts = [rng.integers(0, len(model.embedding), n) for n in (5, 130, 64, 1)]
-    answers, _, size = generate(ctx, model, prompts, a.tokens, a.bits, a.window, a.sinks)
+    answers, _, size = generate(ctx, model, prompts, a.tokens, a.bits, a.window, a.sinks, pages_on_gpu=a.pages == "gpu")
     for p, t in zip(prompts, answers):
         print("%4d tokens ->" % len(p), *t)
     print("%d bytes of cache in %d bits" % (size, a.bits))
