@@ -15,6 +15,7 @@ struct MxProductArgs {
   void *y;
   int64_t y_stride, residual_stride;
   int rows, cols, blocks, dtype;
+  FastDiv row_count;
   int depth;                        // numbers of a row, where x is elements; x_stride counts those then
   int splits, split_chunks;         // of the sums over 512 numbers each, among workgroups: of each tile; of them
   float *part;                      // their sums
@@ -97,15 +98,8 @@ __device__ __forceinline__ void mx_put_four(void *y, int64_t row, int n, int col
       if (n + i < cols) mx_store(y, row + n + i, dtype, v[i]);
   }
 }
-// four neighbours of a row of y
-__device__ __forceinline__ void mx_result(const MxProductArgs &a, int m, int n, float4m v) {
-  if (a.bias) v += mx_four(a.bias, 0, n, a.cols, TPUHIP_F32);
-  if (a.residual) v += mx_four(a.residual, (int64_t)m * a.residual_stride, n, a.cols, a.dtype);
-  mx_put_four(a.y, (int64_t)m * a.y_stride, n, a.cols, a.dtype, v);
-}
-
 // A few rows of x, 16 at most: they lie in LDS as codes while a workgroup goes from 16 columns of y (rows of w) to the next.  Its waves take every
-// so manieth 512 numbers of the sums, a chunk; w comes from memory as it lies, a chunk ahead, whichever columns that belongs to; the waves' sums meet in LDS,
+// so manieth 512 numbers of the sums, a chunk; w comes from memory as it lies, two chunks ahead, whichever columns they belong to; the waves' sums meet in LDS,
 // added in the waves' order.
 //   TYPE: of x's elements, which the workgroup quantises for itself, eight numbers a lane; kMxCodes: x is a matrix.
 constexpr int kMxCodes = -1, kMxFew = 16;
@@ -133,15 +127,26 @@ __global__ __launch_bounds__(64 * WAVES) void mx_stream_kernel(MxProductArgs a) 
     for (int s = 0; s < 4; ++s) c.w[s] = *(const uint4m *)(w + (int64_t)min(chunk * 16 + 4 * s + g, a.blocks - 1) * kMxBytes);
     c.s = mx_scales(a.ws + n * a.ws_stride, chunk, a.blocks, g);
   };
-  Chunk now;
+  Chunk now, next;
   int tile = (int)blockIdx.x;
+  // a wave's chunks, of one tile after the other
+  const auto load_after = [&](Chunk &c, int &tile, int &chunk) {
+    chunk += WAVES;
+    if (chunk >= chunks) {
+      chunk = wave;
+      tile += (int)gridDim.x;
+    }
+    if (tile < tiles) load(c, tile, chunk);
+  };
+  int ahead_tile = tile, ahead = wave;
   constexpr int BATCH = 4;
   for (int first = wave; first < max(count, 1 + wave); first += BATCH * WAVES) {
     MxRaw<TYPE> raw[BATCH];
     const auto item = [&](int b, int &m, int &chunk) {         // rows of a chunk follow each other
       const int i = first + b * WAVES;
-      chunk = i / a.rows;
-      m = i % a.rows;
+      uint32_t rest = (uint32_t)i;
+      chunk = (int)a.row_count.split(rest);
+      m = (int)rest;
       return i < count;
     };
 #pragma unroll
@@ -175,7 +180,10 @@ __global__ __launch_bounds__(64 * WAVES) void mx_stream_kernel(MxProductArgs a) 
         }
       }
     }
-    if (first == wave && wave < chunks) load(now, min(tile, tiles - 1), wave);   // behind x, which is waited for first
+    if (first == wave && wave < chunks) {                      // behind x, which is waited for first
+      load(now, tile, wave);
+      load_after(next, ahead_tile, ahead);
+    }
 #pragma unroll
     for (int b = 0; b < BATCH; ++b) {
       int m, chunk;
@@ -205,11 +213,18 @@ __global__ __launch_bounds__(64 * WAVES) void mx_stream_kernel(MxProductArgs a) 
   __syncthreads();
   const uint4m *mine = rows + min(r, a.rows - 1) * 17;         // behind the last row it again: its results go nowhere
   for (int turn = 0; tile < tiles; tile += (int)gridDim.x, ++turn) {
+    // a wave adds the others' sums up while they go on; it is there again before they are written the time after the next
+    const int n = tile * 16 + g * 4;
+    const bool adds = wave == turn % WAVES, result = adds && r < a.rows && n < a.cols;
+    float4m bias = {}, residual = {};
+    if (result) {
+      if (a.bias) bias = mx_four(a.bias, 0, n, a.cols, TPUHIP_F32);
+      if (a.residual) residual = mx_four(a.residual, r * a.residual_stride, n, a.cols, a.dtype);
+    }
     float4m acc = {};
     for (int chunk = wave; chunk < chunks; chunk += WAVES) {
-      const bool last = chunk + WAVES >= chunks;
-      Chunk next;
-      load(next, min(last ? tile + (int)gridDim.x : tile, tiles - 1), last ? wave : chunk + WAVES);
+      Chunk third;
+      load_after(third, ahead_tile, ahead);
       const uint4m *x = mine + chunk * a.rows * 17;
       const uint32_t sx = mx_picked(x[16], g);
       four_times([&](auto s) {
@@ -217,16 +232,15 @@ __global__ __launch_bounds__(64 * WAVES) void mx_stream_kernel(MxProductArgs a) 
         acc = mx_mfma<S>(now.w[S], x[4 * S + g], acc, now.s, sx);
       });
       now = next;
+      next = third;
     }
     sums[turn & 1][wave][lane] = acc;
     __syncthreads();
-    // a wave adds them while the others go on; it is there again before they are written the time after the next
-    if (wave == turn % WAVES) {
-      const int n = tile * 16 + g * 4;
+    if (adds) {
       float4m v = sums[turn & 1][0][lane];
 #pragma unroll
       for (int i = 1; i < WAVES; ++i) v += sums[turn & 1][i][lane];
-      if (r < a.rows && n < a.cols) mx_result(a, r, n, v);
+      if (result) mx_put_four(a.y, r * a.y_stride, n, a.cols, a.dtype, v + bias + residual);
     }
   }
 }
@@ -588,6 +602,7 @@ static int mx_product_args(tpuhip_ctx *ctx, const tpuhip_mx_product_desc *d, con
   a->residual_stride = d->residual_stride;
   a->rows = x->rows;
   a->cols = w->rows;
+  a->row_count = FastDiv(std::max(x->rows, 1));
   a->blocks = mx_blocks(x->cols);
   a->dtype = d->dtype;
   return TPUHIP_OK;
@@ -596,8 +611,8 @@ static int mx_product_args(tpuhip_ctx *ctx, const tpuhip_mx_product_desc *d, con
 // Forms of the tile kernel, and what a call takes in each, in microseconds: some for the first loads and the results, and a stage as much as `low` with one
 // workgroup and `full` with `at_once` of them on each CU, which is as many as have room; more come in turns.  Measured, and as worked out here, with
 // sums of 4096 numbers (16 stages):
-//   32 x 64     64 .. 256 tiles  7.0   7.1 | 6.5  7.8     512   9.5 |  9.5
-//   64 x 64     64 .. 256        7.8   8.6 | 7.7  9.9     512  12.8 | 12.8     2048  42 | 51
+//   32 x 64     64 .. 256 tiles  7.0   7.1 | 6.6  8.1     512  10.3 | 10.1
+//   64 x 64     64 .. 256        7.8   9.0 | 7.6  9.6     512  12.8 | 12.1     2048  42 | 49
 //   64 x 128    32 .. 256        9.4  12.0 | 9.4 12.0     512  20.9 | 24
 //   128 x 128   32 .. 224       12.2  15.8 | 12.6 15.3    344  28.9 | 28.9 (a CU each)
 //   128 x 128   128 .. 256      16.4  18.0 | 15.6 19.2    512  27   | 26       516  37 | 34     896  45 | 48
@@ -606,7 +621,7 @@ struct MxForm {
   int rows, cols, at_once;
   float base, low, full;
 };
-constexpr MxForm kMxForms[] = {{32, 64, 2, 3.4f, 0.17f, 0.38f},   {64, 64, 2, 3.8f, 0.20f, 0.56f},   {64, 128, 1, 4.1f, 0.31f, 0.49f},
+constexpr MxForm kMxForms[] = {{32, 64, 2, 3.4f, 0.17f, 0.42f},   {64, 64, 2, 3.8f, 0.20f, 0.52f},   {64, 128, 1, 4.1f, 0.31f, 0.49f},
                                {128, 128, 1, 5.2f, 0.43f, 0.64f}, {128, 128, 2, 4.0f, 0.50f, 1.40f}, {256, 256, 1, 8.0f, 1.00f, 1.90f}};
 constexpr int kMxFormCount = sizeof(kMxForms) / sizeof(kMxForms[0]);
 
