@@ -31,12 +31,12 @@ __device__ __forceinline__ float4m mx_mfma(uint4m a, uint4m b, float4m c, uint32
   const int8m va = {(int)a[0], (int)a[1], (int)a[2], (int)a[3]}, vb = {(int)b[0], (int)b[1], (int)b[2], (int)b[3]};
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(va, vb, c, 4, 4, S, (int)sa, S, (int)sb);
 }
-template <typename F>
-__device__ __forceinline__ void four_times(F f) {
-  f(std::integral_constant<int, 0>{});
-  f(std::integral_constant<int, 1>{});
-  f(std::integral_constant<int, 2>{});
-  f(std::integral_constant<int, 3>{});
+template <int N, int I = 0, typename F>
+__device__ __forceinline__ void times(F f) {                   // f of 0 .. N - 1, as constants
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    times<N, I + 1>(f);
+  }
 }
 
 // Scales 16 chunk .. 16 chunk + 15 of a row.  Past the row's end they are 0, 2^-127: what such numbers of both operands make is below 2^-200, nothing
@@ -227,7 +227,7 @@ __global__ __launch_bounds__(64 * WAVES) void mx_stream_kernel(MxProductArgs a) 
       load_after(third, ahead_tile, ahead);
       const uint4m *x = mine + chunk * a.rows * 17;
       const uint32_t sx = mx_picked(x[16], g);
-      four_times([&](auto s) {
+      times<4>([&](auto s) {
         constexpr int S = decltype(s)::value;
         acc = mx_mfma<S>(now.w[S], x[4 * S + g], acc, now.s, sx);
       });
@@ -278,10 +278,13 @@ __global__ __launch_bounds__(64 * WM * WN, S == 2 ? 2 : 1) void mx_tile_kernel(M
   constexpr int SR = (ROWS + THREADS - 1) / THREADS;                         // rows whose scales a thread brings
   constexpr int SCALES = ROWS * 128, SIZE = SCALES + ROWS * 16;              // where they lie, and a stage's room
   static_assert(BM % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0 && WAVES % 2 == 0 && (S == 2 || (S == 4 && BM < 256)));
-  __shared__ __attribute__((aligned(128))) uint8_t room0[SIZE];
-  __shared__ __attribute__((aligned(128))) uint8_t room1[SIZE];
-  __shared__ __attribute__((aligned(128))) uint8_t room2[S > 2 ? SIZE : 16];
-  __shared__ __attribute__((aligned(128))) uint8_t room3[S > 2 ? SIZE : 16];
+  // arrays of their own: the compiler has a read wait for loads into the same one
+#define TPUHIP_MX_ROOM(I) __shared__ __attribute__((aligned(128))) uint8_t room##I[S > I ? SIZE : 16]
+  TPUHIP_MX_ROOM(0);
+  TPUHIP_MX_ROOM(1);
+  TPUHIP_MX_ROOM(2);
+  TPUHIP_MX_ROOM(3);
+#undef TPUHIP_MX_ROOM
   const auto room = [&](auto u) -> uint8_t * {
     constexpr int U = decltype(u)::value % S;
     if constexpr (U == 0) return room0;
@@ -354,12 +357,18 @@ __global__ __launch_bounds__(64 * WM * WN, S == 2 ? 2 : 1) void mx_tile_kernel(M
     uint32_t x[MF], w[NF];
   };
   Scales sa, sb;                                               // of two stages
+  // An address for each: of neighbours the compiler makes one read of two places, which it does not know to be of this room alone and has wait for all loads
+  // (4096 x 16384, 17 rows: 9.5 us, with addresses of their own 8.6)
   const auto read_scales = [&](const uint8_t *from) {
-    const uint32_t *at = (const uint32_t *)(from + SCALES) + g * ROWS;
+    const auto at = [&](int row, int stage) {
+      int place = SCALES + ((2 * stage + g) * ROWS + row) * 4;
+      asm("" : "+v"(place));
+      return *(const uint32_t *)(from + place);
+    };
 #pragma unroll
-    for (int f = 0; f < MF; ++f) sa.x[f] = at[wm + f * 32 + r], sb.x[f] = at[2 * ROWS + wm + f * 32 + r];
+    for (int f = 0; f < MF; ++f) sa.x[f] = at(wm + f * 32 + r, 0), sb.x[f] = at(wm + f * 32 + r, 1);
 #pragma unroll
-    for (int f = 0; f < NF; ++f) sa.w[f] = at[BM + wn + f * 32 + r], sb.w[f] = at[2 * ROWS + BM + wn + f * 32 + r];
+    for (int f = 0; f < NF; ++f) sa.w[f] = at(BM + wn + f * 32 + r, 0), sb.w[f] = at(BM + wn + f * 32 + r, 1);
   };
   const int at_x = (wm + r) * 128, at_w = (BM + wn + r) * 128, at_block = ((4 * g) ^ (r >> 1 & 7)) * 16;   // of step 0; others by ^ 16 step
   const auto read = [&](Operands &o, const uint8_t *from, int s, int f) {   // one of w's fragments and as many parts of x's
@@ -391,7 +400,11 @@ __global__ __launch_bounds__(64 * WM * WN, S == 2 ? 2 : 1) void mx_tile_kernel(M
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
   };
-  Operands p, q;
+  // Operands of the multiplied step and of the next.  A wave of one fragment of each has a whole stage's, and reads the next stage's meanwhile: it waits
+  // once a stage for LDS, not four times (sums of 16384 numbers, 64 tiles: 32 x 64 14.8 us, by steps 19.1; 64 x 64 17.4 and 22.3).  Of 128 x 128 they
+  // would take the registers that hold two steps' products (34.9 us, by stages 39.2).
+  constexpr bool WHOLE = S > 2 && MF * NF == 1;
+  Operands p[WHOLE ? 4 : 1], q[WHOLE ? 4 : 1];
   load(0, room0);                                              // what is waited for first, first
   const auto first_scales = [&](auto get) {
     const auto of = [&](int row, uint32_t &even, uint32_t &odd) {
@@ -410,14 +423,18 @@ __global__ __launch_bounds__(64 * WM * WN, S == 2 ? 2 : 1) void mx_tile_kernel(M
     first_scales([&](const uint8_t *row) { return mx_scales16(row, chunk0, a.blocks); });
   load_scales(chunk0 + 1);
   __builtin_amdgcn_sched_barrier(0);
-  four_times([&](auto u) {
-    if constexpr (decltype(u)::value > 0 && decltype(u)::value < S) load(decltype(u)::value, room(u));
+  times<S>([&](auto u) {
+    if constexpr (decltype(u)::value > 0) load(decltype(u)::value, room(u));
   });
   turn(std::integral_constant<int, (S - 1) * L>{});
 #pragma unroll
-  for (int f = 0; f < NF; ++f) read(p, room0, 0, f);
+  for (int k = 0; k < (WHOLE ? 4 : 1); ++k)
+#pragma unroll
+    for (int f = 0; f < NF; ++f) read(p[k], room0, k, f);
+  constexpr std::true_type yes{};
+  constexpr std::false_type no{};
   // A stage; MORE: with the loads of the one S behind it; NEXT: there is a next one.  Behind that one's loads come those of S - 2 stages.
-  constexpr std::integral_constant<int, (S - 2) * L> others{};
+  constexpr std::integral_constant<int, (S - 2) * L> rest{};
   const auto stage = [&](auto u, auto behind, auto more, auto next, int t) {
     constexpr int U = decltype(u)::value;
     constexpr bool MORE = decltype(more)::value, NEXT = decltype(next)::value;
@@ -427,47 +444,61 @@ __global__ __launch_bounds__(64 * WM * WN, S == 2 ? 2 : 1) void mx_tile_kernel(M
     constexpr std::integral_constant<int, 2> b2{};
     constexpr std::integral_constant<int, 3> b3{};
     const Scales now = U % 2 ? sb : sa;
-    step(b0, std::true_type{}, now, p, q, here, 1);
-    if constexpr (NEXT && U % 2 == 1) put_scales(chunk0 + t / 2 + 1, here);
-    __builtin_amdgcn_sched_barrier(0);
-    step(b1, std::true_type{}, now, q, p, here, 2);
-    step(b2, std::true_type{}, now, p, q, here, 3);
-    if constexpr (NEXT) {
-      turn(behind);
-      if constexpr (U % 2 == 1) {
-        read_scales(here);
-        if constexpr (MORE) load_scales(chunk0 + t / 2 + 2);   // before the data: what is in registers has come when the data before it have
+    if constexpr (WHOLE) {
+      Operands(&mine)[sizeof(p) / sizeof(p[0])] = U % 2 ? q : p, (&others)[sizeof(p) / sizeof(p[0])] = U % 2 ? p : q;
+      if constexpr (NEXT) {
+        turn(behind);
+        if constexpr (U % 2 == 1) read_scales(here);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int f = 0; f < NF; ++f) read(others[k], there, k, f);
+        if constexpr (U % 2 == 0) {
+          put_scales(chunk0 + t / 2 + 1, there);
+          if constexpr (MORE) load_scales(chunk0 + t / 2 + 2);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (MORE) load(t + S, here);
       }
+      step(b0, no, now, mine[0], others[0], there, 0);
+      step(b1, no, now, mine[1], others[1], there, 0);
+      step(b2, no, now, mine[2], others[2], there, 0);
+      step(b3, no, now, mine[3], others[3], there, 0);
+    } else {
+      step(b0, yes, now, p[0], q[0], here, 1);
+      if constexpr (NEXT && U % 2 == 1) put_scales(chunk0 + t / 2 + 1, here);
       __builtin_amdgcn_sched_barrier(0);
-      if constexpr (MORE) load(t + S, here);
+      step(b1, yes, now, q[0], p[0], here, 2);
+      step(b2, yes, now, p[0], q[0], here, 3);
+      if constexpr (NEXT) {
+        turn(behind);
+        if constexpr (U % 2 == 1) {
+          read_scales(here);
+          if constexpr (MORE) load_scales(chunk0 + t / 2 + 2);   // before the data: what is in registers has come when the data before it have
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (MORE) load(t + S, here);
+      }
+      step(b3, next, now, q[0], p[0], there, 0);
     }
-    step(b3, next, now, q, p, there, 0);
   };
   constexpr std::integral_constant<int, 0> u0{};
   constexpr std::integral_constant<int, 1> u1{};
-  constexpr std::integral_constant<int, 2> u2{};
-  constexpr std::integral_constant<int, 3> u3{};
-  constexpr std::true_type yes{};
-  constexpr std::false_type no{};
   // No way out of a loop in between: the compiler would have it wait for loads on that way.
   int t = 0;
   if constexpr (S == 2) {                                      // in pairs; behind the last stage come scales of 0
     for (; t + 2 < stages; t += 2) {
-      stage(u0, others, yes, yes, t);
-      stage(u1, others, yes, yes, t + 1);
+      stage(u0, rest, yes, yes, t);
+      stage(u1, rest, yes, yes, t + 1);
     }
-    stage(u0, others, no, yes, t);
-    if (BM >= 256 || t + 1 < stages) stage(u1, others, no, no, t + 1);   // of the largest tiles always: a way around it costs them registers
-  } else {                                                     // one to three are left, of four that have been asked for (those that there are not: zeros)
-    for (; t + 4 <= stages; t += 4) {
-      stage(u0, others, yes, yes, t);
-      stage(u1, others, yes, yes, t + 1);
-      stage(u2, others, yes, yes, t + 2);
-      stage(u3, others, yes, yes, t + 3);
-    }
-    if (t < stages) stage(u0, std::integral_constant<int, 2 * L>{}, no, yes, t);
-    if (t + 1 < stages) stage(u1, std::integral_constant<int, L>{}, no, yes, t + 1);
-    if (t + 2 < stages) stage(u2, std::integral_constant<int, 0>{}, no, yes, t + 2);
+    stage(u0, rest, no, yes, t);
+    if (BM >= 256 || t + 1 < stages) stage(u1, rest, no, no, t + 1);   // of the largest tiles always: a way around it costs them registers
+  } else {                                                     // up to S - 1 are left, of S that have been asked for (those that there are not: zeros)
+    for (; t + S <= stages; t += S) times<S>([&](auto u) { stage(u, rest, yes, yes, t + decltype(u)::value); });
+    times<S - 1>([&](auto u) {
+      constexpr int U = decltype(u)::value;
+      if (t + U < stages) stage(u, std::integral_constant<int, (S - 2 - U) * L>{}, no, yes, t + U);
+    });
   }
   turn(std::integral_constant<int, 0>{});                      // nothing is on its way to LDS any more
   if (a.splits > 1) {
@@ -609,20 +640,20 @@ static int mx_product_args(tpuhip_ctx *ctx, const tpuhip_mx_product_desc *d, con
 }
 
 // Forms of the tile kernel, and what a call takes in each, in microseconds: some for the first loads and the results, and a stage as much as `low` with one
-// workgroup and `full` with `at_once` of them on each CU, which is as many as have room; more come in turns.  Measured, and as worked out here, with
-// sums of 4096 numbers (16 stages):
-//   32 x 64     64 .. 256 tiles  7.0   7.1 | 6.6  8.1     512  10.3 | 10.1
-//   64 x 64     64 .. 256        7.8   9.0 | 7.6  9.6     512  12.8 | 12.1     2048  42 | 49
-//   64 x 128    32 .. 256        9.4  12.0 | 9.4 12.0     512  20.9 | 24
-//   128 x 128   32 .. 224       12.2  15.8 | 12.6 15.3    344  28.9 | 28.9 (a CU each)
-//   128 x 128   128 .. 256      16.4  18.0 | 15.6 19.2    512  27   | 26       516  37 | 34     896  45 | 48
+// workgroup, `one` with one on each CU and `full` with `at_once` of them, which is as many as have room; more come in turns.  Measured | as worked out
+// here, with sums of 4096 numbers (16 stages):
+//   32 x 64     64 .. 256 tiles  6.4   6.8 | 6.2  6.6     512   9.9 |  9.3
+//   64 x 64     64 .. 256        6.9   8.3 | 7.1  7.8     512  13.4 | 12.3     1024  23.2 | 24.6
+//   64 x 128    32 .. 256        9.4  12.4 | 9.4 12.0     512  22   | 24
+//   128 x 128   32 .. 224       12.2  15.8 | 12.5 15.0    344  28.9 | 28.9 (a CU each)
+//   128 x 128   128 .. 256      16.4  18.0 | 15.2 18.4    512  27   | 26       516  37 | 34     896  45 | 46
 //   256 x 256   64 .. 256       27    38.5 | 27.6 38.4    1024 (32 stages)  270 | 275
 struct MxForm {
   int rows, cols, at_once;
-  float base, low, full;
+  float base, low, one, full;
 };
-constexpr MxForm kMxForms[] = {{32, 64, 2, 3.4f, 0.17f, 0.42f},   {64, 64, 2, 3.8f, 0.20f, 0.52f},   {64, 128, 1, 4.1f, 0.31f, 0.49f},
-                               {128, 128, 1, 5.2f, 0.43f, 0.64f}, {128, 128, 2, 4.0f, 0.50f, 1.40f}, {256, 256, 1, 8.0f, 1.00f, 1.90f}};
+constexpr MxForm kMxForms[] = {{32, 64, 2, 3.4f, 0.17f, 0.20f, 0.37f},   {64, 64, 2, 3.5f, 0.21f, 0.27f, 0.55f},   {64, 128, 1, 4.1f, 0.31f, 0.49f, 0.49f},
+                               {128, 128, 1, 5.2f, 0.43f, 0.64f, 0.64f}, {128, 128, 2, 4.0f, 0.60f, 0.90f, 1.40f}, {256, 256, 1, 8.0f, 1.00f, 1.90f, 1.90f}};
 constexpr int kMxFormCount = sizeof(kMxForms) / sizeof(kMxForms[0]);
 
 struct MxChoice {
@@ -639,7 +670,9 @@ static MxChoice mx_choose(int64_t rows, int64_t cols, int blocks, int num_cu) {
     const int64_t tiles = ceil_div64(rows, form.rows) * ceil_div64(cols, form.cols), room = (int64_t)form.at_once * num_cu;
     for (int splits = 1; splits <= 8 && (splits == 1 || (form.rows < 256 && tiles * splits <= num_cu && splits * 2 <= stages)); splits *= 2) {
       const int64_t whole = tiles * splits / room, rest = tiles * splits % room;
-      const float each = whole * form.full + (rest ? form.low + (form.full - form.low) * rest / room : 0.0f), size = form.rows * form.cols / 4096.0f;
+      const float load = (float)rest / num_cu, size = form.rows * form.cols / 4096.0f;
+      const float last = load <= 1 ? form.low + (form.one - form.low) * load : form.one + (form.full - form.one) * (load - 1);
+      const float each = whole * form.full + (rest ? last : 0.0f);
       const float join = splits > 1 ? 0.8f + 0.4f * splits + size * (0.7f + 0.3f * splits) : 0.0f;
       const float starts = form.at_once == 1 ? whole + (rest != 0) : std::max(1.0f, (float)tiles * splits / room);   // with others at work meanwhile
       const float cost = form.base * starts + each * ((stages + splits - 1) / splits) + join;
