@@ -594,7 +594,8 @@ int tpuhip_kv_attention(tpuhip_ctx *ctx, const tpuhip_kv_cache *cache, const tpu
  * itself.  All arrays are int32 in device memory and the caller's: lens (n_seq), the tokens that each sequence holds; table (n_seq rows of
  * max_pages, table_stride apart), its pages, -1 behind the last; free_pages (pages) and n_free (1), a stack of pages that nobody has, the
  * last of the first *n_free the next to go.  A page belongs to one sequence.  What the arrays say is cut to what there is: a length to
- * max_pages * page_tokens and 2^30, a page that does not exist gives slots of -1. */
+ * max_pages * page_tokens and 2^30, a page that does not exist gives slots of -1.  Calls can be captured into a graph, and allocate nothing but
+ * what a context's first cache or attention does. */
 typedef struct {
   int n_seq, pages, page_tokens;      /* 1..65535 sequences; pages and page_tokens as the cache's */
   int max_pages, table_stride;
@@ -625,11 +626,11 @@ int tpuhip_kv_pages_trim(tpuhip_ctx *ctx, const tpuhip_kv_pages *pages, const in
  *   e = floor(log2(max |x|)) - 2, at least -127 (zeros: -127),   code = the nearest to x / 2^e, a tie to the even one, at most 6,
  * and of a block that holds an infinity or a NaN the byte 255, which makes a NaN of all its numbers.  Row i's codes begin at codes + i *
  * codes_stride, its scales at scales + i * scales_stride; codes and codes_stride are multiples of 16 bytes (of a product's matrices below 2^24), scales
- * lie anywhere.  Codes past the
- * last column are zeros: quantising writes them so, and codes from elsewhere have to be.
+ * lie anywhere.  Codes past the last column are zeros: quantising writes them so, and codes from elsewhere have to be.
  *
  * Memory is the caller's, on the context's device; calls can be captured into a graph and allocate nothing, but for the 32 MiB of partial sums
- * that a context has (see above). */
+ * that a context has (see above), which products and pages use as attention does: what is recorded from a context's calls runs neither beside
+ * other recordings of them nor beside its calls. */
 typedef struct {
   int rows, cols;           /* cols: 1..2^24 */
   void *codes, *scales;
@@ -641,7 +642,7 @@ int tpuhip_mx_quantize(tpuhip_ctx *ctx, const tpuhip_mx_matrix *m, const void *x
 int tpuhip_mx_read(tpuhip_ctx *ctx, const tpuhip_mx_matrix *m, void *x, int dtype, int64_t x_stride);
 
 /* y = x w^T (+ bias) (+ residual): x has y's rows, w a row for each of y's columns, both as many columns.  bias: float32, one a column of y, or
- * NULL; residual: like y, of its type, or NULL, and may be y itself.  Products are exact and summed in 32 bits (terms below 2^-126 may
+ * NULL; residual: like y, of its type, or NULL, and may be y itself; y shares memory with nothing else that a call reads.  Products are exact and summed in 32 bits (terms below 2^-126 may
  * count as 0), and what the sum, the bias and the residual come to is rounded once.  The order of the sums depends on sizes alone, unless
  * a context has no memory for partial sums (it gets it with its first product or cache outside of a recording). */
 typedef struct {

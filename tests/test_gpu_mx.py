@@ -201,6 +201,28 @@ def test_long_sums(ctx, rows, cols, n):
         assert np.array_equal(out.numpy(), want)
 
 
+# sizes that take the tiles between the smallest and the largest, and parts of them; sums with a whole number of parts and of pieces, and with a rest
+@pytest.mark.parametrize("rows,cols,n", [(514, 16384, 500), (514, 16600, 500), (640, 32768, 200), (1921, 4096, 1000), (1921, 4400, 1000), (1543, 1250, 2048),
+                                         (1543, 1600, 2048), (1606, 16384, 1000), (1606, 16900, 1000), (1158, 520, 2048), (1795, 300, 8190)])
+def test_tiles_and_parts_with_a_residual_and_what_is_no_number(ctx, rows, cols, n):
+    """a NaN block of x in its last row and one of w in the middle: their row and column, and nothing else"""
+    rng = np.random.default_rng(rows + cols)
+    x, w = codes_of(rng, rows, cols, 127, 127), codes_of(rng, n, cols, 127, 127)
+    want = O.values(*x, cols).astype(np.float32) @ O.values(*w, cols).astype(np.float32).T
+    more = rng.integers(-1000, 1000, (rows, n)).astype(np.float32)
+    assert cols * 36 < 2 ** 24 / 4 - 1000              # in units of 2^-2, in any order
+    want += more
+    x[1][rows - 1, -1] = w[1][n // 2, 0] = 255
+    want[rows - 1] = want[:, n // 2] = np.nan
+    a, b, out = matrix(ctx, *x, cols), matrix(ctx, *w, cols), DeviceArray(ctx, (rows, n), "f32")
+    for _ in range(2):
+        ctx.upload(out.ptr, more)
+        mx.product(ctx, a, b, out, residual=out)
+        assert np.array_equal(out.numpy(), want, equal_nan=True)
+    for m in (a, b, out):
+        m.free()
+
+
 @pytest.mark.parametrize("ready", [False, True])
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("rows,cols,n", SHAPES)

@@ -70,6 +70,12 @@ def test_products_that_are_refused(x, out, more, says):
     assert not [c for c in ctx.lib.calls if "mx" in c[0]]
 
 
+def test_a_product_in_the_place_of_its_rows_is_refused():
+    ctx, x = context(), Array((6, 70), "f32")
+    refuses(lambda: mx.plan_product(ctx, x, matrix(ctx, 70, 70), x), "place")
+    mx.plan_product(ctx, Array((6, 70), "f32"), matrix(ctx, 70, 70), x, residual=x)()
+
+
 def test_matrices_that_are_refused():
     ctx = context()
     codes, scales = Array((4, 48), "u8"), Array((4, 3), "u8")

@@ -102,7 +102,7 @@ class _Linear(_Plan):
 def plan_product(ctx, x, w, out, bias=None, residual=None):
     """A call that computes out = x w^T (+ bias) (+ residual).  w: an MXMatrix [columns of out, k]; x: one too, [rows of out, k], or an array of
     bf16, f16 or f32, which the call quantises (in memory that the plan keeps).  out, residual (may be out): bf16, f16 or f32, [rows, columns]; bias:
-    f32, [columns]."""
+    f32, [columns].  out shares memory with nothing else that the call reads."""
     if not isinstance(w, MXMatrix):
         _refuse("w: no MXMatrix")
     if not isinstance(x, MXMatrix) and len(x.shape) != 2:
@@ -110,6 +110,8 @@ def plan_product(ctx, x, w, out, bias=None, residual=None):
     rows, k = (x.rows, x.cols) if isinstance(x, MXMatrix) else (_int(x.shape[0], "rows"), int(x.shape[1]))
     if k != w.cols:
         _refuse("x has %d columns, w %d" % (k, w.cols))
+    if x is out:
+        _refuse("out in the place of x")
     for m in (x, w):
         if isinstance(m, MXMatrix) and m.ctx.device != ctx.device:
             _refuse("a matrix lies on device %d, the context works on device %d" % (m.ctx.device, ctx.device))
