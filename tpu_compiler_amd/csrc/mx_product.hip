@@ -250,7 +250,12 @@ __global__ __launch_bounds__(64 * WAVES) void mx_stream_kernel(MxProductArgs a) 
 // stage's last products all waves have read it and the next one has come (one barrier a stage), and its room is filled anew.
 //   Order in LDS: rows of 128 bytes, block c of a row in place c ^ row / 2 % 8, so that sixteen lanes that read the same block of rows next to each
 // other use all 64 banks (with row % 8 each read took twice the time).  Lane (r, g) has blocks 4g..4g + 3 of a stage: its scales are four bytes.
-// Scales come by way of registers, two stages' at a time, and are written in the odd stages, behind the data that are being multiplied: an access to LDS waits for the loads that are on their way to the same array, and one to an array that has none for all of them.
+// Scales come by way of registers, two stages' at a time, and lie behind a stage's data: an access to LDS waits for the loads that are on their way to the
+// same array, and one to an array that has none for all of them.
+//   Bound by what a CU takes in: a small tile's rows of both operands come at 48 of 64 bytes a clock, with the scales, 16 bytes of a line each, more.
+// Without a stage's products, or its reads, 64 x 64 tiles take as long (sums of 16384 numbers, 64 rows: 18.7 us; 14.7 without the scales, 11.5 without
+// the data).  256 x 256 are bound by products: 8192 x 8192 x 8192 take 266 us, 4.1 PFLOP/s, at a clock of 1.6 GHz that the power leaves (products of registers alone,
+// of random numbers: 6.2 PFLOP/s; 231 us without loads, 253 without results).
 constexpr int kMxStage = 8;   // blocks of a stage
 
 typedef __attribute__((address_space(3))) uint8_t mx_lds;
@@ -335,19 +340,21 @@ __global__ __launch_bounds__(64 * WM * WN, S == 2 ? 2 : 1) void mx_tile_kernel(M
 #pragma unroll
     for (int i = 0; i < SR; ++i) next_scales[i] = *(const uint4m_any *)(scale_rows[i] + max(min(chunk * 16, a.blocks - 16), 0));
   };
-  const auto put_scales = [&](int chunk, uint8_t *to) {
+  const auto put_scales = [&](auto ends, int chunk, uint8_t *to) {   // ends: of a chunk that may reach past the row's end
     const int drop = min(chunk * 16 - min(chunk * 16, a.blocks - 16), 15);
     const uint32_t one = drop & 4 ? ~0u : 0u, two = drop & 8 ? ~0u : 0u, bytes = drop & 3;
     const auto pick = [](uint32_t mask, uint32_t x, uint32_t y) { return (x & mask) | (y & ~mask); };
 #pragma unroll
     for (int i = 0; i < SR; ++i) {
       uint4m v = next_scales[i];
-      v = (uint4m){pick(one, v[1], v[0]), pick(one, v[2], v[1]), pick(one, v[3], v[2]), v[3] & ~one};
-      v = (uint4m){pick(two, v[2], v[0]), pick(two, v[3], v[1]), v[2] & ~two, v[3] & ~two};
-      v = (uint4m){__builtin_amdgcn_alignbyte(v[1], v[0], bytes), __builtin_amdgcn_alignbyte(v[2], v[1], bytes),
-                   __builtin_amdgcn_alignbyte(v[3], v[2], bytes), __builtin_amdgcn_alignbyte(0, v[3], bytes)};
-#pragma unroll
-      for (int k = 0; k < 4; ++k) ((uint32_t *)(to + SCALES))[k * ROWS + min(i * THREADS + (int)threadIdx.x, ROWS - 1)] = v[k];   // some threads have the same row
+      if constexpr (decltype(ends)::value) {
+        v = (uint4m){pick(one, v[1], v[0]), pick(one, v[2], v[1]), pick(one, v[3], v[2]), v[3] & ~one};
+        v = (uint4m){pick(two, v[2], v[0]), pick(two, v[3], v[1]), v[2] & ~two, v[3] & ~two};
+        v = (uint4m){__builtin_amdgcn_alignbyte(v[1], v[0], bytes), __builtin_amdgcn_alignbyte(v[2], v[1], bytes),
+                     __builtin_amdgcn_alignbyte(v[3], v[2], bytes), __builtin_amdgcn_alignbyte(0, v[3], bytes)};
+      }
+      uint32_t *at = (uint32_t *)(to + SCALES) + min(i * THREADS + (int)threadIdx.x, ROWS - 1) * 4;   // some threads have the same row
+      at[0] = v[0], at[1] = v[2], at[2] = v[1], at[3] = v[3];
     }
   };
   struct Operands {
@@ -357,18 +364,21 @@ __global__ __launch_bounds__(64 * WM * WN, S == 2 ? 2 : 1) void mx_tile_kernel(M
     uint32_t x[MF], w[NF];
   };
   Scales sa, sb;                                               // of two stages
-  // An address for each: of neighbours the compiler makes one read of two places, which it does not know to be of this room alone and has wait for all loads
-  // (4096 x 16384, 17 rows: 9.5 us, with addresses of their own 8.6)
+  // Two stages' scales of a lane lie next to each other.  A fragment's address is one that the compiler knows nothing of: of neighbours it makes one read
+  // of two places, which it does not know to be of this room alone and has wait for all loads (4096 x 16384, 17 rows: 9.5 us, so 8.6).
+  int places[MF + NF];
+#pragma unroll
+  for (int f = 0; f < MF + NF; ++f) {
+    places[f] = SCALES + (f < MF ? wm + f * 32 + r : BM + wn + (f - MF) * 32 + r) * 16 + g * 8;
+    asm("" : "+v"(places[f]));
+  }
   const auto read_scales = [&](const uint8_t *from) {
-    const auto at = [&](int row, int stage) {
-      int place = SCALES + ((2 * stage + g) * ROWS + row) * 4;
-      asm("" : "+v"(place));
-      return *(const uint32_t *)(from + place);
-    };
 #pragma unroll
-    for (int f = 0; f < MF; ++f) sa.x[f] = at(wm + f * 32 + r, 0), sb.x[f] = at(wm + f * 32 + r, 1);
-#pragma unroll
-    for (int f = 0; f < NF; ++f) sa.w[f] = at(BM + wn + f * 32 + r, 0), sb.w[f] = at(BM + wn + f * 32 + r, 1);
+    for (int f = 0; f < MF + NF; ++f) {
+      const uint2m v = *(const uint2m *)(from + places[f]);
+      (f < MF ? sa.x[f] : sa.w[f - MF]) = v[0];
+      (f < MF ? sb.x[f] : sb.w[f - MF]) = v[1];
+    }
   };
   const int at_x = (wm + r) * 128, at_w = (BM + wn + r) * 128, at_block = ((4 * g) ^ (r >> 1 & 7)) * 16;   // of step 0; others by ^ 16 step
   const auto read = [&](Operands &o, const uint8_t *from, int s, int f) {   // one of w's fragments and as many parts of x's
@@ -435,7 +445,7 @@ __global__ __launch_bounds__(64 * WM * WN, S == 2 ? 2 : 1) void mx_tile_kernel(M
   constexpr std::false_type no{};
   // A stage; MORE: with the loads of the one S behind it; NEXT: there is a next one.  Behind that one's loads come those of S - 2 stages.
   constexpr std::integral_constant<int, (S - 2) * L> rest{};
-  const auto stage = [&](auto u, auto behind, auto more, auto next, int t) {
+  const auto stage = [&](auto u, auto behind, auto more, auto next, auto ends, int t) {
     constexpr int U = decltype(u)::value;
     constexpr bool MORE = decltype(more)::value, NEXT = decltype(next)::value;
     uint8_t *const here = room(u), *const there = room(std::integral_constant<int, U + 1>{});
@@ -454,7 +464,7 @@ __global__ __launch_bounds__(64 * WM * WN, S == 2 ? 2 : 1) void mx_tile_kernel(M
 #pragma unroll
           for (int f = 0; f < NF; ++f) read(others[k], there, k, f);
         if constexpr (U % 2 == 0) {
-          put_scales(chunk0 + t / 2 + 1, there);
+          put_scales(ends, chunk0 + t / 2 + 1, there);
           if constexpr (MORE) load_scales(chunk0 + t / 2 + 2);
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -466,7 +476,7 @@ __global__ __launch_bounds__(64 * WM * WN, S == 2 ? 2 : 1) void mx_tile_kernel(M
       step(b3, no, now, mine[3], others[3], there, 0);
     } else {
       step(b0, yes, now, p[0], q[0], here, 1);
-      if constexpr (NEXT && U % 2 == 1) put_scales(chunk0 + t / 2 + 1, here);
+      if constexpr (NEXT && U % 2 == 1) put_scales(ends, chunk0 + t / 2 + 1, here);
       __builtin_amdgcn_sched_barrier(0);
       step(b1, yes, now, q[0], p[0], here, 2);
       step(b2, yes, now, p[0], q[0], here, 3);
@@ -488,16 +498,20 @@ __global__ __launch_bounds__(64 * WM * WN, S == 2 ? 2 : 1) void mx_tile_kernel(M
   int t = 0;
   if constexpr (S == 2) {                                      // in pairs; behind the last stage come scales of 0
     for (; t + 2 < stages; t += 2) {
-      stage(u0, rest, yes, yes, t);
-      stage(u1, rest, yes, yes, t + 1);
+      stage(u0, rest, yes, yes, yes, t);
+      stage(u1, rest, yes, yes, yes, t + 1);
     }
-    stage(u0, rest, no, yes, t);
-    if (BM >= 256 || t + 1 < stages) stage(u1, rest, no, no, t + 1);   // of the largest tiles always: a way around it costs them registers
-  } else {                                                     // up to S - 1 are left, of S that have been asked for (those that there are not: zeros)
-    for (; t + S <= stages; t += S) times<S>([&](auto u) { stage(u, rest, yes, yes, t + decltype(u)::value); });
-    times<S - 1>([&](auto u) {
+    stage(u0, rest, no, yes, yes, t);
+    if (BM >= 256 || t + 1 < stages) stage(u1, rest, no, no, yes, t + 1);   // of the largest tiles always: a way around it costs them registers
+  } else {
+    // The loop ends before a chunk that may reach past a row's end is put, as a wave has a SIMD to itself where tiles are few: 64 x 64, sums of 16384
+    // numbers, 64 tiles: 16.2 us, with the shifts of the ends in it 17.6; 128 x 128 31.6 and 35.0.  Up to S + 2 stages are left then, of S that have been
+    // asked for (those that there are not: zeros).
+    for (; t + S + 3 <= stages; t += S) times<S>([&](auto u) { stage(u, rest, yes, yes, no, t + decltype(u)::value); });
+    times<S + 2>([&](auto u) {
       constexpr int U = decltype(u)::value;
-      if (t + U < stages) stage(u, std::integral_constant<int, (S - 2 - U) * L>{}, no, yes, t + U);
+      constexpr std::integral_constant<int, (U < 2 ? S - 2 : U < S ? S - U : 0) * L> behind{};
+      if (t + U < stages) stage(u, behind, std::bool_constant<(U < 2)>{}, yes, yes, t + U);
     });
   }
   turn(std::integral_constant<int, 0>{});                      // nothing is on its way to LDS any more
