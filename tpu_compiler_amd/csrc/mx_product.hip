@@ -99,10 +99,11 @@ __device__ __forceinline__ void mx_put_four(void *y, int64_t row, int n, int col
   }
 }
 // A few rows of x, 16 at most: they lie in LDS as codes while a workgroup goes from 16 columns of y (rows of w) to the next.  Its waves take every
-// so manieth 512 numbers of the sums, a chunk; w comes from memory as it lies, two chunks ahead, whichever columns they belong to; the waves' sums meet in LDS,
+// so manieth 512 numbers of the sums, a chunk; w comes from memory as it lies, a chunk ahead, whichever columns that belongs to; the waves' sums meet in LDS,
 // added in the waves' order.
-//   Bound by the reading of w: 65536 columns of 4096 numbers, 143 MB, by a row of float32 take 26.2 us (5.4 TB/s, some of it from the last cache);
-// 4096 columns, 9 MB, 4.3 us, half of that the chain of x, its blocks' scales, w and the sums.
+//   Bound by the reading of w: 65536 columns of 4096 numbers, 143 MB, by a row of float32 take 24.8 us (5.8 TB/s, some of it from the last cache; 29.8
+// with a second chunk ahead, which the compiler moves from register to register and waits for, and 28.5 with biases and residuals asked for before the
+// sums); 4096 columns, 9 MB, 4.3 us, half of that the chain of x, its blocks' scales, w and the sums.
 //   TYPE: of x's elements, which the workgroup quantises for itself, eight numbers a lane; kMxCodes: x is a matrix.
 constexpr int kMxCodes = -1, kMxFew = 16;
 constexpr int kMxFewPieces = 64;   // of x, 512 numbers of a row each
@@ -129,7 +130,7 @@ __global__ __launch_bounds__(64 * WAVES) void mx_stream_kernel(MxProductArgs a) 
     for (int s = 0; s < 4; ++s) c.w[s] = *(const uint4m *)(w + (int64_t)min(chunk * 16 + 4 * s + g, a.blocks - 1) * kMxBytes);
     c.s = mx_scales(a.ws + n * a.ws_stride, chunk, a.blocks, g);
   };
-  Chunk now, next;
+  Chunk now;
   int tile = (int)blockIdx.x;
   // a wave's chunks, of one tile after the other
   const auto load_after = [&](Chunk &c, int &tile, int &chunk) {
@@ -182,10 +183,7 @@ __global__ __launch_bounds__(64 * WAVES) void mx_stream_kernel(MxProductArgs a) 
         }
       }
     }
-    if (first == wave && wave < chunks) {                      // behind x, which is waited for first
-      load(now, tile, wave);
-      load_after(next, ahead_tile, ahead);
-    }
+    if (first == wave && wave < chunks) load(now, tile, wave);   // behind x, which is waited for first
 #pragma unroll
     for (int b = 0; b < BATCH; ++b) {
       int m, chunk;
@@ -215,18 +213,10 @@ __global__ __launch_bounds__(64 * WAVES) void mx_stream_kernel(MxProductArgs a) 
   __syncthreads();
   const uint4m *mine = rows + min(r, a.rows - 1) * 17;         // behind the last row it again: its results go nowhere
   for (int turn = 0; tile < tiles; tile += (int)gridDim.x, ++turn) {
-    // a wave adds the others' sums up while they go on; it is there again before they are written the time after the next
-    const int n = tile * 16 + g * 4;
-    const bool adds = wave == turn % WAVES, result = adds && r < a.rows && n < a.cols;
-    float4m bias = {}, residual = {};
-    if (result) {
-      if (a.bias) bias = mx_four(a.bias, 0, n, a.cols, TPUHIP_F32);
-      if (a.residual) residual = mx_four(a.residual, r * a.residual_stride, n, a.cols, a.dtype);
-    }
     float4m acc = {};
     for (int chunk = wave; chunk < chunks; chunk += WAVES) {
-      Chunk third;
-      load_after(third, ahead_tile, ahead);
+      Chunk next;
+      load_after(next, ahead_tile, ahead);
       const uint4m *x = mine + chunk * a.rows * 17;
       const uint32_t sx = mx_picked(x[16], g);
       times<4>([&](auto s) {
@@ -234,15 +224,21 @@ __global__ __launch_bounds__(64 * WAVES) void mx_stream_kernel(MxProductArgs a) 
         acc = mx_mfma<S>(now.w[S], x[4 * S + g], acc, now.s, sx);
       });
       now = next;
-      next = third;
     }
     sums[turn & 1][wave][lane] = acc;
     __syncthreads();
-    if (adds) {
+    // a wave adds them up while the others go on; it is there again before they are written the time after the next
+    if (wave == turn % WAVES) {
       float4m v = sums[turn & 1][0][lane];
 #pragma unroll
       for (int i = 1; i < WAVES; ++i) v += sums[turn & 1][i][lane];
-      if (result) mx_put_four(a.y, r * a.y_stride, n, a.cols, a.dtype, v + bias + residual);
+      const int n = tile * 16 + g * 4;
+      if (r < a.rows && n < a.cols) {
+        float4m bias = {}, residual = {};
+        if (a.bias) bias = mx_four(a.bias, 0, n, a.cols, TPUHIP_F32);
+        if (a.residual) residual = mx_four(a.residual, r * a.residual_stride, n, a.cols, a.dtype);
+        mx_put_four(a.y, r * a.y_stride, n, a.cols, a.dtype, v + bias + residual);
+      }
     }
   }
 }
