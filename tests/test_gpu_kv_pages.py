@@ -186,6 +186,29 @@ def test_a_recorded_step_goes_on_by_itself(ctx):
     g.close()
 
 
+def test_a_context_s_first_calls_are_recorded():
+    """with pages and slots for several workgroups, of which there is one without a counter; later ones by themselves have it"""
+    c = capi.Context()
+    b = Both(c, 20000, 300, 100, 32)
+    rng = np.random.default_rng(5)
+    new, starts, slots, refused, keep = ints(c, [0] * 300), ints(c, [0] * 301), ints(c, [0] * 9000), ints(c, [0]), ints(c, [0] * 300)
+    trim, grow = b.here.plan_trim(keep), b.here.plan_grow(new, starts, slots, refused)
+    g = gpu_capture.Graph(c.h)
+    with g.recording():
+        trim(), grow()
+    for step in range(4):
+        for run in (g.replay, lambda: (trim(), grow())):
+            stay, more = rng.integers(0, 3000, 300), rng.integers(0, 50, 300)
+            c.upload(keep.ptr, stay.astype(np.int32)), c.upload(new.ptr, more.astype(np.int32))
+            run()
+            b.want.trim(stay.tolist())
+            want = b.want.grow(more.tolist(), 9000)
+            assert slots.numpy().tolist() == [int(v) for v in want[1]] and refused.numpy()[0] == want[2]
+            b.same()
+    g.close()
+    c.close()
+
+
 @pytest.mark.parametrize("window,sinks", [(0, 0), (40, 4)])
 def test_the_example_answers_the_same_with_pages_from_the_gpu(ctx, window, sinks):
     """the same pages in the same order: bit for bit"""

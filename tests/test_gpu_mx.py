@@ -307,6 +307,61 @@ def test_a_recorded_product_follows_its_inputs(ctx, rows, cols, n):
     g.close()
 
 
+@pytest.mark.parametrize("x_type,dtype", [("f32", "bf16"), ("bf16", "f32"), ("f16", "bf16"), ("f32", "f16")])
+@pytest.mark.parametrize("rows", [2, 70])
+def test_rows_of_one_type_and_results_of_another(ctx, rows, x_type, dtype):
+    rng, cols, n = np.random.default_rng(rows), 700, 75
+    x, more = O.rounded(rng.standard_normal((rows, cols)), x_type), O.rounded(rng.standard_normal((rows, n)), dtype)
+    w = codes_of(rng, n, cols, 118, 124)
+    want, size = O.product(O.values(*O.quantized(x), cols), O.values(*w, cols), None, more)
+    out = DeviceArray.of(ctx, more, dtype)
+    mx.product(ctx, DeviceArray.of(ctx, x, x_type), matrix(ctx, *w, cols), out, residual=out)
+    assert (np.abs(out.numpy().astype(np.float64) - want) <= O.bound(want, size, cols, dtype)).all()
+
+
+def whole_numbers(ctx, rows, cols, n, seed):
+    """operands and their product, which 32 bits hold in any order"""
+    rng = np.random.default_rng(seed)
+    x, w = codes_of(rng, rows, cols, 127, 127), codes_of(rng, n, cols, 127, 127)
+    assert cols * 36 < 2 ** 24 / 4
+    want, _ = O.product(O.values(*x, cols), O.values(*w, cols))
+    return matrix(ctx, *x, cols), matrix(ctx, *w, cols), DeviceArray.of(ctx, np.full((rows, n), 7.0), "f32"), want
+
+
+def test_two_contexts_at_once():
+    """sums in parts on two streams: each context has counters and parts of its own"""
+    contexts = [capi.Context(), capi.Context()]
+    cases = [[(c,) + whole_numbers(c, rows, 16384, n, n) for rows, n in ((64, 500), (17, 300))] for c in contexts]
+    plans = [mx.plan_product(c, x, w, out) for pair in zip(*cases) for c, x, w, out, _ in pair]
+    for _ in range(10):
+        for plan in plans:
+            plan()
+    for case in cases:
+        for c, _, _, out, want in case:
+            assert np.array_equal(out.numpy(), want)
+    for c in contexts:
+        c.close()
+
+
+def test_a_context_s_first_call_is_recorded():
+    """no memory for parts then, which later calls of the context by themselves have"""
+    c = capi.Context()
+    x, w, out, want = whole_numbers(c, 40, 16384, 300, 1)
+    plan = mx.plan_product(c, x, w, out)
+    g = gpu_capture.Graph(c.h)
+    with g.recording():
+        plan()
+    for _ in range(3):
+        c.upload(out.ptr, np.zeros((40, 300), np.float32))
+        g.replay()
+        assert np.array_equal(out.numpy(), want)
+        c.upload(out.ptr, np.zeros((40, 300), np.float32))
+        plan()
+        assert np.array_equal(out.numpy(), want)
+    g.close()
+    c.close()
+
+
 def test_the_same_call_gives_the_same_bits(ctx):
     rng = np.random.default_rng(9)
     for rows, cols, n in ((1, 4096, 512), (16, 16384, 64), (60, 8192, 128), (128, 4096, 256)):
