@@ -203,7 +203,8 @@ def test_long_sums(ctx, rows, cols, n):
 
 # sizes that take the tiles between the smallest and the largest, and parts of them; sums with a whole number of parts and of pieces, and with a rest
 @pytest.mark.parametrize("rows,cols,n", [(514, 16384, 500), (514, 16600, 500), (640, 32768, 200), (1921, 4096, 1000), (1921, 4400, 1000), (1543, 1250, 2048),
-                                         (1543, 1600, 2048), (1606, 16384, 1000), (1606, 16900, 1000), (1158, 520, 2048), (1795, 300, 8190)])
+                                         (1543, 1600, 2048), (1606, 16384, 1000), (1606, 16900, 1000), (1158, 520, 2048), (1795, 16384, 1000), (1795, 16900, 1000),
+                                         (1543, 300, 5000), (1600, 1100, 5001), (2054, 700, 2048), (1795, 300, 8190)])
 def test_tiles_and_parts_with_a_residual_and_what_is_no_number(ctx, rows, cols, n):
     """a NaN block of x in its last row and one of w in the middle: their row and column, and nothing else"""
     rng = np.random.default_rng(rows + cols)

@@ -569,8 +569,9 @@ __global__ __launch_bounds__(64 * WM * WN, S == 2 ? 2 : 1) void mx_tile_kernel(M
   // Results go through LDS, a wave's by itself, 32 rows at a time: then a lane has four neighbours of a row, the same ones of every row, and FOURS lanes
   // have a row of the wave's.  Four numbers c of row m lie in place c ^ key(m).
   constexpr int FOURS = NF * 8, PASS = 64 / FOURS, PASSES = 32 / PASS;
-  static_assert(WAVES * 32 * FOURS * 16 <= ROWS * 128);
-  float4m *mine = (float4m *)room0 + wave * 32 * FOURS;
+  constexpr int HERE = WAVES * 32 * FOURS * 16 <= ROWS * 128 ? WAVES : WAVES / 2;   // waves that a room is large enough for
+  static_assert(HERE * 32 * FOURS * 16 <= ROWS * 128);
+  float4m *mine = (float4m *)(wave < HERE ? room0 : room1) + wave % HERE * 32 * FOURS;
   const auto key = [](int row) { return FOURS == 8 ? row >> 1 & 7 : row & (FOURS < 16 ? FOURS - 1 : 15); };   // sixteen rows in all banks
   const int four = lane % FOURS, row0 = lane / FOURS, n = n0 + wn + 4 * four;
   const float4m bias = a.bias ? mx_four(a.bias, 0, min(n, a.cols - 1), a.cols, TPUHIP_F32) : (float4m){0, 0, 0, 0};
@@ -654,26 +655,29 @@ static int mx_product_args(tpuhip_ctx *ctx, const tpuhip_mx_product_desc *d, con
 // Forms of the tile kernel, and what a call takes in each, in microseconds: some for the first loads and the results, and a stage as much as `low` with one
 // workgroup, `one` with one on each CU and `full` with `at_once` of them, which is as many as have room; more come in turns.  Measured | as worked out
 // here, with sums of 4096 numbers (16 stages):
-//   32 x 64     64 .. 256 tiles  6.4   6.8 | 6.2  6.6     512   9.9 |  9.3
-//   64 x 64     64 .. 256        6.9   8.3 | 7.1  7.8     512  13.4 | 12.3     1024  23.2 | 24.6
-//   64 x 128    32 .. 256        9.4  12.4 | 9.4 12.0     512  22   | 24
-//   128 x 128   32 .. 224       12.2  15.8 | 12.5 15.0    344  28.9 | 28.9 (a CU each)
-//   128 x 128   128 .. 256      16.4  18.0 | 15.2 18.4    512  27   | 26       516  37 | 34     896  45 | 46
-//   256 x 256   64 .. 256       27    38.5 | 27.6 38.4    1024 (32 stages)  270 | 275
+//   32 x 64     64 .. 256 tiles  6.1   6.8 | 6.3  6.6     512   9.8 | 10.4
+//   64 x 64     64 .. 256        6.9   8.2 | 7.1  7.8     512  13.3 | 13.1     1024  21.9 | 23.4
+//   64 x 128    32 .. 256        9.4  12.3 | 9.4 11.9     512  21.5 | 23.9
+//   128 x 128   32 .. 256       12.2  17.5 | 12.5 15.4
+//   128 x 128   128 .. 256      15.0  18.2 | 16.7 17.5    512  28.4 | 28.8     1032  60.4 | 62.8
+//   256 x 128   32 .. 256       19.1  25.3 | 19.5 24.0    688  68.0 | 70.3
+//   256 x 256   64 .. 256       29.9  43.0 | 29.7 42.3    688  115  | 121      1024 (32 stages)  266 | 300
 struct MxForm {
   int rows, cols, at_once;
   float base, low, one, full;
 };
-constexpr MxForm kMxForms[] = {{32, 64, 2, 3.4f, 0.17f, 0.20f, 0.37f},   {64, 64, 2, 3.5f, 0.21f, 0.27f, 0.55f},   {64, 128, 1, 4.1f, 0.31f, 0.49f, 0.49f},
-                               {128, 128, 1, 5.2f, 0.43f, 0.64f, 0.64f}, {128, 128, 2, 4.0f, 0.60f, 0.90f, 1.40f}, {256, 256, 1, 8.0f, 1.00f, 1.90f, 1.90f}};
+constexpr MxForm kMxForms[] = {{32, 64, 2, 3.4f, 0.17f, 0.20f, 0.31f},   {64, 64, 2, 3.5f, 0.21f, 0.27f, 0.47f},   {64, 128, 1, 4.1f, 0.31f, 0.49f, 0.49f},
+                               {128, 128, 1, 5.2f, 0.43f, 0.64f, 0.64f}, {128, 128, 2, 6.0f, 0.62f, 0.72f, 1.20f}, {256, 128, 1, 6.4f, 0.78f, 1.10f, 1.10f},
+                               {256, 256, 1, 9.5f, 1.00f, 2.05f, 2.05f}};
 constexpr int kMxFormCount = sizeof(kMxForms) / sizeof(kMxForms[0]);
 
 struct MxChoice {
   int form, splits;
 };
 // Sums in parts cost their joining, measured in two and in four parts: 32 x 64 tiles 2.1 and 3.6 us, 64 x 64 2.9 and 4, 64 x 128 3.6 and 5.3, 128 x 128 6.6
-// and 10.5.
-static MxChoice mx_choose(int64_t rows, int64_t cols, int blocks, int num_cu) {
+// and 10.5.  bytes: that a result and what it is added to take, which a CU moves 40 KB a microsecond of; two are in the table above.  777 x 2050 x 4999 of
+// float32 with a residual, 8 bytes: 128 x 128 22.9 us, 256 x 128 23.7; of 2 bytes 18.8 and 17.5.
+static MxChoice mx_choose(int64_t rows, int64_t cols, int blocks, int bytes, int num_cu) {
   MxChoice best = {0, 1};
   float least = 0;
   const int stages = (blocks + kMxStage - 1) / kMxStage;
@@ -686,8 +690,10 @@ static MxChoice mx_choose(int64_t rows, int64_t cols, int blocks, int num_cu) {
       const float last = load <= 1 ? form.low + (form.one - form.low) * load : form.one + (form.full - form.one) * (load - 1);
       const float each = whole * form.full + (rest ? last : 0.0f);
       const float join = splits > 1 ? 0.8f + 0.4f * splits + size * (0.7f + 0.3f * splits) : 0.0f;
-      const float starts = form.at_once == 1 ? whole + (rest != 0) : std::max(1.0f, (float)tiles * splits / room);   // with others at work meanwhile
-      const float cost = form.base * starts + each * ((stages + splits - 1) / splits) + join;
+      const float loads = (float)tiles * splits / num_cu;
+      const float starts = form.at_once == 1 ? whole + (rest != 0) : loads <= 1 ? 1 : 1.6f + 0.4f * std::max(loads - 2, 0.0f);   // with others at work meanwhile
+      const float moves = (bytes - 2) * form.rows * form.cols / 40000.0f * (form.at_once == 1 ? starts : std::max(1.3f * loads, 1.0f));
+      const float cost = form.base * starts + each * ((stages + splits - 1) / splits) + join + moves;
       if ((f == 0 && splits == 1) || cost < least) {
         least = cost;
         best = {f, splits};
@@ -741,13 +747,14 @@ static int mx_launch_stream(tpuhip_ctx *ctx, const MxProductArgs &a, int type) {
 // type: of x's elements, where mx_streams() takes those, or kMxCodes: x is a matrix
 static int mx_multiply(tpuhip_ctx *ctx, const MxProductArgs &a, int type) {
   if (mx_streams(a, type)) return mx_chunks(a) > 8 || a.cols > 128 * ctx->num_cu ? mx_launch_stream<8>(ctx, a, type) : mx_launch_stream<4>(ctx, a, type);
-  const MxChoice c = mx_choose(a.rows, a.cols, a.blocks, ctx->num_cu);
+  const MxChoice c = mx_choose(a.rows, a.cols, a.blocks, mx_size(a.dtype) * (a.residual ? 2 : 1), ctx->num_cu);
   switch (c.form) {
     case 0: return mx_launch_tiles<32, 64, 1, 2, 4>(ctx, a, c.splits);
     case 1: return mx_launch_tiles<64, 64, 2, 2, 4>(ctx, a, c.splits);
     case 2: return mx_launch_tiles<64, 128, 1, 4, 4>(ctx, a, c.splits);
     case 3: return mx_launch_tiles<128, 128, 2, 2, 4>(ctx, a, c.splits);
     case 4: return mx_launch_tiles<128, 128, 2, 2, 2>(ctx, a, c.splits);
+    case 5: return mx_launch_tiles<256, 128, 4, 2, 2>(ctx, a, c.splits);
     default: return mx_launch_tiles<256, 256, 2, 4, 2>(ctx, a, c.splits);
   }
 }
