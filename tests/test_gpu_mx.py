@@ -187,6 +187,19 @@ def test_tiles_of_every_size_come_out_as_they_are_each_time(ctx, rows, cols, n):
         m.free()
 
 
+# a few rows, short sums into many columns: waves in two, four and eight groups, a last column that leaves some without
+@pytest.mark.parametrize("rows,cols", [(1, 40), (3, 512), (16, 224), (2, 700), (1, 1500), (5, 2048), (4, 2040)])
+@pytest.mark.parametrize("n", [8193, 16400, 20001, 33000, 65541])
+def test_few_rows_into_many_columns(ctx, rows, cols, n):
+    x, w, out, want = whole_numbers(ctx, rows, cols, n, n + cols)
+    mx.product(ctx, x, w, out)
+    assert np.array_equal(out.numpy(), want)
+    values = DeviceArray(ctx, (rows, cols), "f32")
+    x.read(values)
+    mx.product(ctx, values, w, out, residual=out)      # blocks' largest numbers may be too small for a scale of 1: still the same values
+    assert np.array_equal(out.numpy(), 2 * want)
+
+
 # long sums, shared by workgroups
 @pytest.mark.parametrize("rows,cols,n", [(1, 16384, 100), (2, 20000, 64), (17, 16384, 200), (40, 16384, 1000), (64, 8192, 4096), (128, 16384, 2048), (16, 30000, 512)])
 def test_long_sums(ctx, rows, cols, n):

@@ -17,6 +17,7 @@ struct MxProductArgs {
   int rows, cols, blocks, dtype;
   FastDiv row_count;
   int depth;                        // numbers of a row, where x is elements; x_stride counts those then
+  int groups;                       // of a workgroup's waves, each with columns of its own: 2^groups
   int splits, split_chunks;         // of the sums over 512 numbers each, among workgroups: of each tile; of them
   float *part;                      // their sums
   int *counters;                    // of each tile: splits that have ended
@@ -100,7 +101,7 @@ __device__ __forceinline__ void mx_put_four(void *y, int64_t row, int n, int col
 }
 // A few rows of x, 16 at most: they lie in LDS as codes while a workgroup goes from 16 columns of y (rows of w) to the next.  Its waves take every
 // so manieth 512 numbers of the sums, a chunk; w comes from memory as it lies, a chunk ahead, whichever columns that belongs to; the waves' sums meet in LDS,
-// added in the waves' order.
+// added in the waves' order.  Where sums are short, groups of waves have columns of their own.
 //   Bound by the reading of w: 65536 columns of 4096 numbers, 143 MB, by a row of float32 take 24.8 us (5.8 TB/s, some of it from the last cache; 29.8
 // with a second chunk ahead, which the compiler moves from register to register and waits for, and 28.5 with biases and residuals asked for before the
 // sums); 4096 columns, 9 MB, 4.3 us, half of that the chain of x, its blocks' scales, w and the sums.
@@ -113,7 +114,7 @@ struct MxRaw {                       // what a lane brings of 512 numbers of a r
   uint4m v[TYPE == TPUHIP_F32 ? 2 : 1];
 };
 
-template <int WAVES, int TYPE>
+template <int WAVES, int TYPE, bool GROUPS>
 __global__ __launch_bounds__(64 * WAVES) void mx_stream_kernel(MxProductArgs a) {
   __shared__ uint4m rows[kMxFewPieces * 17];                   // [chunk][row][17]: 16 blocks of codes, their scales
   __shared__ float4m sums[2][WAVES][64];
@@ -123,6 +124,8 @@ __global__ __launch_bounds__(64 * WAVES) void mx_stream_kernel(MxProductArgs a) 
     uint4m w[4];
     uint32_t s;
   };
+  const int groups = GROUPS ? a.groups : 0, step = (int)gridDim.x << groups;
+  const int per = WAVES >> groups, place = wave & (per - 1), group = (wave << groups) / WAVES;   // waves of a group, which one this is of them
   const auto load = [&](Chunk &c, int tile, int chunk) {
     const int64_t n = min(tile * 16 + r, a.cols - 1);          // past the end, the last row again
     const uint8_t *w = a.w + n * a.w_stride;
@@ -131,17 +134,17 @@ __global__ __launch_bounds__(64 * WAVES) void mx_stream_kernel(MxProductArgs a) 
     c.s = mx_scales(a.ws + n * a.ws_stride, chunk, a.blocks, g);
   };
   Chunk now;
-  int tile = (int)blockIdx.x;
+  int tile = ((int)blockIdx.x << groups) + group;
   // a wave's chunks, of one tile after the other
   const auto load_after = [&](Chunk &c, int &tile, int &chunk) {
-    chunk += WAVES;
+    chunk += per;
     if (chunk >= chunks) {
-      chunk = wave;
-      tile += (int)gridDim.x;
+      chunk = place;
+      tile += step;
     }
     if (tile < tiles) load(c, tile, chunk);
   };
-  int ahead_tile = tile, ahead = wave;
+  int ahead_tile = tile, ahead = place;
   constexpr int BATCH = 4;
   for (int first = wave; first < max(count, 1 + wave); first += BATCH * WAVES) {
     MxRaw<TYPE> raw[BATCH];
@@ -183,7 +186,7 @@ __global__ __launch_bounds__(64 * WAVES) void mx_stream_kernel(MxProductArgs a) 
         }
       }
     }
-    if (first == wave && wave < chunks) load(now, tile, wave);   // behind x, which is waited for first
+    if (first == wave && place < chunks) load(now, tile, place);   // behind x, which is waited for first
 #pragma unroll
     for (int b = 0; b < BATCH; ++b) {
       int m, chunk;
@@ -212,9 +215,9 @@ __global__ __launch_bounds__(64 * WAVES) void mx_stream_kernel(MxProductArgs a) 
   }
   __syncthreads();
   const uint4m *mine = rows + min(r, a.rows - 1) * 17;         // behind the last row it again: its results go nowhere
-  for (int turn = 0; tile < tiles; tile += (int)gridDim.x, ++turn) {
+  for (int turn = 0; tile - group < tiles; tile += step, ++turn) {   // the same number of times for all groups
     float4m acc = {};
-    for (int chunk = wave; chunk < chunks; chunk += WAVES) {
+    for (int chunk = place; chunk < chunks; chunk += per) {
       Chunk next;
       load_after(next, ahead_tile, ahead);
       const uint4m *x = mine + chunk * a.rows * 17;
@@ -228,10 +231,13 @@ __global__ __launch_bounds__(64 * WAVES) void mx_stream_kernel(MxProductArgs a) 
     sums[turn & 1][wave][lane] = acc;
     __syncthreads();
     // a wave adds them up while the others go on; it is there again before they are written the time after the next
-    if (wave == turn % WAVES) {
-      float4m v = sums[turn & 1][0][lane];
+    if (place == (turn & (per - 1))) {
+      float4m v = sums[turn & 1][wave - place][lane];
 #pragma unroll
-      for (int i = 1; i < WAVES; ++i) v += sums[turn & 1][i][lane];
+      for (int i = 1; i < WAVES; ++i) {
+        const float4m more = sums[turn & 1][(wave - place + i) % WAVES][lane];
+        if (i < per) v += more;
+      }
       const int n = tile * 16 + g * 4;
       if (r < a.rows && n < a.cols) {
         float4m bias = {}, residual = {};
@@ -733,13 +739,19 @@ static bool mx_streams(const MxProductArgs &a, int type) {
 }
 
 // Up to two workgroups a CU, each of which goes from columns to columns: of 16384 columns one row takes 9.1 us so, 10.0 with four a CU.  Eight waves
-// where sums are long (16384 numbers: 10.7 us, with four 12.3) or columns many (65536: 26.6 and 30.1), otherwise four (4096 x 4096: 4.7 us, with eight 5.0).
+// where sums are long (16384 numbers: 10.7 us, with four 12.3) or columns many (65536: 24.8 and 30.1), otherwise four (4096 x 4096: 4.3 us, with eight 4.6).
+// Groups where some waves would have nothing and there are columns for all: 3 rows x 224 x 44346 4.5 us, with one group 7.2; 4 x 512 x 65536 5.8 and 8.5.
 template <int WAVES>
-static int mx_launch_stream(tpuhip_ctx *ctx, const MxProductArgs &a, int type) {
-  const int64_t tiles = ceil_div64(a.cols, 16), turns = ceil_div64(tiles, 2 * ctx->num_cu);
-  const auto kernel = type == kMxCodes ? mx_stream_kernel<WAVES, kMxCodes> : type == TPUHIP_BF16 ? mx_stream_kernel<WAVES, TPUHIP_BF16>
-                      : type == TPUHIP_F16 ? mx_stream_kernel<WAVES, TPUHIP_F16> : mx_stream_kernel<WAVES, TPUHIP_F32>;
-  launch(ctx, kernel, dim3((unsigned)ceil_div64(tiles, turns)), dim3(64 * WAVES), a);
+static int mx_launch_stream(tpuhip_ctx *ctx, MxProductArgs a, int type) {
+  const int64_t columns = ceil_div64(a.cols, 16);
+  while (mx_chunks(a) << (a.groups + 1) <= WAVES && columns > (int64_t)2 * ctx->num_cu << a.groups) ++a.groups;
+  const int64_t tiles = ceil_div64(columns, 1 << a.groups), turns = ceil_div64(tiles, 2 * ctx->num_cu);
+  const auto kernel = [&](auto groups) {
+    constexpr bool GROUPS = decltype(groups)::value;
+    return type == kMxCodes ? mx_stream_kernel<WAVES, kMxCodes, GROUPS> : type == TPUHIP_BF16 ? mx_stream_kernel<WAVES, TPUHIP_BF16, GROUPS>
+           : type == TPUHIP_F16 ? mx_stream_kernel<WAVES, TPUHIP_F16, GROUPS> : mx_stream_kernel<WAVES, TPUHIP_F32, GROUPS>;
+  };
+  launch(ctx, a.groups ? kernel(std::true_type{}) : kernel(std::false_type{}), dim3((unsigned)ceil_div64(tiles, turns)), dim3(64 * WAVES), a);
   TPUHIP_CHECK_HIP(hipGetLastError());
   return TPUHIP_OK;
 }
