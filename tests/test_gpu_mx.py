@@ -150,8 +150,9 @@ def test_every_code_and_scale_is_read_as_it_stands(ctx):
         assert np.array_equal(out.numpy().astype(np.float32), want, equal_nan=True)
 
 
-SHAPES = [(1, 1, 1), (1, 32, 16), (1, 4096, 100), (2, 33, 17), (3, 512, 1000), (5, 2050, 33), (8, 4096, 130), (4, 8197, 40), (16, 2000, 50), (16, 100, 64), (17, 64, 65), (31, 1000, 130), (48, 4096, 48),
-          (64, 512, 257), (65, 300, 64), (130, 2050, 70), (200, 640, 333), (257, 1024, 512), (300, 2080, 999)]
+SHAPES = [(1, 1, 1), (1, 32, 16), (1, 4096, 100), (2, 33, 17), (3, 512, 1000), (5, 2050, 33), (8, 4096, 130), (4, 8197, 40), (16, 2000, 50),
+          (16, 100, 64), (17, 64, 65), (31, 1000, 130), (48, 4096, 48), (64, 512, 257), (65, 300, 64), (130, 2050, 70), (200, 640, 333),
+          (257, 1024, 512), (300, 2080, 999)]
 
 
 @pytest.mark.parametrize("rows,cols,n", SHAPES)

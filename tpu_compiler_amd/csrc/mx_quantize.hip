@@ -100,7 +100,8 @@ static int mx_rows(tpuhip_ctx *ctx, const tpuhip_mx_matrix *m, const void *x, in
   if (m->rows == 0) return TPUHIP_OK;
   MxRowsArgs a{};
   const int64_t blocks = (int64_t)m->rows * mx_blocks(m->cols);
-  TPUHIP_REQUIRE(ceil_div64(blocks, kMxThreads / kMxThreadsBlock) <= UINT32_MAX / kMxThreads, "%s: %d rows of %d columns in one call", what, m->rows, m->cols);   // a launch has fewer than 2^32 threads
+  TPUHIP_REQUIRE(ceil_div64(blocks, kMxThreads / kMxThreadsBlock) <= UINT32_MAX / kMxThreads,   // a launch has fewer than 2^32 threads
+                 "%s: %d rows of %d columns in one call", what, m->rows, m->cols);
   a.codes = (uint8_t *)m->codes;
   a.scales = (uint8_t *)m->scales;
   a.x = const_cast<void *>(x);
