@@ -102,7 +102,8 @@ class _Linear(_Plan):
 def plan_product(ctx, x, w, out, bias=None, residual=None):
     """A call that computes out = x w^T (+ bias) (+ residual).  w: an MXMatrix [columns of out, k]; x: one too, [rows of out, k], or an array of
     bf16, f16 or f32, which the call quantises (in memory that the plan keeps).  out, residual (may be out): bf16, f16 or f32, [rows, columns]; bias:
-    f32, [columns].  out shares memory with nothing else that the call reads."""
+    f32, [columns].  out shares memory with nothing else that the call reads.  A plan that quantises is made before a recording, not in it: it may
+    need memory."""
     if not isinstance(w, MXMatrix):
         _refuse("w: no MXMatrix")
     if not isinstance(x, MXMatrix) and len(x.shape) != 2:
