@@ -67,21 +67,24 @@ class MXMatrix:
 
 
 class _Room:
-    """Memory in which a call quantises x.  It is its context's, and goes from a plan that nobody holds to the next one that it is large enough for:
-    calls on one context follow each other, and freeing it would wait for them, which nothing may do while they are recorded."""
+    """Memory in which a call quantises x.  It is its context's, and goes from a plan that nobody holds to the next one of its size: calls on one
+    context follow each other, and freeing it would wait for them, which nothing may do while they are recorded.  Sizes are powers of two, so that
+    products of any lengths come to hold four times what the largest need at most, for as many of them as there are at a time; a plan takes no larger
+    one than its own, as it may stay for good."""
+    SMALLEST = 4096
 
     def __init__(self, ctx, nbytes):
         self.array, self.taken = DeviceArray(ctx, (nbytes,), "u8"), True
 
     @classmethod
     def take(cls, ctx, nbytes):
-        fits = [r for r in ctx.rooms if not r.taken and r.array.nbytes >= nbytes]
-        if fits:
-            r = min(fits, key=lambda r: r.array.nbytes)
-            r.taken = True
-        else:
-            r = cls(ctx, nbytes)
-            ctx.rooms.append(r)
+        size = max(cls.SMALLEST, 1 << (nbytes - 1).bit_length())
+        for r in ctx.rooms:
+            if not r.taken and r.array.nbytes == size:
+                r.taken = True
+                return r
+        r = cls(ctx, size)
+        ctx.rooms.append(r)
         return r
 
     def free(self):
