@@ -715,11 +715,7 @@ static int mx_launch_tiles(tpuhip_ctx *ctx, MxProductArgs a, int splits) {
   const int64_t tiles = ceil_div64(a.rows, BM) * ceil_div64(a.cols, BN);
   TPUHIP_REQUIRE(tiles <= UINT32_MAX / (64 * WM * WN), "a product of %d rows and %d columns in one call", a.rows, a.cols);   // a launch has fewer than 2^32 threads
   const int chunks = (a.blocks + 15) / 16;
-  if (splits > 1 && (tiles > kCounters || tiles * splits * BM * BN * 4 > (int64_t)kJoinBytes)) splits = 1;
-  if (splits > 1) {
-    if (int rc = attention_workspace(ctx)) return rc;
-    if (!ctx->join) splits = 1;
-  }
+  if (splits > 1 && (!ctx->join || tiles > kCounters || tiles * splits * BM * BN * 4 > (int64_t)kJoinBytes)) splits = 1;
   a.split_chunks = (int)ceil_div64(chunks, splits);
   a.splits = (int)ceil_div64(chunks, a.split_chunks);
   a.counters = (int *)ctx->join;
@@ -758,6 +754,8 @@ static int mx_launch_stream(tpuhip_ctx *ctx, MxProductArgs a, int type) {
 
 // type: of x's elements, where mx_streams() takes those, or kMxCodes: x is a matrix
 static int mx_multiply(tpuhip_ctx *ctx, const MxProductArgs &a, int type) {
+  // with any product, not with the first in parts: that one may be recorded, and would be in one part where the same call by itself is in several
+  if (int rc = attention_workspace(ctx)) return rc;
   if (mx_streams(a, type)) return mx_chunks(a) > 8 || a.cols > 128 * ctx->num_cu ? mx_launch_stream<8>(ctx, a, type) : mx_launch_stream<4>(ctx, a, type);
   const MxChoice c = mx_choose(a.rows, a.cols, a.blocks, mx_size(a.dtype) * (a.residual ? 2 : 1), ctx->num_cu);
   switch (c.form) {
