@@ -636,7 +636,8 @@ typedef struct {
   void *codes, *scales;
   int64_t codes_stride, scales_stride;   /* bytes */
 } tpuhip_mx_matrix;
-/* x [rows, cols] of TPUHIP_BF16, TPUHIP_F16 or TPUHIP_F32, rows x_stride elements apart, a row's numbers next to each other */
+/* x [rows, cols] of TPUHIP_BF16, TPUHIP_F16 or TPUHIP_F32, rows x_stride elements apart, a row's numbers next to each other; it shares no memory with the
+ * matrix, here and below */
 int tpuhip_mx_quantize(tpuhip_ctx *ctx, const tpuhip_mx_matrix *m, const void *x, int dtype, int64_t x_stride);
 /* the numbers that a matrix stands for, rounded once to the type */
 int tpuhip_mx_read(tpuhip_ctx *ctx, const tpuhip_mx_matrix *m, void *x, int dtype, int64_t x_stride);

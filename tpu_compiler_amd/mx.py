@@ -3,7 +3,7 @@ HIP library; nothing here computes.
 
 Arrays are device memory as kv_cache takes it: DeviceArray, or anything that has torch's data_ptr(), shape, stride() and dtype."""
 from . import capi
-from .kv_cache import TYPES, DeviceArray, _device, _int, _Plan, _refuse, _type
+from .kv_cache import _SIZES, TYPES, DeviceArray, _device, _int, _Plan, _refuse, _type
 
 BLOCK = 32
 
@@ -17,6 +17,33 @@ def _rows2(x, what, ctx, rows, cols):
     if cols > 1 and st[1] != 1:
         _refuse("%s: the numbers of a row lie %d apart" % (what, st[1]))
     return int(st[0]) if rows > 1 else cols
+
+
+def _meet(a, b):
+    """whether rows of bytes share any: (address, rows, their distance, bytes of one)"""
+    once = (s if s[2] else (s[0], 1, 1, s[3]) for s in (a, b))
+    (at_a, rows_a, step_a, width_a), (at_b, rows_b, step_b, width_b) = sorted(once, key=lambda s: s[1])
+    last_a = at_a + (rows_a - 1) * step_a
+    if last_a + width_a <= at_b or at_b + (rows_b - 1) * step_b + width_b <= at_a:
+        return False
+    if step_a == step_b:                             # then row i of one and row j of the other lie as any others with the same i - j do
+        first = at_a - at_b
+        k = min((width_b - 1 - first) // step_a, rows_a - 1)
+        return k > -rows_b and first + k * step_a > -width_a
+    # the last row of b that begins before a's row ends
+    return any(at_b + min((at + width_a - 1 - at_b) // step_b, rows_b - 1) * step_b + width_b > at
+               for at in range(at_a, last_a + 1, step_a) if at + width_a > at_b)
+
+
+def _apart(x, y, what):
+    """Refuses x where it shares memory with y.  Tensors of torch's may be views of one memory; a DeviceArray's is its own, and what else there is
+    does not say."""
+    def span(a):
+        size, rows = _SIZES[_type(a, what, tuple(_SIZES))], a.shape[0] if len(a.shape) == 2 else 1
+        return a.data_ptr(), rows, a.stride()[0] * size if rows > 1 else 1, a.shape[-1] * size
+
+    if x is y or (all(getattr(a, "device", None) is not None and all(a.shape) for a in (x, y)) and _meet(span(x), span(y))):
+        _refuse(what)
 
 
 class MXMatrix:
@@ -42,9 +69,10 @@ class MXMatrix:
         return self.rows * self.blocks * 17
 
     def _plan(self, fn, x, what):
-        dtype = _type(x, what, tuple(TYPES))
-        return _Plan(self.ctx, fn, (self._d, x.data_ptr(), TYPES[dtype], _rows2(x, what, self.ctx, self.rows, self.cols)),
-                     (self.codes, self.scales, x))
+        dtype, stride = _type(x, what, tuple(TYPES)), _rows2(x, what, self.ctx, self.rows, self.cols)
+        for own in (self.codes, self.scales):
+            _apart(x, own, "%s in the place of the matrix" % what)
+        return _Plan(self.ctx, fn, (self._d, x.data_ptr(), TYPES[dtype], stride), (self.codes, self.scales, x))
 
     def plan_quantize(self, x):
         """a call that quantises x [rows, cols], bf16, f16 or f32, into this matrix"""
@@ -105,8 +133,8 @@ class _Linear(_Plan):
 def plan_product(ctx, x, w, out, bias=None, residual=None):
     """A call that computes out = x w^T (+ bias) (+ residual).  w: an MXMatrix [columns of out, k]; x: one too, [rows of out, k], or an array of
     bf16, f16 or f32, which the call quantises (in memory that the plan keeps).  out, residual (may be out): bf16, f16 or f32, [rows, columns]; bias:
-    f32, [columns].  out shares memory with nothing else that the call reads.  A plan that quantises is made before a recording, not in it: it may
-    need memory."""
+    f32, [columns].  out shares memory with nothing else that the call reads (checked of torch's tensors, which may be views of one memory).  A plan
+    that quantises is made before a recording, not in it: it may need memory."""
     if not isinstance(w, MXMatrix):
         _refuse("w: no MXMatrix")
     if not isinstance(x, MXMatrix) and len(x.shape) != 2:
@@ -114,27 +142,32 @@ def plan_product(ctx, x, w, out, bias=None, residual=None):
     rows, k = (x.rows, x.cols) if isinstance(x, MXMatrix) else (_int(x.shape[0], "rows"), int(x.shape[1]))
     if k != w.cols:
         _refuse("x has %d columns, w %d" % (k, w.cols))
-    if x is out:
-        _refuse("out in the place of x")
     for m in (x, w):
         if isinstance(m, MXMatrix) and m.ctx.device != ctx.device:
             _refuse("a matrix lies on device %d, the context works on device %d" % (m.ctx.device, ctx.device))
     dtype = _type(out, "out", tuple(TYPES))
+    if not isinstance(x, MXMatrix):
+        stride, x_type = _rows2(x, "x", ctx, rows, k), _type(x, "x", tuple(TYPES))
     d = capi.MXProductDesc(TYPES[dtype], _rows2(out, "out", ctx, rows, w.rows), 0, None, None)
+    for a, what in ((x, "x"), (w, "w")):
+        for part in (a.codes, a.scales) if isinstance(a, MXMatrix) else (a,):
+            _apart(out, part, "out in the place of %s" % what)
     if bias is not None:
         _device(bias, "bias", ctx)
         _type(bias, "bias", ("f32",))
         if tuple(bias.shape) != (w.rows,) or (w.rows > 1 and bias.stride()[0] != 1):
             _refuse("bias: %d numbers in a row are wanted, not %s" % (w.rows, tuple(bias.shape)))
+        _apart(out, bias, "out in the place of the bias")
         d.bias = bias.data_ptr()
     if residual is not None:
         if _type(residual, "residual", tuple(TYPES)) != dtype:
             _refuse("out and residual: of one type")
         d.residual, d.residual_stride = residual.data_ptr(), _rows2(residual, "residual", ctx, rows, w.rows)
+        if d.residual != out.data_ptr() or d.residual_stride != d.y_stride:
+            _apart(out, residual, "out neither in the residual's place nor apart from it")
     keep = (w.codes, w.scales, out, bias, residual)
     if isinstance(x, MXMatrix):
         return _Plan(ctx, ctx.lib.tpuhip_mx_product, (d, x._d, w._d, out.data_ptr()), keep + (x.codes, x.scales))
-    stride, x_type = _rows2(x, "x", ctx, rows, k), _type(x, "x", tuple(TYPES))
     codes, scales = -(-w.blocks // 8) * 128, -(-w.blocks // 16) * 16      # rows that begin at lines of the caches
     room = _Room.take(ctx, rows * (codes + scales))
     at = room.array.data_ptr()
