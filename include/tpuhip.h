@@ -613,7 +613,7 @@ int tpuhip_kv_pages_grow(tpuhip_ctx *ctx, const tpuhip_kv_pages *pages, const in
                          int32_t *slots, int32_t *refused);
 /* keep[b] tokens of sequence b stay (all, if it has no more; none if negative): the end of a draft, or of a sequence.  The pages behind them are
  * free, their entries of the table -1, and the stack is as if they had never been taken: the next to grow get the same ones in the
- * same order.  The rows of what stays are as they were. */
+ * same order.  The rows of what stays are as they were.  keep shares no memory with the batch's arrays. */
 int tpuhip_kv_pages_trim(tpuhip_ctx *ctx, const tpuhip_kv_pages *pages, const int32_t *keep);
 
 /* ---- Microscaled 4-bit floating point ----------------------------------------
@@ -643,9 +643,11 @@ int tpuhip_mx_quantize(tpuhip_ctx *ctx, const tpuhip_mx_matrix *m, const void *x
 int tpuhip_mx_read(tpuhip_ctx *ctx, const tpuhip_mx_matrix *m, void *x, int dtype, int64_t x_stride);
 
 /* y = x w^T (+ bias) (+ residual): x has y's rows, w a row for each of y's columns, both as many columns.  bias: float32, one a column of y, or
- * NULL; residual: like y, of its type, or NULL, and may be y itself; y shares memory with nothing else that a call reads.  Products are exact and summed in 32 bits (terms below 2^-126 may
- * count as 0), and what the sum, the bias and the residual come to is rounded once.  The order of the sums depends on sizes alone, unless
- * a context has no memory for partial sums (it gets it with its first product or cache outside of a recording). */
+ * NULL; residual: like y, of its type, or NULL, and may be y itself, with y's stride; y shares memory with nothing else that a call reads.  Products are
+ * exact and summed in 32 bits (terms below 2^-126 may count as 0), and what the sum, the bias and the residual come to is rounded once.  The order
+ * of the sums depends on the sizes, on whether x is in 4 bits or quantised in the call, on y's type, on whether there is a residual and on the
+ * device's number of CUs: the same call gives the same bits, and one that differs in any of these may differ by what sums in 32 bits do.  A
+ * context without memory for partial sums has another order as well; it gets that memory with its first product or cache outside of a recording. */
 typedef struct {
   int dtype;                          /* of y and residual: TPUHIP_BF16, TPUHIP_F16 or TPUHIP_F32 */
   int64_t y_stride, residual_stride;  /* elements */

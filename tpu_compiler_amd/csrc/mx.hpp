@@ -99,8 +99,8 @@ __device__ __forceinline__ void mx_load8(const void *x, int64_t i, int dtype, fl
     }
   }
 }
-// ONCE: past the L2 as far as that goes, which operands need more.  Large products end their tiles at the same time: 8192 x 8192 x 8192 take 266 us so,
-// and 276 otherwise.
+// ONCE: past the L2 as far as that goes, which operands need more.  Large products end their tiles at the same time: 8192 x 8192 x 8192 took 266 us so
+// and 276 otherwise, in turn on one card.
 template <bool ONCE = false>
 __device__ __forceinline__ void mx_store4(void *x, int64_t i, int dtype, float4m v) {
   if (dtype == TPUHIP_F32) {

@@ -258,8 +258,8 @@ __global__ __launch_bounds__(64 * WAVES) void mx_stream_kernel(MxProductArgs a) 
 // same array, and one to an array that has none for all of them.
 //   Bound by what a CU takes in: a small tile's rows of both operands come at 48 of 64 bytes a clock, with the scales, 16 bytes of a line each, more.
 // Without a stage's products, or its reads, 64 x 64 tiles take as long (sums of 16384 numbers, 64 rows: 18.7 us; 14.7 without the scales, 11.5 without
-// the data).  256 x 256 are bound by products: 8192 x 8192 x 8192 take 266 us, 4.1 PFLOP/s, at a clock of 1.6 GHz that the power leaves (products of registers alone,
-// of random numbers: 6.2 PFLOP/s; 231 us without loads, 253 without results).
+// the data).  256 x 256 are bound by products: 8192 x 8192 x 8192 take 282 to 292 us on different cards, 3.8 PFLOP/s, and 270 at best, at a clock of 1.6 GHz
+// that the power leaves (products of registers alone, of random numbers: 6.2 PFLOP/s; on a card that took 266 us, 231 without loads, 253 without results).
 constexpr int kMxStage = 8;   // blocks of a stage
 
 typedef __attribute__((address_space(3))) uint8_t mx_lds;
@@ -667,7 +667,9 @@ static int mx_product_args(tpuhip_ctx *ctx, const tpuhip_mx_product_desc *d, con
 //   128 x 128   32 .. 256       12.2  17.5 | 12.5 15.4
 //   128 x 128   128 .. 256      15.0  18.2 | 16.7 17.5    512  28.4 | 28.8     1032  60.4 | 62.8
 //   256 x 128   32 .. 256       19.1  25.3 | 19.5 24.0    688  68.0 | 70.3
-//   256 x 256   64 .. 256       29.9  43.0 | 29.7 42.3    688  115  | 121      1024 (32 stages)  266 | 300
+//   256 x 256   64 .. 256       29.9  43.0 | 29.7 42.3    688  115  | 121      1024 (32 stages)  282 | 300
+// Over 156 sizes of bfloat16 results what is chosen takes 1.2 % more than the quickest form in the mean and 15.5 % at the worst, with results of
+// float32, biases and residuals 1.5 % and 28.6 %.
 struct MxForm {
   int rows, cols, at_once;
   float base, low, one, full;

@@ -13,9 +13,9 @@ struct MxRowsArgs {
 };
 
 // Four threads a block, eight numbers each: one or two loads of 16 bytes, a wave's next to each other, and two exchanges between neighbouring lanes for
-// the block's largest size.  Bound by memory: 8192 x 8192 of bfloat16, 170 MB, are quantised in 29.7 us (5.7 TB/s, some of it from the last cache) and
-// read back in 26.4; 4999 x 2050 of float32, parts of longer rows that begin anywhere, 46 MB, take 9.6 and 10.3 us; a row of 4096 1.5 and 1.7,
-// latency.
+// the block's largest size.  Bound by memory: 8192 x 8192 of bfloat16, 170 MB, are quantised in 31 us (5.5 TB/s, some of it from the last cache), 37
+// where the caches are full of another kernel's results, and read back in 27; 4999 x 2050 of float32, parts of longer rows that begin anywhere, 46 MB, take
+// 9.4 and 11.6 us; a row of 4096 1.5 and 1.9, latency.
 constexpr int kMxThreads = 256, kMxThreadsBlock = 4;
 
 __global__ __launch_bounds__(kMxThreads) void mx_quantize_kernel(MxRowsArgs a) {
