@@ -75,3 +75,12 @@ def test_a_room_is_large_enough_and_one_plan_s_at_a_time(ctx):
     rooms = [p._room for p in plans]
     assert len(set(map(id, rooms))) == len(rooms)
     assert all(r.array.nbytes >= need(w, p._keep[2].shape[0]) for r, p in zip(rooms, plans))
+
+
+def test_a_matrix_of_the_caller_s_arrays_has_nothing_to_free(ctx):
+    """a tensor of torch's is freed when nobody holds it"""
+    weights(ctx, 64, 700).free()
+    assert "tpuhip_free" not in ctx.lib.names()
+    own = mx.MXMatrix(ctx, 64, 700)
+    own.free()
+    assert ctx.lib.names().count("tpuhip_free") == 2

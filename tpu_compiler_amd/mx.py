@@ -90,8 +90,10 @@ class MXMatrix:
         self.plan_read(out)()
 
     def free(self):
+        """frees its DeviceArrays; other arrays are their owners'"""
         for a in (self.codes, self.scales):
-            a.free()
+            if isinstance(a, DeviceArray):
+                a.free()
 
 
 class _Room:
