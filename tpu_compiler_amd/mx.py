@@ -19,30 +19,32 @@ def _rows2(x, what, ctx, rows, cols):
     return int(st[0]) if rows > 1 else cols
 
 
+def _span(x, dtype, rows, cols, stride):
+    """an array and where its rows lie: (address, rows, their distance, bytes of one); an address of None if nothing else can lie there.  Tensors of torch's may
+    be views of one memory; a DeviceArray's is its own, and what else there is does not say."""
+    size = _SIZES[dtype]
+    return x, (x.data_ptr() if rows and getattr(x, "device", None) is not None else None, rows, stride * size, cols * size)
+
+
 def _meet(a, b):
-    """whether rows of bytes share any: (address, rows, their distance, bytes of one)"""
-    once = (s if s[2] else (s[0], 1, 1, s[3]) for s in (a, b))
-    (at_a, rows_a, step_a, width_a), (at_b, rows_b, step_b, width_b) = sorted(once, key=lambda s: s[1])
-    last_a = at_a + (rows_a - 1) * step_a
-    if last_a + width_a <= at_b or at_b + (rows_b - 1) * step_b + width_b <= at_a:
+    """whether rows share bytes"""
+    (at_a, rows_a, step_a, width_a), (at_b, rows_b, step_b, width_b) = a, b
+    if at_a + (rows_a - 1) * step_a + width_a <= at_b or at_b + (rows_b - 1) * step_b + width_b <= at_a:
         return False
+    once = (s if s[1] > 1 and s[2] else (s[0], 1, 1, s[3]) for s in (a, b))
+    (at_a, rows_a, step_a, width_a), (at_b, rows_b, step_b, width_b) = sorted(once, key=lambda s: s[1])
     if step_a == step_b:                             # then row i of one and row j of the other lie as any others with the same i - j do
         first = at_a - at_b
         k = min((width_b - 1 - first) // step_a, rows_a - 1)
         return k > -rows_b and first + k * step_a > -width_a
     # the last row of b that begins before a's row ends
     return any(at_b + min((at + width_a - 1 - at_b) // step_b, rows_b - 1) * step_b + width_b > at
-               for at in range(at_a, last_a + 1, step_a) if at + width_a > at_b)
+               for at in range(at_a, at_a + (rows_a - 1) * step_a + 1, step_a) if at + width_a > at_b)
 
 
 def _apart(x, y, what):
-    """Refuses x where it shares memory with y.  Tensors of torch's may be views of one memory; a DeviceArray's is its own, and what else there is
-    does not say."""
-    def span(a):
-        size, rows = _SIZES[_type(a, what, tuple(_SIZES))], a.shape[0] if len(a.shape) == 2 else 1
-        return a.data_ptr(), rows, a.stride()[0] * size if rows > 1 else 1, a.shape[-1] * size
-
-    if x is y or (all(getattr(a, "device", None) is not None and all(a.shape) for a in (x, y)) and _meet(span(x), span(y))):
+    """refuses the span x where it shares memory with y"""
+    if x[0] is y[0] or (x[1][0] is not None and y[1][0] is not None and _meet(x[1], y[1])):
         _refuse(what)
 
 
@@ -62,6 +64,7 @@ class MXMatrix:
         self.codes, self.scales = codes, scales
         _type(codes, "codes", ("u8",)), _type(scales, "scales", ("u8",))
         strides = [_rows2(codes, "codes", ctx, self.rows, 16 * self.blocks), _rows2(scales, "scales", ctx, self.rows, self.blocks)]
+        self._spans = [_span(x, "u8", self.rows, width, stride) for x, width, stride in zip((codes, scales), (16 * self.blocks, self.blocks), strides)]
         self._d = capi.MXMatrixDesc(self.rows, self.cols, codes.data_ptr(), scales.data_ptr(), *strides)
 
     @property
@@ -70,8 +73,8 @@ class MXMatrix:
 
     def _plan(self, fn, x, what):
         dtype, stride = _type(x, what, tuple(TYPES)), _rows2(x, what, self.ctx, self.rows, self.cols)
-        for own in (self.codes, self.scales):
-            _apart(x, own, "%s in the place of the matrix" % what)
+        for own in self._spans:
+            _apart(_span(x, dtype, self.rows, self.cols, stride), own, "%s in the place of the matrix" % what)
         return _Plan(self.ctx, fn, (self._d, x.data_ptr(), TYPES[dtype], stride), (self.codes, self.scales, x))
 
     def plan_quantize(self, x):
@@ -151,22 +154,24 @@ def plan_product(ctx, x, w, out, bias=None, residual=None):
     if not isinstance(x, MXMatrix):
         stride, x_type = _rows2(x, "x", ctx, rows, k), _type(x, "x", tuple(TYPES))
     d = capi.MXProductDesc(TYPES[dtype], _rows2(out, "out", ctx, rows, w.rows), 0, None, None)
-    for a, what in ((x, "x"), (w, "w")):
-        for part in (a.codes, a.scales) if isinstance(a, MXMatrix) else (a,):
-            _apart(out, part, "out in the place of %s" % what)
+    here = _span(out, dtype, rows, w.rows, d.y_stride)
+    for part in x._spans if isinstance(x, MXMatrix) else (_span(x, x_type, rows, k, stride),):
+        _apart(here, part, "out in the place of x")
+    for part in w._spans:
+        _apart(here, part, "out in the place of w")
     if bias is not None:
         _device(bias, "bias", ctx)
         _type(bias, "bias", ("f32",))
         if tuple(bias.shape) != (w.rows,) or (w.rows > 1 and bias.stride()[0] != 1):
             _refuse("bias: %d numbers in a row are wanted, not %s" % (w.rows, tuple(bias.shape)))
-        _apart(out, bias, "out in the place of the bias")
+        _apart(here, _span(bias, "f32", 1, w.rows, 0), "out in the place of the bias")
         d.bias = bias.data_ptr()
     if residual is not None:
         if _type(residual, "residual", tuple(TYPES)) != dtype:
             _refuse("out and residual: of one type")
         d.residual, d.residual_stride = residual.data_ptr(), _rows2(residual, "residual", ctx, rows, w.rows)
         if d.residual != out.data_ptr() or d.residual_stride != d.y_stride:
-            _apart(out, residual, "out neither in the residual's place nor apart from it")
+            _apart(here, _span(residual, dtype, rows, w.rows, d.residual_stride), "out neither in the residual's place nor apart from it")
     keep = (w.codes, w.scales, out, bias, residual)
     if isinstance(x, MXMatrix):
         return _Plan(ctx, ctx.lib.tpuhip_mx_product, (d, x._d, w._d, out.data_ptr()), keep + (x.codes, x.scales))
